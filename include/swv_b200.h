@@ -51,7 +51,7 @@ extern "C" {
 #define SWV_F16 2
 
 /* Library ABI version (major*100 + minor).  103: swv_block_sparse_attn_ws_fwd, swv_dsa_module_bwd and their size
- * queries. */
+ * queries; 104: swv_layer_norm_*, swv_rope_axes_apply, swv_packed_attn_*. */
 int swv_version(void);
 
 /* Text for a negative return code or a positive device status code. */
@@ -399,6 +399,59 @@ int swv_nsa_attn_fwd(const void* q, const int64_t q_strides[4], const void* k, c
 int swv_rope2d_apply(const void* x, const int64_t x_strides[3], void* y, const int64_t y_strides[3], int dtype,
                      const float* coords, int64_t L, int H, int head_dim, float coord_high, float theta,
                      int skip_tokens, void* stream);
+
+/* Layer norm over the last dimension of N rows of E values (nn.LayerNorm; every block of the reference's encoders has
+ * two, M:108-166).  mu and 1/sqrt(var + eps) of every row go to `mean`, `rstd` (N) f32 (both or neither; the
+ * backward pass needs them); w and b (E) may be NULL (1 and 0).  Rows x_stride / y_stride / ... elements apart, unit
+ * inner stride.  x of any dtype; y (and dy) of x's dtype or SWV_F32, and of any dtype where x is SWV_F32; dx of
+ * x's dtype; w, b, dw, db each of any dtype.
+ * Backward: dx (N,E), dw and db (E), either may be NULL.  `workspace`: swv_layer_norm_bwd_bytes(), only for dw, db. */
+int swv_layer_norm_fwd(const void* x, int64_t x_stride, int x_dtype, const void* w, int w_dtype, const void* b,
+                       int b_dtype, void* y, int64_t y_stride, int y_dtype, float* mean, float* rstd, int64_t N, int E,
+                       float eps, void* stream);
+int swv_layer_norm_bwd_bytes(int64_t N, int E, size_t* bytes);
+int swv_layer_norm_bwd(const void* dy, int64_t dy_stride, int y_dtype, const void* x, int64_t x_stride, int x_dtype,
+                       const void* w, int w_dtype, const float* mean, const float* rstd, void* dx, int64_t dx_stride,
+                       void* dw, int dw_dtype, void* db, int db_dtype, int64_t N, int E, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Rotary positions with several axes (the rotation of swv_rope2d_apply, rope.py:33-37, for up to 8 axes).  Pair i
+ * of the `pairs` rotated pairs of every head turns by  position[t][axis[i]] * freq[i]  (`inverse`: by minus that, the
+ * gradient); the pairs are channels (2i, 2i+1), or with `halves` (i, pairs + i); the channels from 2*pairs on are
+ * copied.  The angle is formed in 64 bits.  freq_host (pairs) f64 and axis_host (pairs) u8 are HOST arrays, read during
+ * the call; pairs <= 128.
+ *   x, y (T,H,head_dim): strides (t,h,d) with unit inner stride, y may be x;  positions (T,axes) of pos_dtype, rows
+ *   pos_stride elements apart. */
+#define SWV_POS_F32 0
+#define SWV_POS_I32 1
+#define SWV_POS_I64 2
+int swv_rope_axes_apply(const void* x, const int64_t x_strides[3], void* y, const int64_t y_strides[3], int dtype,
+                        const void* positions, int pos_dtype, int64_t pos_stride, const double* freq_host,
+                        const uint8_t* axis_host, int pairs, int axes, int halves, int inverse, int64_t T, int H,
+                        int head_dim, void* stream);
+
+/* Attention over packed sequences (dense softmax attention inside each of n_seq sequences that lie one behind the
+ * other; for one sequence F.scaled_dot_product_attention of the reference's dense ViT-5, models_vit5.py:101).
+ * Query head h reads key head h / (H / Hkv), H / Hkv <= 128.  Causal: query i of a sequence of lq queries and lk keys
+ * sees the keys j <= i + lk - lq.  A row that sees no key gives zeros and lse = -inf.
+ *
+ * swv_packed_plan turns the lengths (HOST arrays) into the kernels' work tables: one int32 HOST array that the caller
+ * copies to the device; both copies are passed to every call.  *bytes (may be NULL) gets its size, also when `plan` is
+ * NULL or too small (SWV_ERR_WORKSPACE).  At most 2^29 tokens.
+ *
+ *   q, o, dq, d_out (Tq,H,D), k, v, dk, dv (Tk,Hkv,D) bf16: strides (t,h,d), unit inner stride, rows on 16 bytes;
+ *   D a multiple of 8 up to 128; Tq, Tk at least the plan's tokens: rows behind them are neither read nor written;
+ *   lse (H,Tq) f32, natural logarithm of each row's sum of exponentials, NULL if not wanted (the backward pass
+ *   takes it); scale > 0; `workspace` of swv_packed_attn_bytes() / swv_packed_attn_bwd_bytes(), 16-byte aligned.
+ * Inside one sequence a NaN or an infinity in a value row can reach earlier (causally masked) queries whose key tiles
+ * hold that row; other sequences it never reaches. */
+int swv_packed_plan(int n_seq, const int64_t* q_lens_host, const int64_t* k_lens_host, int H, int Hkv, int causal,
+                    int32_t* plan_host, size_t plan_bytes, size_t* bytes);
+int swv_packed_attn_bytes(const int32_t* plan_host, int D, size_t* bytes);
+int swv_packed_attn_fwd(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                        const void* v, const int64_t v_strides[3], void* o, const int64_t o_strides[3], float* lse,
+                        const int32_t* plan_host, const int32_t* plan, int64_t Tq, int64_t Tk, int D, float scale,
+                        void* workspace, size_t workspace_bytes, int* status, void* stream);
 
 #ifdef __cplusplus
 }

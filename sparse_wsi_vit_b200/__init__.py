@@ -10,11 +10,13 @@ from .ops import block_sparse_attention, rope2d
 from .modules import DeepSeekSparseAttention, DSAViTBlock, DSAViTSlideEncoder, IndexerProjection
 from .static_modules import (BlockSparse2DViTBlock, BlockSparse2DViTSlideEncoder, BlockSparseAttention2D,
                              StaticSparseAttention, StaticSparseViTBlock, StaticSparseViTSlideEncoder)
+from .packed import PackedPlan, RopeAxes, layer_norm, packed_attention, rope_axes
 from . import ingest, patterns, training
 
 __all__ = [
     "DSAAttentionFunction", "LightningIndexerFunction", "check_status", "dsa_attention_gather",
     "dsa_attention_masked", "dsa_indexer_topk", "dsa_sparse_attention", "DeepSeekSparseAttention",
     "DSAViTBlock", "DSAViTSlideEncoder", "IndexerProjection", "block_sparse_attention", "rope2d", "patterns", "ingest", "training",
+    "PackedPlan", "RopeAxes", "layer_norm", "packed_attention", "rope_axes",
     "BlockSparseAttention2D", "BlockSparse2DViTBlock", "BlockSparse2DViTSlideEncoder", "StaticSparseAttention", "StaticSparseViTBlock", "StaticSparseViTSlideEncoder",
 ]

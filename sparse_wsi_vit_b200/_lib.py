@@ -21,6 +21,8 @@ EXPORTS = [
     "swv_dsa_attn_bwd", "swv_dsa_indexer_bwd", "swv_dsa_prologue_fwd", "swv_dsa_attn_lists_fwd",
     "swv_dsa_attn_lists_scratch_bytes", "swv_dsa_workspace_bytes_topk", "swv_block_sparse_workspace_bytes", "swv_block_sparse_attn_ws_fwd",
     "swv_dsa_module_bwd_bytes", "swv_dsa_module_bwd",
+    "swv_layer_norm_fwd", "swv_layer_norm_bwd_bytes", "swv_layer_norm_bwd", "swv_rope_axes_apply",
+    "swv_packed_plan", "swv_packed_attn_bytes", "swv_packed_attn_fwd",
 ]
 
 
@@ -101,6 +103,21 @@ def _load():
     lib.swv_nsa_attn_fwd.argtypes = [
         c_void_p, i64p, c_void_p, i64p, c_void_p, i64p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
         c_int, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]
+    lib.swv_layer_norm_fwd.argtypes = [
+        c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64,
+        c_int, c_float, c_void_p]
+    lib.swv_layer_norm_bwd_bytes.argtypes = [c_int64, c_int, POINTER(c_size_t)]
+    lib.swv_layer_norm_bwd.argtypes = [
+        c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64,
+        c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]
+    lib.swv_rope_axes_apply.argtypes = [
+        c_void_p, i64p, c_void_p, i64p, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+        c_int64, c_int, c_int, c_void_p]
+    lib.swv_packed_plan.argtypes = [c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, POINTER(c_size_t)]
+    lib.swv_packed_attn_bytes.argtypes = [c_void_p, c_int, POINTER(c_size_t)]
+    lib.swv_packed_attn_fwd.argtypes = [
+        c_void_p, i64p, c_void_p, i64p, c_void_p, i64p, c_void_p, i64p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+        c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]
     for name in EXPORTS[2:]:
         getattr(lib, name).restype = c_int
     return lib

@@ -80,11 +80,29 @@ int nsa_attn_impl(const void* q, const int64_t* qs, const void* k, const int64_t
                   const int64_t* vs, const float* gate, void* out, int out_dtype, int B, int Hq, int Hkv, int T,
                   int D, int cmp_block, int cmp_stride, int sel_block, int n_sel, int window, void* workspace,
                   size_t workspace_bytes, int32_t* blocks_out, int* status, cudaStream_t st);
+int layer_norm_fwd_impl(const void* x, int64_t xs, int x_dtype, const void* w, int w_dtype, const void* b, int b_dtype,
+                        void* y, int64_t ys, int y_dtype, float* mean, float* rstd, int64_t N, int E, float eps,
+                        cudaStream_t st);
+int layer_norm_bwd_bytes_impl(int64_t N, int E, size_t* bytes);
+int layer_norm_bwd_impl(const void* dy, int64_t dys, int y_dtype, const void* x, int64_t xs, int x_dtype, const void* w,
+                        int w_dtype, const float* mean, const float* rstd, void* dx, int64_t dxs, void* dw, int dw_dtype,
+                        void* db, int db_dtype, int64_t N, int E, void* workspace, size_t workspace_bytes,
+                        cudaStream_t st);
+int rope_axes_impl(const void* x, const int64_t* xs, void* y, const int64_t* ys, int dtype, const void* pos,
+                   int pos_dtype, int64_t pos_stride, const double* freq_host, const uint8_t* axis_host, int pairs,
+                   int axes, int halves, int inverse, int64_t T, int H, int hd, cudaStream_t st);
+int packed_plan_impl(int n_seq, const int64_t* q_lens, const int64_t* k_lens, int H, int Hkv, int causal, int32_t* plan,
+                     size_t plan_bytes, size_t* bytes);
+int packed_attn_bytes_impl(const int32_t* plan_host, int D, size_t* bytes);
+int packed_attn_fwd_impl(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v,
+                         const int64_t* vs, void* o, const int64_t* os, float* lse, const int32_t* plan_host,
+                         const int32_t* plan, int64_t Tq, int64_t Tk, int D, float scale, void* workspace,
+                         size_t workspace_bytes, int* status, cudaStream_t st);
 }  // namespace swv
 
 extern "C" {
 
-int swv_version(void) { return 103; }
+int swv_version(void) { return 104; }
 
 const char* swv_strerror(int code) {
   switch (code) {
@@ -314,6 +332,49 @@ int swv_nsa_attn_fwd(const void* q, const int64_t q_strides[4], const void* k, c
   return swv::nsa_attn_impl(q, q_strides, k, k_strides, v, v_strides, gate, out, out_dtype, B, Hq, Hkv, T, D,
                             cmp_block, cmp_stride, sel_block, n_sel, window, workspace, workspace_bytes, blocks_out,
                             status, static_cast<cudaStream_t>(stream));
+}
+
+int swv_layer_norm_fwd(const void* x, int64_t x_stride, int x_dtype, const void* w, int w_dtype, const void* b,
+                       int b_dtype, void* y, int64_t y_stride, int y_dtype, float* mean, float* rstd, int64_t N, int E,
+                       float eps, void* stream) {
+  return swv::layer_norm_fwd_impl(x, x_stride, x_dtype, w, w_dtype, b, b_dtype, y, y_stride, y_dtype, mean, rstd, N, E,
+                                  eps, static_cast<cudaStream_t>(stream));
+}
+
+int swv_layer_norm_bwd_bytes(int64_t N, int E, size_t* bytes) { return swv::layer_norm_bwd_bytes_impl(N, E, bytes); }
+
+int swv_layer_norm_bwd(const void* dy, int64_t dy_stride, int y_dtype, const void* x, int64_t x_stride, int x_dtype,
+                       const void* w, int w_dtype, const float* mean, const float* rstd, void* dx, int64_t dx_stride,
+                       void* dw, int dw_dtype, void* db, int db_dtype, int64_t N, int E, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  return swv::layer_norm_bwd_impl(dy, dy_stride, y_dtype, x, x_stride, x_dtype, w, w_dtype, mean, rstd, dx, dx_stride, dw,
+                                  dw_dtype, db, db_dtype, N, E, workspace, workspace_bytes,
+                                  static_cast<cudaStream_t>(stream));
+}
+
+int swv_rope_axes_apply(const void* x, const int64_t x_strides[3], void* y, const int64_t y_strides[3], int dtype,
+                        const void* positions, int pos_dtype, int64_t pos_stride, const double* freq_host,
+                        const uint8_t* axis_host, int pairs, int axes, int halves, int inverse, int64_t T, int H,
+                        int head_dim, void* stream) {
+  return swv::rope_axes_impl(x, x_strides, y, y_strides, dtype, positions, pos_dtype, pos_stride, freq_host, axis_host,
+                             pairs, axes, halves, inverse, T, H, head_dim, static_cast<cudaStream_t>(stream));
+}
+
+int swv_packed_plan(int n_seq, const int64_t* q_lens_host, const int64_t* k_lens_host, int H, int Hkv, int causal,
+                    int32_t* plan_host, size_t plan_bytes, size_t* bytes) {
+  return swv::packed_plan_impl(n_seq, q_lens_host, k_lens_host, H, Hkv, causal, plan_host, plan_bytes, bytes);
+}
+
+int swv_packed_attn_bytes(const int32_t* plan_host, int D, size_t* bytes) {
+  return swv::packed_attn_bytes_impl(plan_host, D, bytes);
+}
+
+int swv_packed_attn_fwd(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                        const void* v, const int64_t v_strides[3], void* o, const int64_t o_strides[3], float* lse,
+                        const int32_t* plan_host, const int32_t* plan, int64_t Tq, int64_t Tk, int D, float scale,
+                        void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  return swv::packed_attn_fwd_impl(q, q_strides, k, k_strides, v, v_strides, o, o_strides, lse, plan_host, plan, Tq, Tk, D,
+                                   scale, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

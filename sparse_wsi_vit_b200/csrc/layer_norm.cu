@@ -1,0 +1,441 @@
+// Layer norm over the last dimension of N rows of E values, forward and backward.
+//
+//   mu = mean(x)   rstd = 1 / sqrt(mean((x - mu)^2) + eps)   xh = (x - mu) rstd   y = xh w + b
+//   g  = dy w      dx = rstd (g - mean(g) - xh mean(g xh))   dw = sum_rows dy xh  db = sum_rows dy
+//
+// A group of threads (a warp, or a CTA for wide rows) owns a row: it is read once into registers, the variance is
+// taken from the centred values (a second sum over the registers, so a large offset of the row costs no bits), and
+// the result is written from the registers.  All sums are fp32.  The groups stay resident and walk over the rows, so
+// the weights -- and in the backward pass the sums of dw and db -- stay in registers; the next row is loaded before
+// the present one is reduced.  Each CTA leaves its dw and db sums in the workspace and a second kernel adds them up in
+// a fixed order: no atomics, the same bits every time.
+//
+// Bound: HBM, 2 N E elements forward, 3 N E backward.
+#include <algorithm>
+#include <type_traits>
+
+#include "elements.cuh"
+
+namespace swv {
+namespace {
+
+constexpr int kLnThreads = 256;
+
+struct LnParams {
+  const void* x;
+  const void* dy;
+  const void* w;
+  const void* b;
+  void* y;                  // forward: y; backward: dx
+  float *mean, *rstd;       // (N), optional in the forward pass
+  float* part;              // backward: [grid][2][E] sums of dy xh and of dy, or null
+  int64_t N, xs, dys, ys;   // rows and their distances in elements
+  int E, w_dtype, b_dtype;
+  float eps;
+};
+
+// sums over the threads of a group: a warp, or the whole CTA
+template <int TPR, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float* smem, int& phase) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+  }
+  if constexpr (TPR > 32) {
+    // two buffers in turn: a warp may be one reduction ahead of the others, never two
+    float* buf = smem + (phase & 1) * (2 * (TPR / 32));
+    ++phase;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) buf[k * (TPR / 32) + (threadIdx.x >> 5)] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < TPR / 32; ++i) v[k] += buf[k * (TPR / 32) + i];
+    }
+  }
+}
+
+template <typename T, typename U, int VEC, int ITER, int TPR>
+__global__ void __launch_bounds__(kLnThreads) layer_norm_fwd_kernel(const LnParams p) {
+  __shared__ float red[4 * (kLnThreads / 32)];
+  int phase = 0;
+  const int t = threadIdx.x % TPR;
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kLnThreads / TPR);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (kLnThreads / TPR) + threadIdx.x / TPR;
+  const float inv_e = 1.f / p.E;
+  float w[ITER * VEC], b[ITER * VEC], v[ITER * VEC], nx[ITER * VEC];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int c = (i * TPR + t) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const bool in = c + e < p.E;
+      w[i * VEC + e] = in ? (p.w != nullptr ? load_as_f32(p.w, p.w_dtype, c + e) : 1.f) : 0.f;
+      b[i * VEC + e] = in && p.b != nullptr ? load_as_f32(p.b, p.b_dtype, c + e) : 0.f;
+    }
+  }
+  auto fetch = [&](int64_t r, float (&d)[ITER * VEC]) {
+    const T* xr = static_cast<const T*>(p.x) + r * p.xs;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (r < p.N && c < p.E) load_run<T, VEC>(xr + c, d + i * VEC);
+      else
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[i * VEC + e] = 0.f;
+    }
+  };
+  fetch(row, nx);
+  for (; row < p.N; row += groups) {
+#pragma unroll
+    for (int i = 0; i < ITER * VEC; ++i) v[i] = nx[i];
+    fetch(row + groups, nx);
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < ITER * VEC; ++i) s[0] += v[i];
+    group_sum<TPR>(s, red, phase);
+    const float mu = s[0] * inv_e;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = (i * TPR + t) * VEC + e < p.E ? v[i * VEC + e] - mu : 0.f;
+        v[i * VEC + e] = d;
+        s[0] = fmaf(d, d, s[0]);
+      }
+    }
+    group_sum<TPR>(s, red, phase);
+    const float rstd = 1.f / sqrtf(fmaf(s[0], inv_e, p.eps));
+    U* yr = static_cast<U*>(p.y) + row * p.ys;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * TPR + t) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i * VEC + e] = fmaf(v[i * VEC + e] * rstd, w[i * VEC + e], b[i * VEC + e]);
+      if (c < p.E) store_run<U, VEC>(yr + c, v + i * VEC);
+    }
+    if (t == 0 && p.mean != nullptr) {
+      p.mean[row] = mu;
+      p.rstd[row] = rstd;
+    }
+  }
+}
+
+template <typename T, typename U, int VEC, int ITER, int TPR>
+__global__ void __launch_bounds__(kLnThreads) layer_norm_bwd_kernel(const LnParams p) {
+  __shared__ float red[4 * (kLnThreads / 32)];
+  int phase = 0;
+  constexpr int R = ITER * VEC;
+  const int t = threadIdx.x % TPR;
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kLnThreads / TPR);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (kLnThreads / TPR) + threadIdx.x / TPR;
+  const float inv_e = 1.f / p.E;
+  float w[R], dw[R], db[R], x[R], g[R];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int c = (i * TPR + t) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      w[i * VEC + e] = c + e < p.E ? (p.w != nullptr ? load_as_f32(p.w, p.w_dtype, c + e) : 1.f) : 0.f;
+      dw[i * VEC + e] = db[i * VEC + e] = 0.f;
+    }
+  }
+  for (; row < p.N; row += groups) {
+    const T* xr = static_cast<const T*>(p.x) + row * p.xs;
+    const U* dyr = static_cast<const U*>(p.dy) + row * p.dys;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * TPR + t) * VEC;
+      if (c < p.E) {
+        load_run<T, VEC>(xr + c, x + i * VEC);
+        load_run<U, VEC>(dyr + c, g + i * VEC);
+      }
+    }
+    const float mu = p.mean[row], rstd = p.rstd[row];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int k = i * VEC + e;
+        const bool in = (i * TPR + t) * VEC + e < p.E;
+        const float xh = in ? (x[k] - mu) * rstd : 0.f, d = in ? g[k] : 0.f;
+        dw[k] = fmaf(d, xh, dw[k]);
+        db[k] += d;
+        x[k] = xh;
+        g[k] = d * w[k];
+        s[0] += g[k];
+        s[1] = fmaf(g[k], xh, s[1]);
+      }
+    }
+    group_sum<TPR>(s, red, phase);
+    const float m0 = s[0] * inv_e, m1 = s[1] * inv_e;
+    T* dxr = static_cast<T*>(p.y) + row * p.ys;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * TPR + t) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[i * VEC + e] = rstd * (g[i * VEC + e] - m0 - x[i * VEC + e] * m1);
+      if (c < p.E) store_run<T, VEC>(dxr + c, x + i * VEC);
+    }
+  }
+  if (p.part == nullptr) return;
+  // the groups' sums of this CTA, one group after the other
+  float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.E;
+  if constexpr (TPR == kLnThreads) {
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int c = (i * TPR + t) * VEC + e;
+        if (c < p.E) {
+          out[c] = dw[i * VEC + e];
+          out[p.E + c] = db[i * VEC + e];
+        }
+      }
+    }
+  } else {
+    __shared__ float acc[2][TPR * R];
+    const int mine = threadIdx.x / TPR;
+    for (int k = 0; k < kLnThreads / TPR; ++k) {
+      if (mine == k) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const int c = (i * TPR + t) * VEC + e;
+            acc[0][c] = (k == 0 ? 0.f : acc[0][c]) + dw[i * VEC + e];
+            acc[1][c] = (k == 0 ? 0.f : acc[1][c]) + db[i * VEC + e];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
+      out[c] = acc[0][c];
+      out[p.E + c] = acc[1][c];
+    }
+  }
+}
+
+// Rows that do not fit the registers: one CTA per row, which it reads again for each of its sums (from L2).
+template <typename T, typename U>
+__global__ void __launch_bounds__(kLnThreads) layer_norm_wide_fwd_kernel(const LnParams p) {
+  __shared__ float red[4 * (kLnThreads / 32)];
+  int phase = 0;
+  const float inv_e = 1.f / p.E;
+  for (int64_t row = blockIdx.x; row < p.N; row += gridDim.x) {
+    const T* xr = static_cast<const T*>(p.x) + row * p.xs;
+    float s[1] = {0.f};
+    for (int c = threadIdx.x; c < p.E; c += kLnThreads) s[0] += to_f32(xr[c]);
+    group_sum<kLnThreads>(s, red, phase);
+    const float mu = s[0] * inv_e;
+    s[0] = 0.f;
+    for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
+      const float d = to_f32(xr[c]) - mu;
+      s[0] = fmaf(d, d, s[0]);
+    }
+    group_sum<kLnThreads>(s, red, phase);
+    const float rstd = 1.f / sqrtf(fmaf(s[0], inv_e, p.eps));
+    U* yr = static_cast<U*>(p.y) + row * p.ys;
+    for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
+      const float w = p.w != nullptr ? load_as_f32(p.w, p.w_dtype, c) : 1.f;
+      const float b = p.b != nullptr ? load_as_f32(p.b, p.b_dtype, c) : 0.f;
+      yr[c] = from_f32<U>(fmaf((to_f32(xr[c]) - mu) * rstd, w, b));
+    }
+    if (threadIdx.x == 0 && p.mean != nullptr) {
+      p.mean[row] = mu;
+      p.rstd[row] = rstd;
+    }
+  }
+}
+
+// The same for the backward pass; a thread's columns are its own, so it adds dw and db into the CTA's row of the
+// workspace without conflict.
+template <typename T, typename U>
+__global__ void __launch_bounds__(kLnThreads) layer_norm_wide_bwd_kernel(const LnParams p) {
+  __shared__ float red[4 * (kLnThreads / 32)];
+  int phase = 0;
+  const float inv_e = 1.f / p.E;
+  float* part = p.part == nullptr ? nullptr : p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.E;
+  for (int64_t row = blockIdx.x; row < p.N; row += gridDim.x) {
+    const bool first = row == blockIdx.x;
+    const T* xr = static_cast<const T*>(p.x) + row * p.xs;
+    const U* dyr = static_cast<const U*>(p.dy) + row * p.dys;
+    const float mu = p.mean[row], rstd = p.rstd[row];
+    float s[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
+      const float xh = (to_f32(xr[c]) - mu) * rstd, d = to_f32(dyr[c]);
+      const float g = d * (p.w != nullptr ? load_as_f32(p.w, p.w_dtype, c) : 1.f);
+      s[0] += g;
+      s[1] = fmaf(g, xh, s[1]);
+      if (part != nullptr) {
+        part[c] = fmaf(d, xh, first ? 0.f : part[c]);
+        part[p.E + c] = (first ? 0.f : part[p.E + c]) + d;
+      }
+    }
+    group_sum<kLnThreads>(s, red, phase);
+    const float m0 = s[0] * inv_e, m1 = s[1] * inv_e;
+    T* dxr = static_cast<T*>(p.y) + row * p.ys;
+    for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
+      const float xh = (to_f32(xr[c]) - mu) * rstd;
+      const float g = to_f32(dyr[c]) * (p.w != nullptr ? load_as_f32(p.w, p.w_dtype, c) : 1.f);
+      dxr[c] = from_f32<T>(rstd * (g - m0 - xh * m1));
+    }
+  }
+}
+
+// dw[c] = sum over the CTAs' rows of the workspace: eight lanes of rows for 32 columns, added up in order
+__global__ void __launch_bounds__(256) layer_norm_sum_kernel(const float* part, int parts, int E, void* dw, int dw_dtype,
+                                                             void* db, int db_dtype) {
+  __shared__ float s[8][33];
+  const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;                   // column of [dw | db]
+  float a = 0.f;
+  if (c < 2 * E)
+    for (int k = r; k < parts; k += 8) a += part[static_cast<int64_t>(k) * 2 * E + c];
+  s[r][lane] = a;
+  __syncthreads();
+  if (r == 0 && c < 2 * E) {
+    a = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a += s[k][lane];
+    if (c < E) {
+      if (dw != nullptr) store_from_f32(dw, dw_dtype, c, a);
+    } else if (db != nullptr) {
+      store_from_f32(db, db_dtype, c - E, a);
+    }
+  }
+}
+
+// Which kernel serves a row: runs of 8 elements where every row starts on 16 bytes and E is a multiple of 8, single
+// elements otherwise; a warp a row up to 32 elements a thread, then a CTA, then the form that reads the row again.
+struct LnForm {
+  int vec, tpr, iter;       // iter = 0: the form for wide rows
+};
+LnForm ln_form(int E, bool vec8) {
+  LnForm f;
+  f.vec = vec8 ? 8 : 1;
+  f.tpr = E <= 1024 ? 32 : kLnThreads;
+  const int n = (E + f.vec * f.tpr - 1) / (f.vec * f.tpr);
+  if (f.vec == 8) f.iter = n <= 1 ? 1 : n <= 2 ? 2 : n <= 3 ? 3 : n <= 4 ? 4 : 0;
+  else f.iter = n <= 8 ? 8 : n <= 32 ? 32 : 0;
+  return f;
+}
+
+int ln_grid(int64_t N, int tpr, int per_sm) {
+  const int64_t rows = kLnThreads / tpr;
+  return static_cast<int>(std::min<int64_t>((N + rows - 1) / rows, static_cast<int64_t>(sm_count()) * per_sm));
+}
+constexpr int kLnFwdCtas = 4, kLnBwdCtas = 2;     // resident CTAs per SM
+
+template <typename T, typename U, bool BWD>
+int ln_launch(const LnParams& p, const LnForm& f, int grid, cudaStream_t st) {
+#define SWV_LN(V, I, R)                                                            \
+  if (f.vec == V && f.iter == I && f.tpr == R) {                                    \
+    if constexpr (BWD) layer_norm_bwd_kernel<T, U, V, I, R><<<grid, kLnThreads, 0, st>>>(p); \
+    else layer_norm_fwd_kernel<T, U, V, I, R><<<grid, kLnThreads, 0, st>>>(p);      \
+  } else
+  SWV_LN(8, 1, 32) SWV_LN(8, 2, 32) SWV_LN(8, 3, 32) SWV_LN(8, 4, 32)
+  SWV_LN(8, 1, kLnThreads) SWV_LN(8, 2, kLnThreads) SWV_LN(8, 3, kLnThreads) SWV_LN(8, 4, kLnThreads)
+  SWV_LN(1, 8, 32) SWV_LN(1, 32, 32) SWV_LN(1, 8, kLnThreads) SWV_LN(1, 32, kLnThreads) {
+    if constexpr (BWD) layer_norm_wide_bwd_kernel<T, U><<<grid, kLnThreads, 0, st>>>(p);
+    else layer_norm_wide_fwd_kernel<T, U><<<grid, kLnThreads, 0, st>>>(p);
+  }
+#undef SWV_LN
+  SWV_CUDA_OK(cudaGetLastError());
+  return SWV_OK;
+}
+
+template <bool BWD>
+int ln_dispatch(const LnParams& p, int x_dtype, int y_dtype, const LnForm& f, int grid, cudaStream_t st) {
+  using bf = __nv_bfloat16;
+  if (x_dtype == SWV_F32) {
+    if (y_dtype == SWV_F32) return ln_launch<float, float, BWD>(p, f, grid, st);
+    if (y_dtype == SWV_BF16) return ln_launch<float, bf, BWD>(p, f, grid, st);
+    return ln_launch<float, __half, BWD>(p, f, grid, st);
+  }
+  if (x_dtype == SWV_BF16) {
+    if (y_dtype == SWV_BF16) return ln_launch<bf, bf, BWD>(p, f, grid, st);
+    return ln_launch<bf, float, BWD>(p, f, grid, st);
+  }
+  if (y_dtype == SWV_F16) return ln_launch<__half, __half, BWD>(p, f, grid, st);
+  return ln_launch<__half, float, BWD>(p, f, grid, st);
+}
+
+int ln_check(int64_t N, int E, int x_dtype, int y_dtype, const void* w, int w_dtype, const void* b, int b_dtype) {
+  if (N < 0 || E < 1) return SWV_ERR_SHAPE;
+  if (!dtype_known(x_dtype) || !dtype_known(y_dtype)) return SWV_ERR_DTYPE;
+  if (x_dtype != SWV_F32 && y_dtype != x_dtype && y_dtype != SWV_F32) return SWV_ERR_DTYPE;
+  if ((w != nullptr && !dtype_known(w_dtype)) || (b != nullptr && !dtype_known(b_dtype))) return SWV_ERR_DTYPE;
+  return SWV_OK;
+}
+
+}  // namespace
+
+int layer_norm_fwd_impl(const void* x, int64_t xs, int x_dtype, const void* w, int w_dtype, const void* b, int b_dtype,
+                        void* y, int64_t ys, int y_dtype, float* mean, float* rstd, int64_t N, int E, float eps,
+                        cudaStream_t st) {
+  const int rc = ln_check(N, E, x_dtype, y_dtype, w, w_dtype, b, b_dtype);
+  if (rc != SWV_OK) return rc;
+  if (N == 0) return SWV_OK;
+  if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return SWV_ERR_NULL;
+  const bool vec = E % 8 == 0 && rows_vec8(x, xs, dtype_bytes(x_dtype)) && rows_vec8(y, ys, dtype_bytes(y_dtype));
+  const LnForm f = ln_form(E, vec);
+  LnParams p{};
+  p.x = x; p.w = w; p.b = b; p.y = y; p.mean = mean; p.rstd = rstd;
+  p.N = N; p.xs = xs; p.ys = ys; p.E = E; p.w_dtype = w_dtype; p.b_dtype = b_dtype; p.eps = eps;
+  return ln_dispatch<false>(p, x_dtype, y_dtype, f, ln_grid(N, f.iter == 0 ? kLnThreads : f.tpr, kLnFwdCtas), st);
+}
+
+// The backward pass takes no more CTAs than this, whichever form serves it: room for their sums.
+int layer_norm_bwd_bytes_impl(int64_t N, int E, size_t* bytes) {
+  if (!bytes) return SWV_ERR_NULL;
+  if (N < 0 || E < 1) return SWV_ERR_SHAPE;
+  *bytes = static_cast<size_t>(std::min<int64_t>(std::max<int64_t>(N, 1), static_cast<int64_t>(sm_count()) * kLnBwdCtas)) * 2 * E *
+           sizeof(float);
+  return SWV_OK;
+}
+
+int layer_norm_bwd_impl(const void* dy, int64_t dys, int y_dtype, const void* x, int64_t xs, int x_dtype, const void* w,
+                        int w_dtype, const float* mean, const float* rstd, void* dx, int64_t dxs, void* dw, int dw_dtype,
+                        void* db, int db_dtype, int64_t N, int E, void* workspace, size_t workspace_bytes,
+                        cudaStream_t st) {
+  const int rc = ln_check(N, E, x_dtype, y_dtype, w, w_dtype, nullptr, 0);
+  if (rc != SWV_OK) return rc;
+  if ((dw != nullptr && !dtype_known(dw_dtype)) || (db != nullptr && !dtype_known(db_dtype))) return SWV_ERR_DTYPE;
+  if (N > 0 && (!dy || !x || !mean || !rstd || !dx)) return SWV_ERR_NULL;
+  const bool sums = dw != nullptr || db != nullptr;
+  const bool vec = E % 8 == 0 && rows_vec8(x, xs, dtype_bytes(x_dtype)) && rows_vec8(dy, dys, dtype_bytes(y_dtype)) &&
+                   rows_vec8(dx, dxs, dtype_bytes(x_dtype));
+  const LnForm f = ln_form(E, vec);
+  const int grid = N == 0 ? 0 : ln_grid(N, f.iter == 0 ? kLnThreads : f.tpr, kLnBwdCtas);
+  if (sums && N > 0) {
+    size_t need = static_cast<size_t>(grid) * 2 * E * sizeof(float);
+    if (!workspace) return SWV_ERR_NULL;
+    if (workspace_bytes < need) return SWV_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 3) return SWV_ERR_ALIGN;
+  }
+  LnParams p{};
+  p.x = x; p.dy = dy; p.w = w; p.y = dx;
+  p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
+  p.part = sums ? static_cast<float*>(workspace) : nullptr;
+  p.N = N; p.xs = xs; p.dys = dys; p.ys = dxs; p.E = E; p.w_dtype = w_dtype;
+  if (N > 0) {
+    const int r = ln_dispatch<true>(p, x_dtype, y_dtype, f, grid, st);
+    if (r != SWV_OK) return r;
+  }
+  if (sums) {                                             // (no rows: the sums are zero)
+    layer_norm_sum_kernel<<<(2 * E + 31) / 32, 256, 0, st>>>(p.part, grid, E, dw, dw_dtype, db, db_dtype);
+    SWV_CUDA_OK(cudaGetLastError());
+  }
+  return SWV_OK;
+}
+
+}  // namespace swv

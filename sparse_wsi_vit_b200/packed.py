@@ -1,0 +1,324 @@
+"""Operators of a dense transformer over packed batches: several sequences (bags, slides) of different lengths lie one
+behind the other in token-major tensors, without padding.
+
+  packed_attention : softmax attention of every token over its own sequence, optionally causal, grouped heads,
+                     forward and backward; a ``PackedPlan`` holds the work tables of the batch's lengths
+  rope_axes        : rotary positions with up to eight axes (for example level, row and column of a patch)
+  layer_norm       : layer norm over the last dimension
+
+All of them are differentiable once, run on the current CUDA stream of the inputs' device and raise ``SwvError`` for
+calls that the kernels do not serve.  The reference's dense ViT-5 has the same pieces for one slide at a time
+(src/sparse_wsi_vit/models/vit_5/models_vit5.py:72-115, rope.py:72-97).
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import numpy as np
+import torch
+
+from ._lib import SwvError, check, dtype_code, lib, strides
+from .ops import _CHECK, _require_cuda, _stream, _workspace, check_status, status_word
+
+_POS_CODES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+
+
+def _on(dev):
+    """Launches go to the inputs' device, whichever one is current."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _same_device(*ts):
+    _require_cuda(*ts)
+    if any(t.device != ts[0].device for t in ts):
+        raise SwvError("all tensors of a call must be on one device")
+
+
+# --------------------------------------------------------------------------- #
+# layer norm
+# --------------------------------------------------------------------------- #
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _code(t):
+    return 0 if t is None else dtype_code(t.dtype)
+
+
+def _rows2d(t):
+    """``t`` as rows of its last dimension: a view where the rows are evenly spaced, else a copy."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+    return t.reshape(-1, t.shape[-1])
+
+
+def _norm_fwd(x, weight, bias, eps, out_dtype, want_stats):
+    E = x.shape[-1]
+    x2 = _rows2d(x)
+    N = x2.shape[0]
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty((2, N), dtype=torch.float32, device=x.device).unbind(0)
+    with _on(x.device):
+        check(lib.swv_layer_norm_fwd(x2.data_ptr(), x2.stride(0), dtype_code(x.dtype), _ptr(weight), _code(weight), _ptr(bias),
+                                     _code(bias), y.data_ptr(), E, dtype_code(out_dtype), _ptr(mean), _ptr(rstd), N, E, eps,
+                                     _stream(x.device)), "swv_layer_norm_fwd")
+    return y, mean, rstd
+
+
+class LayerNormFunction(torch.autograd.Function):
+    """``layer_norm`` with its gradients; the sums over the rows are added up in a fixed order."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, out_dtype):
+        y, mean, rstd = _norm_fwd(x, weight, bias, eps, out_dtype, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        E, dev = x.shape[-1], x.device
+        x2, dy2 = _rows2d(x), _rows2d(dy)
+        N = x2.shape[0]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dw = torch.empty(E, dtype=weight.dtype, device=dev) if weight is not None and ctx.needs_input_grad[1] else None
+        db = torch.empty(E, dtype=ctx.bias_dtype, device=dev) if ctx.bias_dtype is not None and ctx.needs_input_grad[2] else None
+        n = ctypes.c_size_t()
+        ws = None
+        if dw is not None or db is not None:
+            check(lib.swv_layer_norm_bwd_bytes(N, E, ctypes.byref(n)), "swv_layer_norm_bwd_bytes")
+            ws = _workspace(dev, n.value)
+        with _on(dev):
+            check(lib.swv_layer_norm_bwd(dy2.data_ptr(), dy2.stride(0), dtype_code(dy.dtype), x2.data_ptr(), x2.stride(0),
+                                         dtype_code(x.dtype), _ptr(weight), _code(weight), mean.data_ptr(), rstd.data_ptr(),
+                                         dx.data_ptr(), E, _ptr(dw), _code(dw), _ptr(db), _code(db), N, E, _ptr(ws), n.value,
+                                         _stream(dev)), "swv_layer_norm_bwd")
+        return dx, dw, db, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
+    """Layer norm over the last dimension of ``x (..., E)``, as ``torch.nn.functional.layer_norm(x, (E,), weight, bias)``.
+
+    ``x`` fp32, bf16 or fp16; ``weight`` and ``bias`` (E,) of any of the three types, or None.  The statistics and all
+    sums are fp32.  ``out_dtype``: x's type (the default) or fp32, for an fp32 ``x`` any of the three.  Rows may be evenly
+    spaced views; other layouts are copied."""
+    _same_device(*(t for t in (x, weight, bias) if t is not None))
+    out_dtype = out_dtype or x.dtype
+    for t in (x.dtype, out_dtype):
+        dtype_code(t)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise SwvError("layer_norm needs a last dimension of one value or more")
+    if x.dtype != torch.float32 and out_dtype not in (x.dtype, torch.float32):
+        raise SwvError(f"layer_norm of {x.dtype} gives {x.dtype} or float32, not {out_dtype}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != (x.shape[-1],):
+            raise SwvError(f"{name} has shape {tuple(t.shape)}, expected {(x.shape[-1],)}")
+    weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return LayerNormFunction.apply(x, weight, bias, float(eps), out_dtype)
+    return _norm_fwd(x, weight, bias, float(eps), out_dtype, False)[0]
+
+
+# --------------------------------------------------------------------------- #
+# rotary positions with several axes
+# --------------------------------------------------------------------------- #
+class RopeAxes:
+    """How the channel pairs of a head turn: which axis of the position each pair follows, and how fast.
+
+    ``sections``: the number of pairs of each axis, in channel order; pairs beyond their sum are not rotated.
+    ``ladder``: "axis" -- every axis has frequencies theta^(-i / n) of its own, i = 0 .. n - 1 over its n pairs (with
+    two equal sections and scales 1 / coord_high this is ``rope2d``); "head" -- one ladder theta^(-p / R) over all R
+    rotated pairs p, of which every axis has its section.
+    ``pairing``: "adjacent" -- pair p is channels (2p, 2p + 1); "halves" -- channels (p, R + p).
+    ``scales``: a factor for the positions of each axis (default 1)."""
+
+    def __init__(self, head_dim, sections, theta=10000.0, scales=None, ladder="axis", pairing="adjacent"):
+        sections = [int(n) for n in sections]
+        scales = [1.0] * len(sections) if scales is None else [float(s) for s in scales]
+        R = sum(sections)
+        if not 1 <= len(sections) <= 8 or min(sections) < 0 or R < 1 or 2 * R > head_dim or R > 128:
+            raise SwvError(f"sections {sections}: one to eight axes and 1 to min(head_dim / 2, 128) pairs (head_dim {head_dim})")
+        if len(scales) != len(sections):
+            raise SwvError(f"{len(scales)} scales for {len(sections)} axes")
+        if ladder not in ("axis", "head") or pairing not in ("adjacent", "halves"):
+            raise SwvError(f"ladder is 'axis' or 'head', pairing 'adjacent' or 'halves'; got {ladder!r}, {pairing!r}")
+        if not theta > 0:
+            raise SwvError("theta must be positive")
+        self.head_dim, self.sections, self.pairs, self.halves = int(head_dim), tuple(sections), R, pairing == "halves"
+        power = [(sum(sections[:a]) + i) / R if ladder == "head" else i / n for a, n in enumerate(sections) for i in range(n)]
+        self._axis = np.repeat(np.arange(len(sections)), sections).astype(np.uint8)
+        self._freq = np.asarray(scales)[self._axis] * np.float64(theta) ** -np.asarray(power, dtype=np.float64)
+
+
+def _rope_apply(x, positions, rope, inverse, out=None):
+    T, H, hd = x.shape
+    if x.stride(2) != 1:
+        x = x.contiguous()
+    y = torch.empty((T, H, hd), dtype=x.dtype, device=x.device) if out is None else out
+    s3 = lambda t: (ctypes.c_int64 * 3)(*t.stride())
+    with _on(x.device):
+        check(lib.swv_rope_axes_apply(x.data_ptr(), s3(x), y.data_ptr(), s3(y), dtype_code(x.dtype), positions.data_ptr(),
+                                      _POS_CODES[positions.dtype], positions.stride(0), rope._freq.ctypes.data,
+                                      rope._axis.ctypes.data, rope.pairs, len(rope.sections), int(rope.halves), int(inverse),
+                                      T, H, hd, _stream(x.device)), "swv_rope_axes_apply")
+    return y
+
+
+class RopeAxesFunction(torch.autograd.Function):
+    """``rope_axes`` with its gradient: the upstream gradient turned by the opposite angles."""
+
+    @staticmethod
+    def forward(ctx, x, positions, rope):
+        ctx.save_for_backward(positions)
+        ctx.rope = rope
+        return _rope_apply(x, positions, rope, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return _rope_apply(g, ctx.saved_tensors[0], ctx.rope, True), None, None
+
+
+def rope_axes(x, positions, rope, out=None):
+    """Turns the heads ``x (T, H, head_dim)`` (fp32, bf16 or fp16) by ``positions (T, axes)`` (fp32, int32 or int64) as
+    ``rope`` (a ``RopeAxes``) says.  The queries and keys of a fused projection turn in one call as its leading heads.
+    ``out``: where to write, ``x`` itself included (inference only)."""
+    _same_device(x, positions)
+    if x.dim() != 3 or x.shape[2] != rope.head_dim:
+        raise SwvError(f"x has shape {tuple(x.shape)}, expected (tokens, heads, {rope.head_dim})")
+    if x.shape[1] < 1:
+        raise SwvError("rope_axes needs one head or more")
+    dtype_code(x.dtype)
+    if positions.dtype not in _POS_CODES:
+        raise SwvError(f"positions are float32, int32 or int64, not {positions.dtype}")
+    if tuple(positions.shape) != (x.shape[0], len(rope.sections)):
+        raise SwvError(f"positions have shape {tuple(positions.shape)}, expected {(x.shape[0], len(rope.sections))}")
+    if positions.stride(1) != 1 and positions.shape[1] > 1:
+        positions = positions.contiguous()
+    grad = torch.is_grad_enabled() and x.requires_grad
+    if out is not None:
+        if grad:
+            raise SwvError("rope_axes writes into `out` only where no gradient is asked for")
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
+            raise SwvError("out must have x's shape, type and device, and unit inner stride")
+        if x.stride(2) != 1 and out.data_ptr() != x.data_ptr():
+            x = x.contiguous()
+    return RopeAxesFunction.apply(x, positions, rope) if grad else _rope_apply(x, positions, rope, False, out)
+
+
+# --------------------------------------------------------------------------- #
+# packed attention
+# --------------------------------------------------------------------------- #
+class PackedPlan:
+    """The work tables of one packed batch, for any number of calls with its lengths (all layers of an encoder).
+
+    ``q_lengths`` / ``k_lengths``: tokens of every sequence (k_lengths None: the same); ``heads`` query heads share
+    ``kv_heads`` key / value heads evenly.  ``causal``: query i of a sequence sees the keys j <= i + lk - lq.
+    Made on the host and copied to ``device`` once; a captured CUDA graph keeps using the plan it was captured with, so
+    the plan must outlive it."""
+
+    def __init__(self, q_lengths, k_lengths=None, *, heads, kv_heads=None, causal=False, device="cuda"):
+        ql = np.ascontiguousarray(np.asarray(q_lengths, dtype=np.int64).reshape(-1))
+        kl = ql if k_lengths is None else np.ascontiguousarray(np.asarray(k_lengths, dtype=np.int64).reshape(-1))
+        if len(ql) != len(kl):
+            raise SwvError(f"{len(ql)} query lengths and {len(kl)} key lengths")
+        self.heads, self.kv_heads, self.causal = int(heads), int(heads if kv_heads is None else kv_heads), bool(causal)
+        device = torch.device(device)
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
+        self.q_tokens, self.k_tokens = int(ql.sum()), int(kl.sum())
+        size = ctypes.c_size_t()
+        words = np.empty(1 << 14, dtype=np.int32)
+        for _ in range(2):
+            rc = lib.swv_packed_plan(len(ql), ql.ctypes.data, kl.ctypes.data, self.heads, self.kv_heads, int(self.causal),
+                                     words.ctypes.data, words.nbytes, ctypes.byref(size))
+            if rc != -5:                                  # (the tables need a larger array)
+                break
+            words = np.empty(size.value // 4, dtype=np.int32)
+        check(rc, "swv_packed_plan")
+        self._host = words[: size.value // 4].copy()
+        self._table = torch.from_numpy(self._host).to(self.device)      # (waits for the copy: any stream may use it)
+        self._bytes = {}
+
+    def bytes_for(self, D, backward=False):
+        key = (D, backward)
+        if key not in self._bytes:
+            n = ctypes.c_size_t()
+            f = lib.swv_packed_attn_bwd_bytes if backward else lib.swv_packed_attn_bytes
+            check(f(self._host.ctypes.data, D, ctypes.byref(n)), "swv_packed_attn_bytes")
+            self._bytes[key] = n.value
+        return self._bytes[key]
+
+
+def _rows_ok(t):
+    return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and min(t.stride()) > 0
+
+
+def _aligned(t):
+    """A layout that the copy engines take: rows on 16 bytes."""
+    return t if _rows_ok(t) else torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
+def _attn_check(q, k, v, plan):
+    _same_device(q, k, v)
+    if not isinstance(plan, PackedPlan):
+        raise SwvError("packed_attention needs a PackedPlan")
+    if plan.device != q.device:
+        raise SwvError(f"the plan is on {plan.device}, the tensors on {q.device}")
+    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+        raise SwvError("packed_attention needs bf16 q, k and v")
+    if any(t.dim() != 3 for t in (q, k, v)) or k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise SwvError("packed_attention takes q (Tq, heads, D) and k, v (Tk, kv_heads, D)")
+    if q.shape[1] != plan.heads or k.shape[1] != plan.kv_heads:
+        raise SwvError(f"{q.shape[1]} and {k.shape[1]} heads, the plan is for {plan.heads} and {plan.kv_heads}")
+    if q.shape[0] < plan.q_tokens or k.shape[0] < plan.k_tokens:
+        raise SwvError(f"{q.shape[0]} query and {k.shape[0]} key tokens, the plan's sequences have {plan.q_tokens} and "
+                       f"{plan.k_tokens}")
+    D = q.shape[2]
+    if D % 8 or not 8 <= D <= 128:
+        raise SwvError(f"packed_attention supports head dimensions that are multiples of 8 up to 128, not {D}")
+
+
+def _attn_fwd(q, k, v, plan, scale, want_lse, out=None):
+    dev, D = q.device, q.shape[2]
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    o = out
+    if o is None:
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        if plan.q_tokens < q.shape[0]:
+            o[plan.q_tokens:].zero_()                     # rows behind the last sequence
+    lse = None
+    if want_lse:
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev)
+        if plan.q_tokens < q.shape[0]:
+            lse[:, plan.q_tokens:].fill_(-float("inf"))
+    nws = plan.bytes_for(D)
+    ws = _workspace(dev, nws) if nws else None
+    with _on(dev):
+        check(lib.swv_packed_attn_fwd(q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v),
+                                      o.data_ptr(), strides(o), _ptr(lse), plan._host.ctypes.data, plan._table.data_ptr(),
+                                      q.shape[0], k.shape[0], D, scale, _ptr(ws), nws, status_word(dev).data_ptr(),
+                                      _stream(dev)), "swv_packed_attn_fwd")
+    if _CHECK:
+        check_status(dev, "swv_packed_attn_fwd")
+    return o, lse
+
+
+def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
+    """Softmax attention inside each sequence of a packed batch.
+
+    ``q (Tq, heads, D)``, ``k, v (Tk, kv_heads, D)`` bf16, D a multiple of 8 up to 128, any strides (views of a fused
+    projection are read as they are if their rows lie on 16 bytes); ``plan``: the batch's ``PackedPlan``; ``scale``
+    defaults to 1 / sqrt(D).  Returns ``(Tq, heads, D)`` bf16, with ``return_lse`` also the rows' log-sum-exp (heads, Tq)
+    fp32, which has no gradient.  A row that sees no key is zero (lse -inf), and so are rows behind the last
+    sequence; with ``out`` (inference only) those are left as they were."""
+    _attn_check(q, k, v, plan)
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise SwvError("scale must be positive and finite")
+    o, lse = _attn_fwd(q, k, v, plan, scale, return_lse, out)
+    return (o, lse) if return_lse else o
