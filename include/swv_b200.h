@@ -453,6 +453,14 @@ int swv_packed_attn_fwd(const void* q, const int64_t q_strides[3], const void* k
                         const int32_t* plan_host, const int32_t* plan, int64_t Tq, int64_t Tk, int D, float scale,
                         void* workspace, size_t workspace_bytes, int* status, void* stream);
 
+int swv_packed_attn_bwd_bytes(const int32_t* plan_host, int64_t Tq, int D, size_t* bytes);
+int swv_packed_attn_bwd(const void* d_out, const int64_t d_out_strides[3], const void* q, const int64_t q_strides[3],
+                        const void* k, const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                        const void* o, const int64_t o_strides[3], const float* lse, void* dq, const int64_t dq_strides[3],
+                        void* dk, const int64_t dk_strides[3], void* dv, const int64_t dv_strides[3],
+                        const int32_t* plan_host, const int32_t* plan, int64_t Tq, int64_t Tk, int D, float scale,
+                        void* workspace, size_t workspace_bytes, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

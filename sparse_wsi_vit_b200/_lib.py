@@ -23,6 +23,7 @@ EXPORTS = [
     "swv_dsa_module_bwd_bytes", "swv_dsa_module_bwd",
     "swv_layer_norm_fwd", "swv_layer_norm_bwd_bytes", "swv_layer_norm_bwd", "swv_rope_axes_apply",
     "swv_packed_plan", "swv_packed_attn_bytes", "swv_packed_attn_fwd",
+    "swv_packed_attn_bwd_bytes", "swv_packed_attn_bwd",
 ]
 
 
@@ -118,6 +119,10 @@ def _load():
     lib.swv_packed_attn_fwd.argtypes = [
         c_void_p, i64p, c_void_p, i64p, c_void_p, i64p, c_void_p, i64p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
         c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]
+    lib.swv_packed_attn_bwd_bytes.argtypes = [c_void_p, c_int64, c_int, POINTER(c_size_t)]
+    lib.swv_packed_attn_bwd.argtypes = (
+        [c_void_p, i64p] * 5 + [c_void_p] + [c_void_p, i64p] * 3 +
+        [c_void_p, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p])
     for name in EXPORTS[2:]:
         getattr(lib, name).restype = c_int
     return lib

@@ -20,7 +20,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libswv_b200.so")
 SOURCES = ["indexer.cu", "dsa_attn.cu", "dsa_attn_lists.cu", "dsa_gather.cu", "dsa_bwd.cu", "dsa_bwd_tiles.cu", "block_sparse.cu", "nsa.cu", "layer_norm.cu", "rope_axes.cu", "packed_plan.cu",
-           "packed_attn.cu", "capi.cu"]
+           "packed_attn.cu", "packed_attn_bwd.cu", "capi.cu"]
 HEADERS = ["ptx.cuh", "common.cuh", "elements.cuh", "packed.cuh", os.path.join("..", "..", "include", "swv_b200.h")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

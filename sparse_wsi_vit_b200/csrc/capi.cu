@@ -98,6 +98,12 @@ int packed_attn_fwd_impl(const void* q, const int64_t* qs, const void* k, const 
                          const int64_t* vs, void* o, const int64_t* os, float* lse, const int32_t* plan_host,
                          const int32_t* plan, int64_t Tq, int64_t Tk, int D, float scale, void* workspace,
                          size_t workspace_bytes, int* status, cudaStream_t st);
+int packed_attn_bwd_bytes_impl(const int32_t* plan_host, int64_t Tq, int D, size_t* bytes);
+int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, const int64_t* qs, const void* k,
+                         const int64_t* ks, const void* v, const int64_t* vs, const void* o, const int64_t* os,
+                         const float* lse, void* dq, const int64_t* dqs, void* dk, const int64_t* dks, void* dv,
+                         const int64_t* dvs, const int32_t* plan_host, const int32_t* plan, int64_t Tq, int64_t Tk, int D,
+                         float scale, void* workspace, size_t workspace_bytes, int* status, cudaStream_t st);
 }  // namespace swv
 
 extern "C" {
@@ -375,6 +381,21 @@ int swv_packed_attn_fwd(const void* q, const int64_t q_strides[3], const void* k
                         void* workspace, size_t workspace_bytes, int* status, void* stream) {
   return swv::packed_attn_fwd_impl(q, q_strides, k, k_strides, v, v_strides, o, o_strides, lse, plan_host, plan, Tq, Tk, D,
                                    scale, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
+}
+
+int swv_packed_attn_bwd_bytes(const int32_t* plan_host, int64_t Tq, int D, size_t* bytes) {
+  return swv::packed_attn_bwd_bytes_impl(plan_host, Tq, D, bytes);
+}
+
+int swv_packed_attn_bwd(const void* d_out, const int64_t d_out_strides[3], const void* q, const int64_t q_strides[3],
+                        const void* k, const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                        const void* o, const int64_t o_strides[3], const float* lse, void* dq, const int64_t dq_strides[3],
+                        void* dk, const int64_t dk_strides[3], void* dv, const int64_t dv_strides[3],
+                        const int32_t* plan_host, const int32_t* plan, int64_t Tq, int64_t Tk, int D, float scale,
+                        void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  return swv::packed_attn_bwd_impl(d_out, d_out_strides, q, q_strides, k, k_strides, v, v_strides, o, o_strides, lse, dq,
+                                   dq_strides, dk, dk_strides, dv, dv_strides, plan_host, plan, Tq, Tk, D, scale, workspace,
+                                   workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,655 @@
+// Attention over packed sequences, backward.
+//
+//   P_ij = exp(scale q_i.k_j - lse_i)          delta_i = dO_i . O_i
+//   dS_ij = P_ij (dO_i . v_j - delta_i)
+//   dV_j = sum_i P_ij dO_i      dK_j = scale sum_i dS_ij q_i      dQ_i = scale sum_j dS_ij k_j
+//
+// Three launches: delta (and lse in powers of two) per row; the keys' side (dK, dV); the queries' side (dQ).  Scores and
+// probabilities are formed again in both: two sums that each stay in one CTA's TMEM, so every gradient is
+// written once, in its own type, and there are no atomics -- the same bits every time.  The rows of a tile are packed from
+// the group's heads as in the forward pass, which makes the sum over a group's heads part of the product.
+//
+// One kernel for both sides.  The lane side (128 rows) stays in shared memory, the streamed side passes through two rings:
+//   kDkv : lanes = keys;    streamed: Q (ring A), dO (ring B)     S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//   kDq  : lanes = queries; streamed: K (ring A), V (ring B)      S = Q K^T,   dP = dO V^T,   dQ += dS K
+// warp 0: TMA producer; warp 1: issues the products; warp 2: lse and delta of the streamed rows (kDkv); warp 3: zeroes the
+// streamed rows behind the sequence's end (they are summed over, and 0 x NaN would reach the sums); warps 4..11: eight
+// warps turn a tile's S and dP into P and dS, (row quarter, half of the columns) each.  P and dS go back into TMEM as bf16 pairs over the
+// columns that the warp read, as the A operand of the gradient products (16-bit operands: 2^-9 of each entry, independent).
+// TMEM: kDkv  S [0,128), dP [128,256), dV [256,256+D), dK [256+D,256+2D)
+//       kDq   S twice [0,256), dP [256,384), dQ [384,384+D)
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "packed.cuh"
+
+namespace swv {
+
+bool packed_aligned(const void* p, const int64_t* s, int es);
+int packed_tmap(CUtensorMap* out, const void* base, const int64_t* s, int64_t tokens, int heads_kv, int group, int d,
+                int box_tok);
+int packed_plan_header(const int32_t* plan_host, PackedHeader* h);
+
+namespace {
+
+enum { kDkv = 0, kDq = 1 };
+constexpr int kBwdThreads = 384;
+
+struct PackedBwdParams {
+  const PackedUnit* units;
+  int n_units, group, tok, Tq, d, Hkv;
+  const float2* stats;          // [Hkv][Tq][group] {lse in powers of two, delta}; +inf where a row sees no key
+  void *g1, *g2;                // kDkv: dK, dV; kDq: dQ
+  int64_t g1_t, g1_h, g2_t, g2_h;
+  float scale, scale_log2;
+  float* part;                  // [slot][Hkv][128][D (kDq) or 2 D (kDkv: dV, dK)] sums of divided units, before the scale
+  int* status;
+};
+
+template <int D, int MODE>
+struct BwdCfg {
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kA = D == 64 ? 4 : (MODE == kDkv ? 2 : 3);       // stages of ring A and ring B
+  static constexpr int kB = D == 64 ? 4 : (MODE == kDkv ? 2 : 1);
+  static constexpr int kOffA = 2 * kTileBytes;
+  static constexpr int kOffB = kOffA + kA * kTileBytes;
+  static constexpr int kOffStats = kOffB + kB * kTileBytes;             // [2][2][128] floats
+  static constexpr int kOffCtl = kOffStats + 2 * 2 * kTile * 4;
+};
+struct BwdCtl {
+  uint64_t lane_full, a_full[4], a_empty[4], b_full[4], b_empty[4], tail_a, tail_b;
+  uint64_t s_full[2], dp_full, p_ready, ds_ready, p_done, ds_done, all_done, stat_full[2], stat_empty[2];
+  uint32_t tmem_base, abort_flag;
+};
+template <int D, int MODE>
+constexpr size_t bwd_smem() { return 1024 + BwdCfg<D, MODE>::kOffCtl + sizeof(BwdCtl) + 64; }
+
+// bits [lo, hi) of the 32 columns from `base` on
+__device__ __forceinline__ uint32_t column_bits(int lo, int hi, int base) {
+  auto low = [](int n) { return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u); };
+  return low(hi - base) & ~low(lo - base);
+}
+
+// zeroes rows [first, 128) of a tile of D / 64 swizzled halves (whole 128-byte rows, so the swizzle does not matter)
+template <int D>
+__device__ __forceinline__ void zero_rows(uint32_t tile, int first, int thread, int threads) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+    for (int i = first * 8 + thread; i < kTile * 8; i += threads) sts128(tile + c * (kTile * 128) + i * 16, 0u, 0u, 0u, 0u);
+}
+
+template <int D, int MODE>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    packed_attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_l1, const __grid_constant__ CUtensorMap tm_l2,
+                           const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                           const PackedBwdParams p) {
+  using Cfg = BwdCfg<D, MODE>;
+  constexpr int NA = Cfg::kA, NB = Cfg::kB, TB = Cfg::kTileBytes;
+  constexpr uint32_t kIdescS = make_idesc(/*bf16*/ 1, kTile, kTile, 0, 0);
+  constexpr uint32_t kIdescG = make_idesc(/*bf16*/ 1, kTile, D, 0, /*B is MN-major*/ 1);
+  constexpr uint32_t kColDp = MODE == kDkv ? 128 : 256;
+  constexpr uint32_t kColG = MODE == kDkv ? 256 : 384;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  BwdCtl* ctl = reinterpret_cast<BwdCtl*>(smem + Cfg::kOffCtl);
+  float* stats = reinterpret_cast<float*>(smem + Cfg::kOffStats);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int kvh = blockIdx.x / p.n_units;
+  const PackedUnit u = p.units[blockIdx.x % p.n_units];
+  const int n = u.b1 - u.b0;
+  const int per = MODE == kDkv ? p.tok * p.group : kTile;      // streamed rows a tile
+  const int step = MODE == kDkv ? p.tok : kTile;               // streamed tokens a tile
+  const int last_rows = min(step, u.len - (u.b1 - 1) * step) * (MODE == kDkv ? p.group : 1);
+  const bool tail = n > 0 && last_rows < per;                  // the last tile holds rows behind the sequence
+
+  if (threadIdx.x == 0) {
+    mbar_init(&ctl->lane_full, 1);
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&ctl->a_full[s], 1);
+      mbar_init(&ctl->a_empty[s], 1);
+      mbar_init(&ctl->b_full[s], 1);
+      mbar_init(&ctl->b_empty[s], 1);
+    }
+    mbar_init(&ctl->tail_a, 1);
+    mbar_init(&ctl->tail_b, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&ctl->s_full[s], 1);
+      mbar_init(&ctl->stat_full[s], 1);
+      mbar_init(&ctl->stat_empty[s], 8);
+    }
+    mbar_init(&ctl->dp_full, 1);
+    mbar_init(&ctl->p_ready, 8);
+    mbar_init(&ctl->ds_ready, 8);
+    mbar_init(&ctl->p_done, 1);
+    mbar_init(&ctl->ds_done, 1);
+    mbar_init(&ctl->all_done, 1);
+    ctl->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (MODE == kDkv && per < kTile) {
+    // rows that no load fills: they are summed over as zeros
+    for (int s = 0; s < NA + NB; ++s) zero_rows<D>(smem_u32(smem + Cfg::kOffA + s * TB), per, threadIdx.x, kBwdThreads);
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = ctl->tmem_base;
+  volatile uint32_t* abort_flag = &ctl->abort_flag;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+    if (mbar_wait_bounded(bar, parity, abort_flag)) return true;
+    record_status(p.status, code);
+    return false;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0 && n > 0) {
+      tma_prefetch_desc(&tm_l1);
+      tma_prefetch_desc(&tm_l2);
+      tma_prefetch_desc(&tm_a);
+      tma_prefetch_desc(&tm_b);
+      mbar_expect_tx(&ctl->lane_full, 2 * (MODE == kDkv ? TB : p.tok * p.group * D * 2));
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        if (MODE == kDkv) {
+          tma_load_3d(smem + c * (kTile * 128), &tm_l1, &ctl->lane_full, c * 64, u.t0, kvh);
+          tma_load_3d(smem + TB + c * (kTile * 128), &tm_l2, &ctl->lane_full, c * 64, u.t0, kvh);
+        } else {
+          tma_load_4d(smem + c * (kTile * 128), &tm_l1, &ctl->lane_full, c * 64, 0, u.t0, kvh);
+          tma_load_4d(smem + TB + c * (kTile * 128), &tm_l2, &ctl->lane_full, c * 64, 0, u.t0, kvh);
+        }
+      }
+      for (int j = 0; j < n; ++j) {
+        const int at = u.s0 + (u.b0 + j) * step;
+        // (the stages of the tail are declared full by the warp that cleans them)
+        const bool cut = tail && j == n - 1;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int N = r == 0 ? NA : NB, s = j % N;
+          uint64_t* full = r == 0 ? &ctl->a_full[s] : &ctl->b_full[s];
+          if (*abort_flag != 0u || !wait(r == 0 ? &ctl->a_empty[s] : &ctl->b_empty[s], ((j / N) & 1) ^ 1, kDevWaitStageEmpty))
+            break;
+          uint8_t* dst = smem + (r == 0 ? Cfg::kOffA : Cfg::kOffB) + s * TB;
+          uint64_t* bar = !cut ? full : r == 0 ? &ctl->tail_a : (MODE == kDkv ? &ctl->tail_b : full);
+          mbar_expect_tx(bar, per * D * 2);
+          const CUtensorMap* tm = r == 0 ? &tm_a : &tm_b;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            if (MODE == kDkv) tma_load_4d(dst + c * (kTile * 128), tm, bar, c * 64, 0, at, kvh);
+            else tma_load_3d(dst + c * (kTile * 128), tm, bar, c * 64, at, kvh);
+          }
+        }
+        if (*abort_flag != 0u) break;
+      }
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------------- MMA issuer
+    if (lane == 0 && n > 0) {
+      const uint32_t l1 = smem_u32(smem), l2 = l1 + TB, ra = l1 + Cfg::kOffA, rb = l1 + Cfg::kOffB;
+      bool ok = wait(&ctl->lane_full, 0, kDevWaitQ);
+      auto product = [&](uint32_t col, uint32_t a, uint32_t b) {          // both operands along the channels
+        const uint64_t da = smem_desc_sw128(a), db = smem_desc_sw128(b);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint64_t off = (ks >> 2) * (kTile * 128 / 16) + (ks & 3) * 2;
+          umma_f16_ss(col, da + off, db + off, kIdescS, ks > 0);
+        }
+      };
+      auto gradient = [&](uint32_t col, uint32_t a_col, uint32_t b, bool first) {   // the 128 streamed rows are summed over
+        const uint64_t db = smem_desc_sw128(b, kTile * 128);
+#pragma unroll
+        for (int ks = 0; ks < kTile / 16; ++ks) 
+          umma_f16_ts(col, a_col + (ks >> 2) * 64 + (ks & 3) * 8, db + ks * 128, kIdescG, !first || ks > 0);
+      };
+      if constexpr (MODE == kDkv) {
+        for (int j = 0; ok && j < n; ++j) {
+          const int sa = j % NA, sb = j % NB;
+          ok = wait(&ctl->a_full[sa], (j / NA) & 1, kDevWaitTmaFull) &&
+               (j == 0 || wait(&ctl->p_done, (j - 1) & 1, kDevWaitPvDone));          // P(j-1) lies where S(j) goes
+          if (!ok) break;
+          tc_fence_after();
+          product(tmem_base, l1, ra + sa * TB);
+          umma_commit(&ctl->s_full[0]);
+          if (j > 0) {
+            ok = wait(&ctl->ds_ready, (j - 1) & 1, kDevWaitPReady);
+            if (!ok) break;
+            tc_fence_after();
+            gradient(tmem_base + kColG + D, tmem_base + kColDp, ra + ((j - 1) % NA) * TB, j == 1);
+            umma_commit(&ctl->a_empty[(j - 1) % NA]);
+            umma_commit(&ctl->ds_done);
+          }
+          ok = wait(&ctl->b_full[sb], (j / NB) & 1, kDevWaitTmaFull) &&
+               (j == 0 || wait(&ctl->ds_done, (j - 1) & 1, kDevWaitPvDone));
+          if (!ok) break;
+          tc_fence_after();
+          product(tmem_base + kColDp, l2, rb + sb * TB);
+          umma_commit(&ctl->dp_full);
+          ok = wait(&ctl->p_ready, j & 1, kDevWaitPReady);
+          if (!ok) break;
+          tc_fence_after();
+          gradient(tmem_base + kColG, tmem_base, rb + sb * TB, j == 0);
+          umma_commit(&ctl->b_empty[sb]);
+          umma_commit(&ctl->p_done);
+        }
+        if (ok && wait(&ctl->ds_ready, (n - 1) & 1, kDevWaitPReady)) {
+          tc_fence_after();
+          gradient(tmem_base + kColG + D, tmem_base + kColDp, ra + ((n - 1) % NA) * TB, n == 1);
+          umma_commit(&ctl->all_done);
+        }
+      } else {
+        auto scores = [&](int j) {
+          // dS(j-2) lay where S(j) goes
+          if (!wait(&ctl->a_full[j % NA], (j / NA) & 1, kDevWaitTmaFull) ||
+              (j >= 2 && !wait(&ctl->ds_done, j & 1, kDevWaitPvDone)))
+            return false;
+          tc_fence_after();
+          product(tmem_base + (j & 1) * 128, l1, ra + (j % NA) * TB);
+          umma_commit(&ctl->s_full[j & 1]);
+          return true;
+        };
+        if (ok) ok = scores(0);
+        for (int j = 0; ok && j < n; ++j) {
+          // (dP(j-1) has been read: its dS was ready before dQ took it)
+          ok = wait(&ctl->b_full[j % NB], (j / NB) & 1, kDevWaitTmaFull);
+          if (!ok) break;
+          tc_fence_after();
+          product(tmem_base + kColDp, l2, rb + (j % NB) * TB);
+          umma_commit(&ctl->b_empty[j % NB]);
+          umma_commit(&ctl->dp_full);
+          if (j + 1 < n) ok = scores(j + 1);
+          ok = ok && wait(&ctl->ds_ready, j & 1, kDevWaitPReady);
+          if (!ok) break;
+          tc_fence_after();
+          gradient(tmem_base + kColG, tmem_base + (j & 1) * 128, ra + (j % NA) * TB, j == 0);
+          umma_commit(&ctl->a_empty[j % NA]);
+          umma_commit(j + 1 < n ? &ctl->ds_done : &ctl->all_done);
+        }
+      }
+    }
+  } else if (warp == 2) {
+    // --------------------------- lse and delta of the streamed rows, two tiles ahead at most
+    if (MODE == kDkv) {
+      for (int j = 0; j < n; ++j) {
+        const int tok0 = (u.b0 + j) * step;
+        const int rows = min(step, u.len - tok0) * p.group;
+        const float2* src = p.stats + (static_cast<int64_t>(kvh) * p.Tq + u.s0 + tok0) * p.group;
+        float2 f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 32 + lane;
+          f[i] = r < rows ? __ldg(src + r) : make_float2(__int_as_float(0x7f800000), 0.f);
+        }
+        bool ok = j < 2 || wait(&ctl->stat_empty[j & 1], ((j >> 1) & 1) ^ 1, kDevWaitPReady);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        float* st = stats + (j & 1) * 2 * kTile;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          st[i * 32 + lane] = f[i].x;
+          st[kTile + i * 32 + lane] = f[i].y;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->stat_full[j & 1]);
+      }
+    }
+  } else if (warp == 3) {
+    if (tail) {
+      bool ok = wait(&ctl->tail_a, 0, kDevWaitTmaFull) && (MODE == kDq || wait(&ctl->tail_b, 0, kDevWaitTmaFull));
+      if (__all_sync(0xffffffffu, ok)) {
+        const int sa = (n - 1) % NA, sb = (n - 1) % NB;
+        zero_rows<D>(smem_u32(smem + Cfg::kOffA + sa * TB), last_rows, lane, 32);
+        if (MODE == kDkv) zero_rows<D>(smem_u32(smem + Cfg::kOffB + sb * TB), last_rows, lane, 32);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&ctl->a_full[sa]);
+          if (MODE == kDkv) mbar_arrive(&ctl->b_full[sb]);
+        }
+      }
+    }
+  } else {
+    // ------------------------------- eight warps: (row quarter, half of the columns)
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int row = quarter * 32 + lane, c0 = half * 64;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const float c2 = p.scale_log2;
+    bool ok = true;
+    float lse2 = 0.f, delta = 0.f;
+    int limit = 0;                                             // kDq: keys the row sees from block b0 on
+    const int rows = MODE == kDkv ? u.n : u.n * p.group;
+    const bool row_ok = row < rows;
+    const int tk = MODE == kDkv ? row : row / p.group;         // token of the lane side
+    if (MODE == kDq && row_ok) {
+      const float2 f = __ldg(p.stats + (static_cast<int64_t>(kvh) * p.Tq + u.t0) * p.group + row);
+      lse2 = f.x;
+      delta = f.y;
+      limit = min(u.len, u.off + tk + 1) - u.b0 * kTile;
+    }
+    for (int j = 0; j < n; ++j) {
+      const uint32_t s_col = tmem_base + lane_off + (MODE == kDq ? (j & 1) * 128 : 0);
+      const uint32_t dp_col = tmem_base + lane_off + kColDp;
+      ok = wait(MODE == kDq ? &ctl->s_full[j & 1] : &ctl->s_full[0], MODE == kDq ? (j >> 1) & 1 : j & 1, kDevWaitAccFull) &&
+           (MODE == kDq || wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitAccFull));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const float* st = stats + (j & 1) * 2 * kTile;
+      // the columns that the row sees: keys before its limit, or queries from `lo` on
+      int lo = 0, hi;
+      if (MODE == kDq) {
+        hi = limit - j * kTile;
+      } else {
+        const int tok0 = (u.b0 + j) * step;
+        lo = min(max(u.off + row - tok0, 0), step) * p.group;
+        hi = min(step, u.len - tok0) * p.group;
+      }
+      uint32_t vis[2] = {column_bits(lo, hi, c0), column_bits(lo, hi, c0 + 32)};
+      const bool all = __all_sync(0xffffffffu, (vis[0] & vis[1]) == 0xffffffffu);
+      float pr[64];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32];
+        tmem_ld32(s_col + c0 + c * 32, s);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float4 l = make_float4(lse2, lse2, lse2, lse2);
+          if (MODE == kDkv) l = *reinterpret_cast<const float4*>(st + c0 + c * 32 + i);
+          const float lv[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pr[c * 32 + i + e] = ex2_approx(fmaf(__uint_as_float(s[i + e]), c2, -lv[e]));
+        }
+        if (!all) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((vis[c] >> i) & 1u)) pr[c * 32 + i] = 0.f;
+        }
+      }
+      if (MODE == kDkv) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(pr[c * 16 + 2 * i], pr[c * 16 + 2 * i + 1]);
+          tmem_st8(s_col + c0 + c * 8, w);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->p_ready);
+      }
+      ok = wait(&ctl->dp_full, j & 1, kDevWaitAccFull);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t x[32];
+        tmem_ld32(dp_col + c0 + c * 32, x);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float4 dl = make_float4(delta, delta, delta, delta);
+          if (MODE == kDkv) dl = *reinterpret_cast<const float4*>(st + kTile + c0 + c * 32 + i);
+          const float dv[4] = {dl.x, dl.y, dl.z, dl.w};
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[e] = pr[c * 32 + i + e] * (__uint_as_float(x[i + e]) - dv[e]);
+            // (a selection: what lies behind the sequence may be infinite)
+            if (!all && !((vis[c] >> (i + e)) & 1u)) y[e] = 0.f;
+          }
+          w[c * 16 + i / 2] = pack_bf16x2(y[0], y[1]);
+          w[c * 16 + i / 2 + 1] = pack_bf16x2(y[2], y[3]);
+        }
+      }
+      tmem_st32((MODE == kDkv ? dp_col : s_col) + c0, w);      // dS over dP (kDkv) or over S (kDq)
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&ctl->ds_ready);
+        if (MODE == kDkv) mbar_arrive(&ctl->stat_empty[j & 1]);
+      }
+    }
+    if (ok && n > 0) ok = wait(&ctl->all_done, 0, kDevWaitPvDone);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    if (ok) {
+      // the gradients' columns: kDkv half 0 writes dV, half 1 dK; kDq each half of dQ's columns
+      constexpr int kCols = MODE == kDkv ? D : D / 2;
+      const uint32_t col = tmem_base + lane_off + kColG + half * kCols;
+      const bool divided = u.slot >= 0;
+      const bool is_dv = MODE == kDkv && half == 0;
+      const float f = is_dv ? 1.f : p.scale;
+      const int64_t token = u.t0 + tk;
+      const int head = MODE == kDkv ? kvh : kvh * p.group + row % p.group;
+      uint16_t* out = is_dv ? static_cast<uint16_t*>(p.g2) + token * p.g2_t + head * p.g2_h
+                            : static_cast<uint16_t*>(p.g1) + token * p.g1_t + head * p.g1_h;
+      constexpr int kWidth = MODE == kDkv ? 2 * D : D;
+      float* part = p.part + ((static_cast<int64_t>(divided ? u.slot : 0) * p.Hkv + kvh) * kTile + row) * kWidth + half * kCols;
+      const int ch0 = MODE == kDkv ? 0 : half * kCols;         // first channel
+#pragma unroll 1
+      for (int c = 0; c < kCols / 16; ++c) {
+        uint32_t o[16];
+        if (n > 0) {
+          tmem_ld16(col + c * 16, o);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = 0u;
+        }
+        if (!row_ok) continue;
+        if (divided) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4*>(part + c * 16 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i += 8) {
+            if (ch0 + c * 16 + i >= p.d) continue;
+            uint32_t w4[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              w4[q] = pack_bf16x2(__uint_as_float(o[i + 2 * q]) * f, __uint_as_float(o[i + 2 * q + 1]) * f);
+            *reinterpret_cast<uint4*>(out + ch0 + c * 16 + i) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    __syncwarp();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// delta = dO . O per row, and lse in powers of two; half a warp a row.
+__global__ void __launch_bounds__(256) packed_attn_delta_kernel(const __nv_bfloat16* o, int64_t os_t, int64_t os_h,
+                                                                const __nv_bfloat16* g, int64_t gs_t, int64_t gs_h,
+                                                                const float* lse, float2* stats, int64_t rows, int Tq,
+                                                                int tokens, int group, int d) {
+  const int sub = threadIdx.x & 15;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  if (r >= rows) return;                                       // (half warps leave together: the sums below stay inside one)
+  // rows in the order of the tiles: [kv head][token][head of the group]
+  const int hg = static_cast<int>(r % group);
+  const int64_t t = (r / group) % tokens;
+  const int kvh = static_cast<int>(r / group / tokens);
+  const int head = kvh * group + hg;
+  const int c = sub * 8;
+  float a = 0.f;
+  if (c < d) {
+    const uint4 x = *reinterpret_cast<const uint4*>(o + t * os_t + head * os_h + c);
+    const uint4 y = *reinterpret_cast<const uint4*>(g + t * gs_t + head * gs_h + c);
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), a);
+      a = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ys[i] & 0xffff0000u), a);
+    }
+  }
+  const uint32_t mask = 0xffffu << (threadIdx.x & 16);
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) a += __shfl_xor_sync(mask, a, off);
+  if (sub == 0) {
+    const float l = lse[static_cast<int64_t>(head) * Tq + t];
+    const float inf = __int_as_float(0x7f800000);
+    stats[(static_cast<int64_t>(kvh) * Tq + t) * group + hg] = make_float2(l == -inf ? inf : l * 1.4426950408889634f, a);
+  }
+}
+
+// Adds up the sums of divided units in the parts' order, one warp per row.
+template <int D, int MODE>
+__global__ void __launch_bounds__(256) packed_attn_bwd_join_kernel(const PackedJoin* joins, const PackedBwdParams p) {
+  constexpr int kWidth = MODE == kDkv ? 2 * D : D;
+  const PackedJoin jn = joins[blockIdx.x];
+  const int kvh = blockIdx.y, lane = threadIdx.x & 31;
+  const int rows = MODE == kDkv ? jn.n : jn.n * p.group;
+  const int64_t step = static_cast<int64_t>(p.Hkv) * kTile * kWidth;
+  for (int r = blockIdx.z * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.z * 8) {
+    const float* part = p.part + ((static_cast<int64_t>(jn.slot) * p.Hkv + kvh) * kTile + r) * kWidth;
+    const int64_t token = jn.t0 + (MODE == kDkv ? r : r / p.group);
+    const int head = MODE == kDkv ? kvh : kvh * p.group + r % p.group;
+#pragma unroll
+    for (int c = 0; c < kWidth / 32; ++c) {
+      const int ch = c * 32 + lane;
+      float a = 0.f;
+      for (int k = 0; k < jn.parts; ++k) a += part[k * step + ch];
+      const bool is_dv = MODE == kDkv && ch < D;
+      const int cd = MODE == kDkv ? ch % D : ch;
+      if (cd >= p.d) continue;
+      __nv_bfloat16* out = is_dv ? static_cast<__nv_bfloat16*>(p.g2) + token * p.g2_t + head * p.g2_h
+                                 : static_cast<__nv_bfloat16*>(p.g1) + token * p.g1_t + head * p.g1_h;
+      out[cd] = __float2bfloat16_rn(is_dv ? a : a * p.scale);
+    }
+  }
+}
+
+template <int D, int MODE>
+int launch_bwd(const CUtensorMap& l1, const CUtensorMap& l2, const CUtensorMap& a, const CUtensorMap& b,
+               const PackedBwdParams& p, const PackedJoin* joins, int n_join, cudaStream_t st) {
+  if (p.n_units == 0) return SWV_OK;
+  SWV_CUDA_OK(cudaFuncSetAttribute(packed_attn_bwd_kernel<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(bwd_smem<D, MODE>())));
+  packed_attn_bwd_kernel<D, MODE>
+      <<<static_cast<unsigned>(p.n_units) * p.Hkv, kBwdThreads, bwd_smem<D, MODE>(), st>>>(l1, l2, a, b, p);
+  SWV_CUDA_OK(cudaGetLastError());
+  if (n_join > 0) {
+    packed_attn_bwd_join_kernel<D, MODE><<<dim3(n_join, p.Hkv, 16), 256, 0, st>>>(joins, p);
+    SWV_CUDA_OK(cudaGetLastError());
+  }
+  return SWV_OK;
+}
+
+struct BwdSizes {
+  size_t stats, dq, dkv;
+};
+BwdSizes bwd_sizes(const PackedHeader& h, int64_t Tq, int D) {
+  const size_t Dk = D <= 64 ? 64 : 128;
+  BwdSizes s;
+  s.stats = (static_cast<size_t>(h.H) * Tq * sizeof(float2) + 255) / 256 * 256;
+  s.dq = static_cast<size_t>(h.dq_slots) * h.Hkv * kTile * Dk * sizeof(float);
+  s.dkv = static_cast<size_t>(h.dkv_slots) * h.Hkv * kTile * 2 * Dk * sizeof(float);
+  return s;
+}
+
+}  // namespace
+
+int packed_attn_bwd_bytes_impl(const int32_t* plan_host, int64_t Tq, int D, size_t* bytes) {
+  if (!plan_host || !bytes) return SWV_ERR_NULL;
+  PackedHeader h;
+  const int rc = packed_plan_header(plan_host, &h);
+  if (rc != SWV_OK) return rc;
+  if (Tq < h.Tq) return SWV_ERR_SHAPE;
+  if (D < 8 || D % 8 != 0 || D > 128) return SWV_ERR_UNSUPPORTED;
+  const BwdSizes s = bwd_sizes(h, Tq, D);
+  *bytes = s.stats + s.dq + s.dkv;
+  return SWV_OK;
+}
+
+int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, const int64_t* qs, const void* k,
+                         const int64_t* ks, const void* v, const int64_t* vs, const void* o, const int64_t* os,
+                         const float* lse, void* dq, const int64_t* dqs, void* dk, const int64_t* dks, void* dv,
+                         const int64_t* dvs, const int32_t* plan_host, const int32_t* plan, int64_t Tq, int64_t Tk, int D,
+                         float scale, void* workspace, size_t workspace_bytes, int* status, cudaStream_t st) {
+  if (!plan_host || !gs || !qs || !ks || !vs || !os || !dqs || !dks || !dvs) return SWV_ERR_NULL;
+  PackedHeader h;
+  int rc = packed_plan_header(plan_host, &h);
+  if (rc != SWV_OK) return rc;
+  if (Tq < h.Tq || Tk < h.Tk || Tq > 0x7fffffff || Tk > 0x7fffffff) return SWV_ERR_SHAPE;
+  if (!(scale > 0.f) || !std::isfinite(scale)) return SWV_ERR_SHAPE;
+  if (D < 8 || D % 8 != 0 || D > 128) return SWV_ERR_UNSUPPORTED;
+  if (h.Tq == 0 && h.Tk == 0) return SWV_OK;
+  if (!plan || !status || !workspace) return SWV_ERR_NULL;
+  if (h.Tq > 0 && (!d_out || !q || !o || !lse || !dq)) return SWV_ERR_NULL;
+  if (h.Tk > 0 && (!k || !v || !dk || !dv)) return SWV_ERR_NULL;
+  // one side empty: the maps need some memory, nothing reads it
+  if (h.Tq == 0) { q = d_out = o = k; qs = gs = os = ks; Tq = 1; }
+  if (h.Tk == 0) { k = v = q; ks = vs = qs; Tk = 1; }
+  if (!packed_aligned(q, qs, 2) || !packed_aligned(k, ks, 2) || !packed_aligned(v, vs, 2) || !packed_aligned(o, os, 2) ||
+      !packed_aligned(d_out, gs, 2))
+    return SWV_ERR_ALIGN;
+  if ((h.Tq > 0 && !packed_aligned(dq, dqs, 2)) ||
+      (h.Tk > 0 && (!packed_aligned(dk, dks, 2) || !packed_aligned(dv, dvs, 2))))
+    return SWV_ERR_ALIGN;
+  if (static_cast<int64_t>(std::max(h.n_dq, h.n_dkv)) * h.Hkv > 0x7fffffff || h.Hkv > 65535) return SWV_ERR_TOO_LARGE;
+  const BwdSizes sz = bwd_sizes(h, Tq, D);
+  if (workspace_bytes < sz.stats + sz.dq + sz.dkv) return SWV_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return SWV_ERR_ALIGN;
+
+  PackedBwdParams p{};
+  p.group = h.H / h.Hkv;
+  p.tok = kTile / p.group;
+  p.Tq = static_cast<int>(Tq); p.d = D; p.Hkv = h.Hkv;
+  p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = status;
+  float2* stats = static_cast<float2*>(workspace);
+  p.stats = stats;
+  if (h.Tq > 0) {
+    const int64_t rows = static_cast<int64_t>(h.H) * h.Tq;
+    packed_attn_delta_kernel<<<static_cast<unsigned>((rows + 15) / 16), 256, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(o), os[0], os[1], static_cast<const __nv_bfloat16*>(d_out), gs[0], gs[1], lse,
+        stats, rows, static_cast<int>(Tq), h.Tq, p.group, D);
+    SWV_CUDA_OK(cudaGetLastError());
+  }
+  CUtensorMap tq, tg, tk, tv;
+  if ((rc = packed_tmap(&tq, q, qs, Tq, h.Hkv, p.group, D, p.tok)) != SWV_OK) return rc;
+  if ((rc = packed_tmap(&tg, d_out, gs, Tq, h.Hkv, p.group, D, p.tok)) != SWV_OK) return rc;
+  if ((rc = packed_tmap(&tk, k, ks, Tk, h.Hkv, 0, D, kTile)) != SWV_OK) return rc;
+  if ((rc = packed_tmap(&tv, v, vs, Tk, h.Hkv, 0, D, kTile)) != SWV_OK) return rc;
+  uint8_t* w = static_cast<uint8_t*>(workspace) + sz.stats;
+
+  PackedBwdParams a = p;                                       // keys' side
+  a.units = reinterpret_cast<const PackedUnit*>(plan + h.dkv_off);
+  a.n_units = h.n_dkv;
+  a.g1 = dk; a.g1_t = dks[0]; a.g1_h = dks[1];
+  a.g2 = dv; a.g2_t = dvs[0]; a.g2_h = dvs[1];
+  a.part = reinterpret_cast<float*>(w + sz.dq);
+  const PackedJoin* ja = reinterpret_cast<const PackedJoin*>(plan + h.dkv_join_off);
+  rc = D <= 64 ? launch_bwd<64, kDkv>(tk, tv, tq, tg, a, ja, h.n_dkv_join, st)
+               : launch_bwd<128, kDkv>(tk, tv, tq, tg, a, ja, h.n_dkv_join, st);
+  if (rc != SWV_OK) return rc;
+  PackedBwdParams b = p;                                       // queries' side
+  b.units = reinterpret_cast<const PackedUnit*>(plan + h.dq_off);
+  b.n_units = h.n_dq;
+  b.g1 = dq; b.g1_t = dqs[0]; b.g1_h = dqs[1];
+  b.part = reinterpret_cast<float*>(w);
+  const PackedJoin* jb = reinterpret_cast<const PackedJoin*>(plan + h.dq_join_off);
+  return D <= 64 ? launch_bwd<64, kDq>(tq, tg, tk, tv, b, jb, h.n_dq_join, st)
+                 : launch_bwd<128, kDq>(tq, tg, tk, tv, b, jb, h.n_dq_join, st);
+}
+
+}  // namespace swv

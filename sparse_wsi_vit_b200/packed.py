@@ -244,14 +244,12 @@ class PackedPlan:
         self._table = torch.from_numpy(self._host).to(self.device)      # (waits for the copy: any stream may use it)
         self._bytes = {}
 
-    def bytes_for(self, D, backward=False):
-        key = (D, backward)
-        if key not in self._bytes:
+    def _workspace_bytes(self, D):
+        if D not in self._bytes:
             n = ctypes.c_size_t()
-            f = lib.swv_packed_attn_bwd_bytes if backward else lib.swv_packed_attn_bytes
-            check(f(self._host.ctypes.data, D, ctypes.byref(n)), "swv_packed_attn_bytes")
-            self._bytes[key] = n.value
-        return self._bytes[key]
+            check(lib.swv_packed_attn_bytes(self._host.ctypes.data, D, ctypes.byref(n)), "swv_packed_attn_bytes")
+            self._bytes[D] = n.value
+        return self._bytes[D]
 
 
 def _rows_ok(t):
@@ -296,7 +294,7 @@ def _attn_fwd(q, k, v, plan, scale, want_lse, out=None):
         lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev)
         if plan.q_tokens < q.shape[0]:
             lse[:, plan.q_tokens:].fill_(-float("inf"))
-    nws = plan.bytes_for(D)
+    nws = plan._workspace_bytes(D)
     ws = _workspace(dev, nws) if nws else None
     with _on(dev):
         check(lib.swv_packed_attn_fwd(q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v),
@@ -306,6 +304,43 @@ def _attn_fwd(q, k, v, plan, scale, want_lse, out=None):
     if _CHECK:
         check_status(dev, "swv_packed_attn_fwd")
     return o, lse
+
+
+class PackedAttentionFunction(torch.autograd.Function):
+    """``packed_attention`` with its gradients (no atomics: the same bits every time); the log-sum-exp of the rows is
+    kept for the backward pass."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, plan, scale):
+        o, lse = _attn_fwd(q, k, v, plan, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.plan, ctx.scale = plan, scale
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out, _):
+        q, k, v, o, lse = ctx.saved_tensors
+        plan, dev, D = ctx.plan, q.device, q.shape[2]
+        q, k, v, d_out = _aligned(q), _aligned(k), _aligned(v), _aligned(d_out)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        for n, ts in ((plan.q_tokens, (dq,)), (plan.k_tokens, (dk, dv))):
+            for t in ts:
+                if n < t.shape[0]:
+                    t[n:].zero_()                         # rows behind the last sequence
+        n = ctypes.c_size_t()
+        check(lib.swv_packed_attn_bwd_bytes(plan._host.ctypes.data, q.shape[0], D, ctypes.byref(n)), "swv_packed_attn_bwd_bytes")
+        ws = _workspace(dev, n.value)
+        with _on(dev):
+            check(lib.swv_packed_attn_bwd(
+                d_out.data_ptr(), strides(d_out), q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(),
+                strides(v), o.data_ptr(), strides(o), lse.data_ptr(), dq.data_ptr(), strides(dq), dk.data_ptr(), strides(dk),
+                dv.data_ptr(), strides(dv), plan._host.ctypes.data, plan._table.data_ptr(), q.shape[0], k.shape[0], D,
+                ctx.scale, ws.data_ptr(), n.value, status_word(dev).data_ptr(), _stream(dev)), "swv_packed_attn_bwd")
+        if _CHECK:
+            check_status(dev, "swv_packed_attn_bwd")
+        return dq, dk, dv, None, None
 
 
 def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
@@ -320,5 +355,11 @@ def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise SwvError("scale must be positive and finite")
-    o, lse = _attn_fwd(q, k, v, plan, scale, return_lse, out)
+    grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
+    if out is not None:
+        if grad:
+            raise SwvError("packed_attention writes into `out` only where no gradient is asked for")
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not _rows_ok(out):
+            raise SwvError("out must have q's shape, type and device, and rows on 16 bytes")
+    o, lse = PackedAttentionFunction.apply(q, k, v, plan, scale) if grad else _attn_fwd(q, k, v, plan, scale, return_lse, out)
     return (o, lse) if return_lse else o
