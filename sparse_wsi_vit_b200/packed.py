@@ -12,27 +12,40 @@ calls that the kernels do not serve.  The reference's dense ViT-5 has the same p
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import numpy as np
 import torch
 
-from ._lib import SwvError, check, dtype_code, lib, strides
-from .ops import _CHECK, _require_cuda, _stream, _workspace, check_status, status_word
+from ._lib import SwvError, check, dtype_code, lib
+from .ops import _CHECK, _require_cuda, check_status, status_word
 
 _POS_CODES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_I3 = ctypes.c_int64 * 3
+_raw_stream = torch._C._cuda_getCurrentRawStream        # (torch.cuda.current_stream builds an object: 2 us a call)
 
 
-def _on(dev):
-    """Launches go to the inputs' device, whichever one is current."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _call(fn, what, dev, *args):
+    """One call of the library on the current stream of ``dev`` (its last argument), whichever device is current."""
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(i))
+    if rc != 0:
+        check(rc, what)
+    if _CHECK:
+        check_status(dev, what)
 
 
-def _same_device(*ts):
-    _require_cuda(*ts)
-    if any(t.device != ts[0].device for t in ts):
-        raise SwvError("all tensors of a call must be on one device")
+def _same_device(first, *ts):
+    dev = first.device
+    _require_cuda(first)
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise SwvError("all tensors of a call must be on one device")
 
 
 # --------------------------------------------------------------------------- #
@@ -43,29 +56,31 @@ def _ptr(t):
 
 
 def _code(t):
-    return 0 if t is None else dtype_code(t.dtype)
+    return 0 if t is None else _DTYPES[t.dtype]
 
 
 def _rows2d(t):
     """``t`` as rows of its last dimension: a view where the rows are evenly spaced, else a copy."""
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         t = t.contiguous()
     return t.reshape(-1, t.shape[-1])
 
 
 def _norm_fwd(x, weight, bias, eps, out_dtype, want_stats):
-    E = x.shape[-1]
+    E, dev = x.shape[-1], x.device
     x2 = _rows2d(x)
     N = x2.shape[0]
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    mean = rstd = None
+    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    stats = mean = rstd = None
     if want_stats:
-        mean, rstd = torch.empty((2, N), dtype=torch.float32, device=x.device).unbind(0)
-    with _on(x.device):
-        check(lib.swv_layer_norm_fwd(x2.data_ptr(), x2.stride(0), dtype_code(x.dtype), _ptr(weight), _code(weight), _ptr(bias),
-                                     _code(bias), y.data_ptr(), E, dtype_code(out_dtype), _ptr(mean), _ptr(rstd), N, E, eps,
-                                     _stream(x.device)), "swv_layer_norm_fwd")
-    return y, mean, rstd
+        stats = torch.empty(2 * N, dtype=torch.float32, device=dev)      # mean, rstd
+        mean = stats.data_ptr()
+        rstd = mean + 4 * N
+    _call(lib.swv_layer_norm_fwd, "swv_layer_norm_fwd", dev, x2.data_ptr(), x2.stride(0), _DTYPES[x.dtype], _ptr(weight),
+          _code(weight), _ptr(bias), _code(bias), y.data_ptr(), E, _DTYPES[out_dtype], mean, rstd, N, E, eps)
+    return y, stats
 
 
 class LayerNormFunction(torch.autograd.Function):
@@ -73,32 +88,38 @@ class LayerNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype):
-        y, mean, rstd = _norm_fwd(x, weight, bias, eps, out_dtype, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats = _norm_fwd(x, weight, bias, eps, out_dtype, True)
+        ctx.save_for_backward(x, weight, stats)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
         E, dev = x.shape[-1], x.device
         x2, dy2 = _rows2d(x), _rows2d(dy)
         N = x2.shape[0]
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dw = torch.empty(E, dtype=weight.dtype, device=dev) if weight is not None and ctx.needs_input_grad[1] else None
-        db = torch.empty(E, dtype=ctx.bias_dtype, device=dev) if ctx.bias_dtype is not None and ctx.needs_input_grad[2] else None
-        n = ctypes.c_size_t()
-        ws = None
-        if dw is not None or db is not None:
-            check(lib.swv_layer_norm_bwd_bytes(N, E, ctypes.byref(n)), "swv_layer_norm_bwd_bytes")
-            ws = _workspace(dev, n.value)
-        with _on(dev):
-            check(lib.swv_layer_norm_bwd(dy2.data_ptr(), dy2.stride(0), dtype_code(dy.dtype), x2.data_ptr(), x2.stride(0),
-                                         dtype_code(x.dtype), _ptr(weight), _code(weight), mean.data_ptr(), rstd.data_ptr(),
-                                         dx.data_ptr(), E, _ptr(dw), _code(dw), _ptr(db), _code(db), N, E, _ptr(ws), n.value,
-                                         _stream(dev)), "swv_layer_norm_bwd")
+        _, want_w, want_b, _, _ = ctx.needs_input_grad
+        dw = torch.empty(E, dtype=weight.dtype, device=dev) if want_w else None
+        db = torch.empty(E, dtype=ctx.bias_dtype, device=dev) if want_b else None
+        ws, nws = None, ctypes.c_size_t()
+        if want_w or want_b:
+            check(lib.swv_layer_norm_bwd_bytes(N, E, ctypes.byref(nws)), "swv_layer_norm_bwd_bytes")
+            ws = torch.empty(nws.value, dtype=torch.uint8, device=dev)
+        mean = stats.data_ptr()
+        _call(lib.swv_layer_norm_bwd, "swv_layer_norm_bwd", dev, dy2.data_ptr(), dy2.stride(0), _DTYPES[dy.dtype],
+              x2.data_ptr(), x2.stride(0), _DTYPES[x.dtype], _ptr(weight), _code(weight), mean, mean + 4 * N, dx.data_ptr(), E,
+              _ptr(dw), _code(dw), _ptr(db), _code(db), N, E, _ptr(ws), nws.value)
         return dx, dw, db, None, None
+
+
+def _norm_param(t, name, x):
+    if t.dim() != 1 or t.shape[0] != x.shape[-1]:
+        raise SwvError(f"{name} has shape {tuple(t.shape)}, expected {(x.shape[-1],)}")
+    dtype_code(t.dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
@@ -107,19 +128,22 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     ``x`` fp32, bf16 or fp16; ``weight`` and ``bias`` (E,) of any of the three types, or None.  The statistics and all
     sums are fp32.  ``out_dtype``: x's type (the default) or fp32, for an fp32 ``x`` any of the three.  Rows may be evenly
     spaced views; other layouts are copied."""
-    _same_device(*(t for t in (x, weight, bias) if t is not None))
-    out_dtype = out_dtype or x.dtype
-    for t in (x.dtype, out_dtype):
-        dtype_code(t)
+    _same_device(x, weight, bias)
+    dt = x.dtype
+    out_dtype = out_dtype or dt
+    dtype_code(dt), dtype_code(out_dtype)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise SwvError("layer_norm needs a last dimension of one value or more")
-    if x.dtype != torch.float32 and out_dtype not in (x.dtype, torch.float32):
-        raise SwvError(f"layer_norm of {x.dtype} gives {x.dtype} or float32, not {out_dtype}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and tuple(t.shape) != (x.shape[-1],):
-            raise SwvError(f"{name} has shape {tuple(t.shape)}, expected {(x.shape[-1],)}")
-    weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if out_dtype != dt and dt != torch.float32 and out_dtype != torch.float32:
+        raise SwvError(f"layer_norm of {dt} gives {dt} or float32, not {out_dtype}")
+    grad = x.requires_grad
+    if weight is not None:
+        weight = _norm_param(weight, "weight", x)
+        grad = grad or weight.requires_grad
+    if bias is not None:
+        bias = _norm_param(bias, "bias", x)
+        grad = grad or bias.requires_grad
+    if grad and torch.is_grad_enabled():
         return LayerNormFunction.apply(x, weight, bias, float(eps), out_dtype)
     return _norm_fwd(x, weight, bias, float(eps), out_dtype, False)[0]
 
@@ -153,6 +177,7 @@ class RopeAxes:
         power = [(sum(sections[:a]) + i) / R if ladder == "head" else i / n for a, n in enumerate(sections) for i in range(n)]
         self._axis = np.repeat(np.arange(len(sections)), sections).astype(np.uint8)
         self._freq = np.asarray(scales)[self._axis] * np.float64(theta) ** -np.asarray(power, dtype=np.float64)
+        self._call = (self._freq.ctypes.data, self._axis.ctypes.data, R, len(sections), int(self.halves))
 
 
 def _rope_apply(x, positions, rope, inverse, out=None):
@@ -160,12 +185,9 @@ def _rope_apply(x, positions, rope, inverse, out=None):
     if x.stride(2) != 1:
         x = x.contiguous()
     y = torch.empty((T, H, hd), dtype=x.dtype, device=x.device) if out is None else out
-    s3 = lambda t: (ctypes.c_int64 * 3)(*t.stride())
-    with _on(x.device):
-        check(lib.swv_rope_axes_apply(x.data_ptr(), s3(x), y.data_ptr(), s3(y), dtype_code(x.dtype), positions.data_ptr(),
-                                      _POS_CODES[positions.dtype], positions.stride(0), rope._freq.ctypes.data,
-                                      rope._axis.ctypes.data, rope.pairs, len(rope.sections), int(rope.halves), int(inverse),
-                                      T, H, hd, _stream(x.device)), "swv_rope_axes_apply")
+    _call(lib.swv_rope_axes_apply, "swv_rope_axes_apply", x.device, x.data_ptr(), _I3(*x.stride()), y.data_ptr(),
+          _I3(*y.stride()), _DTYPES[x.dtype], positions.data_ptr(), _POS_CODES[positions.dtype], positions.stride(0),
+          *rope._call, inverse, T, H, hd)
     return y
 
 
@@ -242,6 +264,7 @@ class PackedPlan:
         check(rc, "swv_packed_plan")
         self._host = words[: size.value // 4].copy()
         self._table = torch.from_numpy(self._host).to(self.device)      # (waits for the copy: any stream may use it)
+        self._call = (self._host.ctypes.data, self._table.data_ptr())
         self._bytes = {}
 
     def _workspace_bytes(self, D):
@@ -253,7 +276,8 @@ class PackedPlan:
 
 
 def _rows_ok(t):
-    return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and min(t.stride()) > 0
+    a, b, c = t.stride()
+    return c == 1 and a > 0 and b > 0 and not ((a | b) & 7 or t.data_ptr() & 15)
 
 
 def _aligned(t):
@@ -267,42 +291,40 @@ def _attn_check(q, k, v, plan):
         raise SwvError("packed_attention needs a PackedPlan")
     if plan.device != q.device:
         raise SwvError(f"the plan is on {plan.device}, the tensors on {q.device}")
-    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+    bf16 = torch.bfloat16
+    if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
         raise SwvError("packed_attention needs bf16 q, k and v")
-    if any(t.dim() != 3 for t in (q, k, v)) or k.shape != v.shape or k.shape[2] != q.shape[2]:
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
         raise SwvError("packed_attention takes q (Tq, heads, D) and k, v (Tk, kv_heads, D)")
-    if q.shape[1] != plan.heads or k.shape[1] != plan.kv_heads:
-        raise SwvError(f"{q.shape[1]} and {k.shape[1]} heads, the plan is for {plan.heads} and {plan.kv_heads}")
-    if q.shape[0] < plan.q_tokens or k.shape[0] < plan.k_tokens:
-        raise SwvError(f"{q.shape[0]} query and {k.shape[0]} key tokens, the plan's sequences have {plan.q_tokens} and "
+    Tq, H, D = q.shape
+    if H != plan.heads or k.shape[1] != plan.kv_heads:
+        raise SwvError(f"{H} and {k.shape[1]} heads, the plan is for {plan.heads} and {plan.kv_heads}")
+    if Tq < plan.q_tokens or k.shape[0] < plan.k_tokens:
+        raise SwvError(f"{Tq} query and {k.shape[0]} key tokens, the plan's sequences have {plan.q_tokens} and "
                        f"{plan.k_tokens}")
-    D = q.shape[2]
     if D % 8 or not 8 <= D <= 128:
         raise SwvError(f"packed_attention supports head dimensions that are multiples of 8 up to 128, not {D}")
 
 
 def _attn_fwd(q, k, v, plan, scale, want_lse, out=None):
-    dev, D = q.device, q.shape[2]
+    dev = q.device
+    Tq, H, D = q.shape
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     o = out
     if o is None:
-        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        if plan.q_tokens < q.shape[0]:
+        o = torch.empty((Tq, H, D), dtype=torch.bfloat16, device=dev)
+        if plan.q_tokens < Tq:
             o[plan.q_tokens:].zero_()                     # rows behind the last sequence
     lse = None
     if want_lse:
-        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev)
-        if plan.q_tokens < q.shape[0]:
+        lse = torch.empty((H, Tq), dtype=torch.float32, device=dev)
+        if plan.q_tokens < Tq:
             lse[:, plan.q_tokens:].fill_(-float("inf"))
     nws = plan._workspace_bytes(D)
-    ws = _workspace(dev, nws) if nws else None
-    with _on(dev):
-        check(lib.swv_packed_attn_fwd(q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(), strides(v),
-                                      o.data_ptr(), strides(o), _ptr(lse), plan._host.ctypes.data, plan._table.data_ptr(),
-                                      q.shape[0], k.shape[0], D, scale, _ptr(ws), nws, status_word(dev).data_ptr(),
-                                      _stream(dev)), "swv_packed_attn_fwd")
-    if _CHECK:
-        check_status(dev, "swv_packed_attn_fwd")
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _call(lib.swv_packed_attn_fwd, "swv_packed_attn_fwd", dev, q.data_ptr(), _I3(*q.stride()), k.data_ptr(),
+          _I3(*k.stride()), v.data_ptr(), _I3(*v.stride()), o.data_ptr(), _I3(*o.stride()), _ptr(lse), *plan._call, Tq,
+          k.shape[0], D, scale, _ptr(ws), nws, status_word(dev).data_ptr())
     return o, lse
 
 
@@ -324,22 +346,21 @@ class PackedAttentionFunction(torch.autograd.Function):
         q, k, v, o, lse = ctx.saved_tensors
         plan, dev, D = ctx.plan, q.device, q.shape[2]
         q, k, v, d_out = _aligned(q), _aligned(k), _aligned(v), _aligned(d_out)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        for n, ts in ((plan.q_tokens, (dq,)), (plan.k_tokens, (dk, dv))):
-            for t in ts:
-                if n < t.shape[0]:
-                    t[n:].zero_()                         # rows behind the last sequence
+        Tq, Tk = q.shape[0], k.shape[0]
+        dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
+        if plan.q_tokens < Tq:                            # rows behind the last sequence
+            dq[plan.q_tokens:].zero_()
+        if plan.k_tokens < Tk:
+            dk[plan.k_tokens:].zero_()
+            dv[plan.k_tokens:].zero_()
         n = ctypes.c_size_t()
-        check(lib.swv_packed_attn_bwd_bytes(plan._host.ctypes.data, q.shape[0], D, ctypes.byref(n)), "swv_packed_attn_bwd_bytes")
-        ws = _workspace(dev, n.value)
-        with _on(dev):
-            check(lib.swv_packed_attn_bwd(
-                d_out.data_ptr(), strides(d_out), q.data_ptr(), strides(q), k.data_ptr(), strides(k), v.data_ptr(),
-                strides(v), o.data_ptr(), strides(o), lse.data_ptr(), dq.data_ptr(), strides(dq), dk.data_ptr(), strides(dk),
-                dv.data_ptr(), strides(dv), plan._host.ctypes.data, plan._table.data_ptr(), q.shape[0], k.shape[0], D,
-                ctx.scale, ws.data_ptr(), n.value, status_word(dev).data_ptr(), _stream(dev)), "swv_packed_attn_bwd")
-        if _CHECK:
-            check_status(dev, "swv_packed_attn_bwd")
+        check(lib.swv_packed_attn_bwd_bytes(plan._call[0], Tq, D, ctypes.byref(n)), "swv_packed_attn_bwd_bytes")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        dqs, dks = _I3(*dq.stride()), _I3(*dk.stride())
+        _call(lib.swv_packed_attn_bwd, "swv_packed_attn_bwd", dev, d_out.data_ptr(), _I3(*d_out.stride()), q.data_ptr(),
+              _I3(*q.stride()), k.data_ptr(), _I3(*k.stride()), v.data_ptr(), _I3(*v.stride()), o.data_ptr(), dqs,
+              lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dks, *plan._call, Tq, Tk, D, ctx.scale,
+              ws.data_ptr(), n.value, status_word(dev).data_ptr())
         return dq, dk, dv, None, None
 
 
@@ -355,7 +376,7 @@ def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise SwvError("scale must be positive and finite")
-    grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
+    grad = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
     if out is not None:
         if grad:
             raise SwvError("packed_attention writes into `out` only where no gradient is asked for")
