@@ -12,11 +12,14 @@
 //   warp 3      : zeroes the value rows behind the sequence's end in its last tile (they belong to the next sequence
 //                 or to nobody, and 0 x NaN would reach O)
 //   warps 4..7 and 8..11 : softmax of tile A and of tile B, one thread per row: the row's 128 scores are read into registers,
-//                 P is written as bf16 pairs over the first half of the score columns, in two halves, so that P V
+//                 P is written as bf16 pairs, in two halves, so that P V
 //                 starts under the second half's exponentials.  P is rounded to bf16 because the product takes
 //                 16-bit operands (2^-9 of each, independent); l sums the unrounded values.
 //                 The stabiliser is raised (and O in TMEM rescaled) only when a row's maximum exceeds it by 2^8.
-// TMEM: S_A [0,128), S_B [128,256), O_A [256,256+D), O_B [256+D,256+2D).
+// The scores' slot is free as soon as they are in registers, so S = Q K(j+1)^T is formed while the exponentials of block j run
+// (D = 128 has one slot for both tiles in turn); P has columns of its own.
+// TMEM: D = 128: S [0,128), P_A, P_B [128,256), O_A [256,384), O_B [384,512)
+//       D = 64:  S_A, S_B [0,256), P_A, P_B [256,384), O_A [384,448), O_B [448,512)
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -47,12 +50,17 @@ struct FwdCfg {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kStages = D == 128 ? 4 : 8;
   static constexpr int kOffRing = 2 * kTileBytes;
+  // TMEM columns
+  static constexpr int kSlots = D == 128 ? 1 : 2;             // score slots: one for both tiles in turn, or one each
+  static constexpr uint32_t kColP = kSlots * 128;             // P of tile A, of tile B: 64 columns of bf16 pairs each
+  static constexpr uint32_t kColO = kColP + 128;
   static constexpr int kOffCtl = kOffRing + kStages * kTileBytes;
 };
 struct FwdCtl {
   uint64_t q_full[2];
   uint64_t full[8], empty[8];
-  uint64_t s_full[2], p_full[2][2], pv_done[2];
+  uint64_t s_full[2], s_read[2], p_full[2][2], pv_done[2];
+  uint64_t exp_done[2][4];                  // a warp's exponentials of a tile are through
   uint64_t tail_full;                       // the last value block of the sequence, before it is cleaned
   uint32_t tmem_base, abort_flag;
 };
@@ -110,9 +118,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&ctl->q_full[t], 1);
       mbar_init(&ctl->s_full[t], 1);
+      mbar_init(&ctl->s_read[t], 4);
       mbar_init(&ctl->p_full[t][0], 4);
       mbar_init(&ctl->p_full[t][1], 4);
       mbar_init(&ctl->pv_done[t], 1);
+      for (int q = 0; q < 4; ++q) mbar_init(&ctl->exp_done[t][q], 1);
     }
     for (int s = 0; s < NST; ++s) {
       mbar_init(&ctl->full[s], 1);
@@ -164,11 +174,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   } else if (warp <= 2) {
     // ---------------------------------------------- one MMA issuer for each tile
     const int t = warp - 1;
-    const int nt = blocks(t);
+    const int nt = blocks(t), nother = blocks(1 - t);
     if (lane == 0 && n > 0) {
       const uint32_t q_addr = smem_u32(smem + t * Cfg::kTileBytes);
       const uint32_t ring = smem_u32(smem + Cfg::kOffRing);
-      const uint32_t s_col = tmem_base + t * kTile, o_col = tmem_base + 2 * kTile + t * D;
+      const uint32_t s_col = tmem_base + (t % Cfg::kSlots) * kTile, p_col = tmem_base + Cfg::kColP + t * 64;
+      const uint32_t o_col = tmem_base + Cfg::kColO + t * D;
       bool ok = nt == 0 || mbar_wait_bounded(&ctl->q_full[t], 0, abort_flag);
       if (!ok) record_status(p.status, kDevWaitQ);
       auto landed = [&](int it) {
@@ -179,8 +190,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       auto scores = [&](int j) {
         const int it = 2 * j, s = it % NST;
         if (!landed(it)) return false;
-        if (j > 0 && !mbar_wait_bounded(&ctl->pv_done[t], (j - 1) & 1, abort_flag)) {   // (P(j-1) lies in these columns)
-          record_status(p.status, kDevWaitPvDone);
+        // The slot's last scores have been read.  One slot: its users are A(0), B(0), A(1), ... until one tile has
+        // no more blocks; two slots: the tile's own last block.
+        const int before = Cfg::kSlots == 1 && j - 1 + t < nother ? j - 1 + t : j - 1;
+        const int whose = Cfg::kSlots == 1 && j - 1 + t < nother ? 1 - t : t;
+        if (before >= 0 && !mbar_wait_bounded(&ctl->s_read[whose], before & 1, abort_flag)) {
+          record_status(p.status, kDevWaitAccEmpty);
           return false;
         }
         tc_fence_after();
@@ -196,6 +211,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       };
       if (ok && nt > 0) ok = scores(0);
       for (int j = 0; ok && j < nt; ++j) {
+        if (j + 1 < nt) ok = scores(j + 1);                  // a block ahead of P V
+        if (!ok) break;
         const int it = 2 * j + 1, s = it % NST;
         if (!landed(it)) break;
         const uint64_t dv = smem_desc_sw128(ring + s * Cfg::kTileBytes, kTile * 128);
@@ -209,12 +226,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           tc_fence_after();
 #pragma unroll
           for (int ks = half * 4; ks < half * 4 + 4; ++ks)
-            umma_f16_ts(o_col, s_col + ks * 8, dv + ks * 128, kIdescPV, (j > 0 || ks > 0));
+            umma_f16_ts(o_col, p_col + ks * 8, dv + ks * 128, kIdescPV, (j > 0 || ks > 0));
         }
         if (!ok) break;
         umma_commit(&ctl->empty[s]);
         umma_commit(&ctl->pv_done[t]);
-        if (j + 1 < nt) ok = scores(j + 1);
       }
       // blocks that only the other tile needs (a stage is given back in the phase in which it was filled)
       for (int it = 2 * nt; ok && it < 2 * n; ++it) {
@@ -241,7 +257,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   } else {
     // ----------------------------------------------------------------- softmax
     const int t = (warp - 4) >> 2;
-    const int nt = blocks(t);
+    const int nt = blocks(t), nother = blocks(1 - t);
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int rows = tokens(t) * p.group;
@@ -250,8 +266,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const int tk = row / p.group;                            // token of the tile
     const int limit = row_ok ? min(u.len, u.off + t * p.tok + tk + 1) - u.b0 * kTile : 0;   // keys it sees from block b0 on
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_col = tmem_base + lane_off + t * kTile;
-    const uint32_t o_col = tmem_base + lane_off + 2 * kTile + t * D;
+    const uint32_t s_col = tmem_base + lane_off + (t % Cfg::kSlots) * kTile;
+    const uint32_t p_col = tmem_base + lane_off + Cfg::kColP + t * 64;
+    const uint32_t o_col = tmem_base + lane_off + Cfg::kColO + t * D;
+    const bool other_live = quarter * 32 < tokens(1 - t) * p.group;
     const float sc = p.scale_log2;
     const float ninf = -__int_as_float(0x7f800000);
     float m_used = ninf;
@@ -265,11 +283,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
+      uint32_t s[kTile];
       if (live) {
-        uint32_t s[kTile];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(s_col + c * 32, *reinterpret_cast<uint32_t(*)[32]>(s + c * 32));
         tc_wait_ld();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->s_read[t]);
+      // P V(j-1) has retired: P's columns are free, O may be rescaled
+      auto retired = [&]() {
+        bool r = j == 0 || mbar_wait_bounded(&ctl->pv_done[t], (j - 1) & 1, abort_flag);
+        if (!r) record_status(p.status, kDevWaitPvDone);
+        r = __all_sync(0xffffffffu, r);
+        tc_fence_after();
+        return r;
+      };
+      if (live) {
         const int vis = limit - j * kTile;                   // the first `vis` columns are seen
         if (__any_sync(0xffffffffu, vis < kTile)) {
 #pragma unroll
@@ -289,12 +320,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           m3 = max_of3(m3, __uint_as_float(s[i + 6]), __uint_as_float(s[i + 7]));
         }
         const float m_new = fmaxf(m_used, fmaxf(max_of3(m0, m1, m2), m3) * sc);
+        ok = retired();
+        if (!ok) break;
         if (__any_sync(0xffffffffu, m_new > m_used + kStep)) {
           const float factor = (m_new == m_used) ? 1.f : ex2_approx(m_used - m_new);
           lh[0] *= factor;
           lh[1] *= factor;
           m_used = m_new;
-          if (j > 0) {                                       // (S(j) ready: P V(j-1) has retired, the issuer waited for it)
+          if (j > 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
@@ -308,6 +341,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         // A row that sees no key has probabilities of zero; one whose scores are all -inf comes out NaN (-inf + inf).
         const float neg_m = limit > 0 ? -m_used : 0.f;
+        // The two tiles take turns at the exponentials, A(0), B(0), A(1), ...: in step with each other they would both
+        // wait for the tensor cores and then share the exponential unit.  (The warps of a quarter share a scheduler.)
+        const int turn = j - 1 + t;                          // the other tile's block whose turn was before this one's
+        if (other_live && turn >= 0 && turn < nother && !mbar_wait_bounded(&ctl->exp_done[1 - t][quarter], turn & 1, abort_flag)) {
+          record_status(p.status, kDevWaitPReady);
+          ok = false;
+        }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           float l0 = 0.f, l1 = 0.f;
@@ -323,17 +363,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
               add2(l0, l1, x0, x1);
               packed[i >> 1] = pack_bf16x2(x0, x1);
             }
-            tmem_st8(s_col + v * 8, packed);
+            tmem_st8(p_col + v * 8, packed);
           }
           lh[half] += l0 + l1;
+          if (half == 1 && lane == 0) mbar_arrive(&ctl->exp_done[t][quarter]);
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl->p_full[t][half]);
         }
-      } else if (lane == 0) {
-        mbar_arrive(&ctl->p_full[t][0]);
-        mbar_arrive(&ctl->p_full[t][1]);
+      } else {
+        ok = retired();                                      // (not ahead of the others' P of block j - 1)
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive(&ctl->p_full[t][0]);
+          mbar_arrive(&ctl->p_full[t][1]);
+        }
       }
     }
     if (nt > 0 && ok && !mbar_wait_bounded(&ctl->pv_done[t], (nt - 1) & 1, abort_flag)) {
