@@ -32,6 +32,13 @@ struct PackedUnit {
   int t0, n, s0, len, off, b0, b1;
   int slot;                               // where a divided unit leaves its sums; -1: it writes its rows itself
 };
+// Registers of the calling warpgroup (all four warps execute it); the block's shares add up to no more than its
+// registers at launch.
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 struct PackedJoin {                       // the slots [slot, slot + parts) are sums of the rows t0 .. t0 + n - 1
   int t0, n, slot, parts;
 };

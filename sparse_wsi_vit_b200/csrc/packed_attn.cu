@@ -142,6 +142,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const uint32_t tmem_base = ctl->tmem_base;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
 
+  // Registers: launched with 384 x 168 = 64512; 128 x 80 + 256 x 208 = 63488 after the exchange.
+  if (warp < 4) {
+  reg_dec<80>();
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (ok) mbar_arrive(&ctl->empty[it % NST]);
       }
     }
-  } else if (warp == 3) {
+  } else {
     if (tail) {
       const int s = (2 * n - 1) % NST;
       bool ok = mbar_wait_bounded(&ctl->tail_full, 0, abort_flag);
@@ -254,8 +257,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (lane == 0) mbar_arrive(&ctl->full[s]);
       }
     }
+  }
   } else {
     // ----------------------------------------------------------------- softmax
+    reg_inc<208>();
     const int t = (warp - 4) >> 2;
     const int nt = blocks(t), nother = blocks(1 - t);
     const int quarter = warp & 3;
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const float sc = p.scale_log2;
     const float ninf = -__int_as_float(0x7f800000);
     float m_used = ninf;
-    float lh[2] = {0.f, 0.f};
+    float l = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
       if (!mbar_wait_bounded(&ctl->s_full[t], j & 1, abort_flag)) {
@@ -324,8 +329,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (!ok) break;
         if (__any_sync(0xffffffffu, m_new > m_used + kStep)) {
           const float factor = (m_new == m_used) ? 1.f : ex2_approx(m_used - m_new);
-          lh[0] *= factor;
-          lh[1] *= factor;
+          l *= factor;
           m_used = m_new;
           if (j > 0) {
 #pragma unroll 1
@@ -348,30 +352,29 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           record_status(p.status, kDevWaitPReady);
           ok = false;
         }
+        float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float l0 = 0.f, l1 = 0.f;
+        for (int v = 0; v < 8; ++v) {
+          uint32_t packed[8];
 #pragma unroll
-          for (int v = half * 4; v < half * 4 + 4; ++v) {
-            uint32_t packed[8];
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float x0, x1;
-              fma2(x0, x1, __uint_as_float(s[v * 16 + i]), __uint_as_float(s[v * 16 + i + 1]), sc, neg_m);
-              x0 = ex2_approx(x0);
-              x1 = ex2_approx(x1);
-              add2(l0, l1, x0, x1);
-              packed[i >> 1] = pack_bf16x2(x0, x1);
-            }
-            tmem_st8(p_col + v * 8, packed);
+          for (int i = 0; i < 16; i += 2) {
+            float x0, x1;
+            fma2(x0, x1, __uint_as_float(s[v * 16 + i]), __uint_as_float(s[v * 16 + i + 1]), sc, neg_m);
+            x0 = ex2_approx(x0);
+            x1 = ex2_approx(x1);
+            add2(l0, l1, x0, x1);
+            packed[i >> 1] = pack_bf16x2(x0, x1);
           }
-          lh[half] += l0 + l1;
-          if (half == 1 && lane == 0) mbar_arrive(&ctl->exp_done[t][quarter]);
-          tc_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->p_full[t][half]);
+          tmem_st8(p_col + v * 8, packed);
+          if (v == 7 && lane == 0) mbar_arrive(&ctl->exp_done[t][quarter]);
+          if (v == 4 || v == 7) {          // the first half is handed over under the next 16 columns' exponentials
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_full[t][v == 7]);
+          }
         }
+        l += l0 + l1;
       } else {
         ok = retired();                                      // (not ahead of the others' P of block j - 1)
         if (!ok) break;
@@ -388,7 +391,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
     if (ok && live) {
-      const float l = lh[0] + lh[1];
       const int head = kvh * p.group + row % p.group;
       const int64_t token = u.t0 + t * p.tok + tk;
       if (u.slot >= 0) {
