@@ -18,7 +18,8 @@ struct PackedHeader {                     // words 0..31 of a plan
   int fwd_join_off, n_fwd_join, fwd_slots;    // units that were divided over the keys (PackedJoin) and their slots
   int dq_join_off, n_dq_join, dq_slots;
   int dkv_join_off, n_dkv_join, dkv_slots;
-  int reserved[9];
+  int longest_q, longest_k;               // tokens of the longest sequence
+  int reserved[7];
 };
 static_assert(sizeof(PackedHeader) == kPlanHeader * 4, "the header is 32 words");
 
@@ -42,5 +43,21 @@ __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.al
 struct PackedJoin {                       // the slots [slot, slot + parts) are sums of the rows t0 .. t0 + n - 1
   int t0, n, slot, parts;
 };
+
+// Which unit and key head a CTA serves.  The units of `at_once` heads go together, the longest units of all of them
+// first: the launch ends with short ones, and what the CTAs in flight read stays in L2.
+__device__ __forceinline__ PackedUnit packed_unit(const PackedUnit* units, int n_units, int heads, int at_once, int& head) {
+  const int g = blockIdx.x / (n_units * at_once);
+  const int r = blockIdx.x - g * n_units * at_once;
+  const int here = min(at_once, heads - g * at_once);
+  head = g * at_once + r % here;
+  return units[r / here];
+}
+// Heads whose two streamed tensors (`rows` rows of the longest sequence) fill half of the L2.
+inline int packed_heads_at_once(int heads, int64_t rows, int D) {
+  const int64_t bytes = 4ll * D * (rows > 0 ? rows : 1);
+  const int64_t n = (64ll << 20) / bytes;
+  return static_cast<int>(n < 1 ? 1 : n > heads ? heads : n);
+}
 
 }  // namespace swv

@@ -39,7 +39,7 @@ struct PackedFwdParams {
   float scale_log2;
   float* part_o;                // [slot][Hkv][256][D] unnormalised rows of divided units
   float2* part_ml;              // [slot][Hkv][256] (stabiliser, sum)
-  int Hkv;
+  int Hkv, heads_at_once;
   int* status;
 };
 
@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   FwdCtl* ctl = reinterpret_cast<FwdCtl*>(smem + Cfg::kOffCtl);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int kvh = blockIdx.x / p.n_units;            // heads slowest: the CTAs in flight share one or two heads' keys
-  const PackedUnit u = p.units[blockIdx.x % p.n_units];
+  int kvh;
+  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
   const int n = u.b1 - u.b0;
   // tokens and key blocks of tile t: its last token sees the fewest keys of no later tile
   auto tokens = [&](int t) { return min(p.tok, u.n - t * p.tok); };
@@ -588,6 +588,7 @@ int packed_attn_fwd_impl(const void* q, const int64_t* qs, const void* k, const 
   p.Tq = static_cast<int>(Tq); p.d = D; p.o = o; p.os_t = os[0]; p.os_h = os[1]; p.lse = lse;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.Hkv = h.Hkv; p.status = status;
+  p.heads_at_once = packed_heads_at_once(h.Hkv, h.longest_k, D);
   const int Dk = D <= 64 ? 64 : 128;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(h.fwd_slots) * h.Hkv * 2 * kTile * Dk);

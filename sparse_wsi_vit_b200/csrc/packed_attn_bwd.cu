@@ -38,7 +38,7 @@ constexpr int kBwdThreads = 384;
 
 struct PackedBwdParams {
   const PackedUnit* units;
-  int n_units, group, tok, Tq, d, Hkv;
+  int n_units, group, tok, Tq, d, Hkv, heads_at_once;
   const float2* stats;          // [Hkv][Tq][group] {lse in powers of two, delta}; +inf where a row sees no key
   void *g1, *g2;                // kDkv: dK, dV; kDq: dQ
   int64_t g1_t, g1_h, g2_t, g2_h;
@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   float* stats = reinterpret_cast<float*>(smem + Cfg::kOffStats);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int kvh = blockIdx.x / p.n_units;
-  const PackedUnit u = p.units[blockIdx.x % p.n_units];
+  int kvh;
+  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
   const int n = u.b1 - u.b0;
   const int per = MODE == kDkv ? p.tok * p.group : kTile;      // streamed rows a tile
   const int step = MODE == kDkv ? p.tok : kTile;               // streamed tokens a tile
@@ -635,6 +635,7 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   PackedBwdParams a = p;                                       // keys' side
   a.units = reinterpret_cast<const PackedUnit*>(plan + h.dkv_off);
   a.n_units = h.n_dkv;
+  a.heads_at_once = packed_heads_at_once(h.Hkv, static_cast<int64_t>(h.longest_q) * p.group, D);
   a.g1 = dk; a.g1_t = dks[0]; a.g1_h = dks[1];
   a.g2 = dv; a.g2_t = dvs[0]; a.g2_h = dvs[1];
   a.part = reinterpret_cast<float*>(w + sz.dq);
@@ -645,6 +646,7 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   PackedBwdParams b = p;                                       // queries' side
   b.units = reinterpret_cast<const PackedUnit*>(plan + h.dq_off);
   b.n_units = h.n_dq;
+  b.heads_at_once = packed_heads_at_once(h.Hkv, h.longest_k, D);
   b.g1 = dq; b.g1_t = dqs[0]; b.g1_h = dqs[1];
   b.part = reinterpret_cast<float*>(w);
   const PackedJoin* jb = reinterpret_cast<const PackedJoin*>(plan + h.dq_join_off);

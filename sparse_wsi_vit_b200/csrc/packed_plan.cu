@@ -102,7 +102,7 @@ void build(int n_seq, const int64_t* ql, const int64_t* kl, int H, int Hkv, int 
   const int tok = kTile / (H / Hkv);              // query tokens of a tile
   const int sms = sm_count();
   Work fwd, dq, dkv;
-  int q0 = 0, k0 = 0;
+  int q0 = 0, k0 = 0, longest_q = 0, longest_k = 0;
   for (int s = 0; s < n_seq; ++s) {
     const int lq = static_cast<int>(ql[s]), lk = static_cast<int>(kl[s]);
     for (int pass = 0; pass < 2; ++pass) {
@@ -135,6 +135,8 @@ void build(int n_seq, const int64_t* ql, const int64_t* kl, int H, int Hkv, int 
       u.slot = -1;
       dkv.units.push_back(u);
     }
+    longest_q = std::max(longest_q, lq);
+    longest_k = std::max(longest_k, lk);
     q0 += lq;
     k0 += lk;
   }
@@ -144,6 +146,7 @@ void build(int n_seq, const int64_t* ql, const int64_t* kl, int H, int Hkv, int 
   PackedHeader h{};
   h.magic = kPlanMagic;
   h.n_seq = n_seq; h.H = H; h.Hkv = Hkv; h.causal = causal; h.Tq = q0; h.Tk = k0;
+  h.longest_q = longest_q; h.longest_k = longest_k;
   out.assign(kPlanHeader, 0);
   auto put = [&](const Work& w, int& off, int& n, int& join_off, int& n_join, int& slots) {
     off = static_cast<int>(out.size());
