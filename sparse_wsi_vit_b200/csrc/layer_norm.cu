@@ -3,11 +3,11 @@
 //   mu = mean(x)   rstd = 1 / sqrt(mean((x - mu)^2) + eps)   xh = (x - mu) rstd   y = xh w + b
 //   g  = dy w      dx = rstd (g - mean(g) - xh mean(g xh))   dw = sum_rows dy xh  db = sum_rows dy
 //
-// A group of threads (a warp, or a CTA for wide rows) owns a row: it is read once into registers, the variance is
+// A group of threads (a warp, four or eight) owns a row: it is read once into registers, the variance is
 // taken from the centred values (a second sum over the registers, so a large offset of the row costs no bits), and
 // the result is written from the registers.  All sums are fp32.  The groups stay resident and walk over the rows, so
-// the weights -- and in the backward pass the sums of dw and db -- stay in registers; the next row is loaded before
-// the present one is reduced.  Each CTA leaves its dw and db sums in the workspace and a second kernel adds them up in
+// the weights stay in shared memory and, in the backward pass, the sums of dw and db in registers; the next row is loaded
+// before the present one is reduced, and a row is kept as it lies in memory (half the registers for 16-bit types).  Each CTA leaves its dw and db sums in the workspace and a second kernel adds them up in
 // a fixed order: no atomics, the same bits every time.
 //
 // Bound: HBM, 2 N E elements forward, 3 N E backward.
@@ -34,7 +34,7 @@ struct LnParams {
   float eps;
 };
 
-// sums over the threads of a group: a warp, or the whole CTA
+// Sums over the threads of a group: a warp, some warps of a CTA (named barrier 1 + the group) or the whole CTA.
 template <int TPR, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* smem, int& phase) {
 #pragma unroll
@@ -43,58 +43,140 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* smem, int& phase
     for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
   }
   if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    const int grp = threadIdx.x / TPR, w = (threadIdx.x % TPR) >> 5;
     // two buffers in turn: a warp may be one reduction ahead of the others, never two
-    float* buf = smem + (phase & 1) * (2 * (TPR / 32));
+    float* buf = smem + ((phase & 1) * (kLnThreads / TPR) + grp) * (2 * W);
     ++phase;
     if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) buf[k * (TPR / 32) + (threadIdx.x >> 5)] = v[k];
+      for (int k = 0; k < K; ++k) buf[k * W + w] = v[k];
     }
-    __syncthreads();
+    if constexpr (TPR == kLnThreads) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(TPR) : "memory");   // (a group's warps do the same rows)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       v[k] = 0.f;
 #pragma unroll
-      for (int i = 0; i < TPR / 32; ++i) v[k] += buf[k * (TPR / 32) + i];
+      for (int i = 0; i < W; ++i) v[k] += buf[k * W + i];
     }
   }
 }
 
+// A run of VEC elements as it lies in memory: half the registers of its fp32 values for 16-bit types.
+template <typename T, int VEC>
+struct Raw {
+  static constexpr int kWords = VEC * static_cast<int>(sizeof(T)) / 4 > 0 ? VEC * static_cast<int>(sizeof(T)) / 4 : 1;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC == 8) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p) + i / 4);      // read once
+        w[i] = a.x; w[i + 1] = a.y; w[i + 2] = a.z; w[i + 3] = a.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = __float_as_uint(*p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void values(float* v) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(w[i]);
+    } else if constexpr (VEC == 8) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+    } else {
+      float unused;
+      unpack2<T>(w[0], v[0], unused);
+    }
+  }
+};
+
+// The weights lie in shared memory as fp32, [w | b]; the columns behind E are zero.
+template <int C>
+__device__ __forceinline__ void stage_row(const void* a, int dtype, int E, float otherwise, float* out) {
+  if (a != nullptr && dtype == SWV_F32 && (reinterpret_cast<uintptr_t>(a) & 15) == 0) {
+    constexpr int kRuns = (C + 4 * kLnThreads - 1) / (4 * kLnThreads);
+    float4 v[kRuns];                                         // all loads in flight together
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+      const int c = (i * kLnThreads + threadIdx.x) * 4;
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float* f = static_cast<const float*>(a) + c;
+      if (c + 3 < E) {
+        v[i] = *reinterpret_cast<const float4*>(f);
+      } else if (c < E) {
+        v[i].x = f[0];
+        if (c + 1 < E) v[i].y = f[1];
+        if (c + 2 < E) v[i].z = f[2];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+      const int c = (i * kLnThreads + threadIdx.x) * 4;
+      if (c < C) *reinterpret_cast<float4*>(out + c) = v[i];
+    }
+    return;
+  }
+  constexpr int kRuns = (C + kLnThreads - 1) / kLnThreads;
+#pragma unroll 8
+  for (int i = 0; i < kRuns; ++i) {
+    const int c = i * kLnThreads + threadIdx.x;
+    if (c < C) out[c] = c >= E ? 0.f : a != nullptr ? load_as_f32(a, dtype, c) : otherwise;
+  }
+}
+template <int VEC, int ITER, int TPR>
+__device__ __forceinline__ void stage_weights(const LnParams& p, float* ws, bool bias) {
+  constexpr int C = VEC * ITER * TPR;
+  stage_row<C>(p.w, p.w_dtype, p.E, 1.f, ws);
+  if (bias) stage_row<C>(p.b, p.b_dtype, p.E, 0.f, ws + C);
+  __syncthreads();
+}
+template <int VEC>
+__device__ __forceinline__ void load_weights(const float* ws, float* v) {
+  if constexpr (VEC == 8) {
+    const float4 a = *reinterpret_cast<const float4*>(ws), b = *reinterpret_cast<const float4*>(ws + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    v[0] = *ws;
+  }
+}
+
 template <typename T, typename U, int VEC, int ITER, int TPR>
-__global__ void __launch_bounds__(kLnThreads) layer_norm_fwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(kLnThreads, VEC * ITER > 24 ? 2 : sizeof(T) == 4 ? 3 : 4) layer_norm_fwd_kernel(const LnParams p) {
   __shared__ float red[4 * (kLnThreads / 32)];
+  extern __shared__ float ws[];
+  constexpr int C = VEC * ITER * TPR;
   int phase = 0;
   const int t = threadIdx.x % TPR;
   const int64_t groups = static_cast<int64_t>(gridDim.x) * (kLnThreads / TPR);
   int64_t row = static_cast<int64_t>(blockIdx.x) * (kLnThreads / TPR) + threadIdx.x / TPR;
   const float inv_e = 1.f / p.E;
-  float w[ITER * VEC], b[ITER * VEC], v[ITER * VEC], nx[ITER * VEC];
-#pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int c = (i * TPR + t) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const bool in = c + e < p.E;
-      w[i * VEC + e] = in ? (p.w != nullptr ? load_as_f32(p.w, p.w_dtype, c + e) : 1.f) : 0.f;
-      b[i * VEC + e] = in && p.b != nullptr ? load_as_f32(p.b, p.b_dtype, c + e) : 0.f;
-    }
-  }
-  auto fetch = [&](int64_t r, float (&d)[ITER * VEC]) {
+  Raw<T, VEC> next[ITER];
+  auto fetch = [&](int64_t r) {
     const T* xr = static_cast<const T*>(p.x) + r * p.xs;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * TPR + t) * VEC;
-      if (r < p.N && c < p.E) load_run<T, VEC>(xr + c, d + i * VEC);
-      else
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) d[i * VEC + e] = 0.f;
+      if (r < p.N && c < p.E) next[i].load(xr + c);
+      else next[i].zero();
     }
   };
-  fetch(row, nx);
+  fetch(row);
+  stage_weights<VEC, ITER, TPR>(p, ws, true);
   for (; row < p.N; row += groups) {
+    float v[ITER * VEC];
 #pragma unroll
-    for (int i = 0; i < ITER * VEC; ++i) v[i] = nx[i];
-    fetch(row + groups, nx);
+    for (int i = 0; i < ITER; ++i) next[i].values(v + i * VEC);
+    fetch(row + groups);
     float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < ITER * VEC; ++i) s[0] += v[i];
@@ -103,9 +185,10 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_fwd_kernel(const LnPara
     s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
+      const bool in = (i * TPR + t) * VEC < p.E;             // (a run lies inside the row or outside it)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = (i * TPR + t) * VEC + e < p.E ? v[i * VEC + e] - mu : 0.f;
+        const float d = in ? v[i * VEC + e] - mu : 0.f;
         v[i * VEC + e] = d;
         s[0] = fmaf(d, d, s[0]);
       }
@@ -116,9 +199,12 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_fwd_kernel(const LnPara
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * TPR + t) * VEC;
+      float w[VEC], b[VEC];
+      load_weights<VEC>(ws + c, w);
+      load_weights<VEC>(ws + C + c, b);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i * VEC + e] = fmaf(v[i * VEC + e] * rstd, w[i * VEC + e], b[i * VEC + e]);
-      if (c < p.E) store_run<U, VEC>(yr + c, v + i * VEC);
+      for (int e = 0; e < VEC; ++e) w[e] = fmaf(v[i * VEC + e] * rstd, w[e], b[e]);
+      if (c < p.E) store_run<U, VEC>(yr + c, w);
     }
     if (t == 0 && p.mean != nullptr) {
       p.mean[row] = mu;
@@ -128,50 +214,64 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_fwd_kernel(const LnPara
 }
 
 template <typename T, typename U, int VEC, int ITER, int TPR>
-__global__ void __launch_bounds__(kLnThreads) layer_norm_bwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_norm_bwd_kernel(const LnParams p) {
   __shared__ float red[4 * (kLnThreads / 32)];
+  extern __shared__ float ws[];
+  constexpr int R = ITER * VEC, C = R * TPR;
   int phase = 0;
-  constexpr int R = ITER * VEC;
   const int t = threadIdx.x % TPR;
   const int64_t groups = static_cast<int64_t>(gridDim.x) * (kLnThreads / TPR);
   int64_t row = static_cast<int64_t>(blockIdx.x) * (kLnThreads / TPR) + threadIdx.x / TPR;
   const float inv_e = 1.f / p.E;
-  float w[R], dw[R], db[R], x[R], g[R];
+  float dw[R], db[R];
+  constexpr bool kAhead = sizeof(T) + sizeof(U) <= 4;        // 16-bit rows: the next one is loaded under the present one's sums
+  Raw<T, VEC> xn[ITER];
+  Raw<U, VEC> gn[ITER];
 #pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int c = (i * TPR + t) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[i * VEC + e] = c + e < p.E ? (p.w != nullptr ? load_as_f32(p.w, p.w_dtype, c + e) : 1.f) : 0.f;
-      dw[i * VEC + e] = db[i * VEC + e] = 0.f;
-    }
-  }
-  for (; row < p.N; row += groups) {
-    const T* xr = static_cast<const T*>(p.x) + row * p.xs;
-    const U* dyr = static_cast<const U*>(p.dy) + row * p.dys;
+  for (int i = 0; i < R; ++i) dw[i] = db[i] = 0.f;
+  auto fetch = [&](int64_t r) {
+    const T* xr = static_cast<const T*>(p.x) + r * p.xs;
+    const U* dyr = static_cast<const U*>(p.dy) + r * p.dys;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * TPR + t) * VEC;
-      if (c < p.E) {
-        load_run<T, VEC>(xr + c, x + i * VEC);
-        load_run<U, VEC>(dyr + c, g + i * VEC);
+      if (r < p.N && c < p.E) {
+        xn[i].load(xr + c);
+        gn[i].load(dyr + c);
+      } else {
+        xn[i].zero();
+        gn[i].zero();
       }
     }
+  };
+  if (kAhead) fetch(row);
+  stage_weights<VEC, ITER, TPR>(p, ws, false);
+  for (; row < p.N; row += groups) {
     const float mu = p.mean[row], rstd = p.rstd[row];
+    if (!kAhead) fetch(row);
+    Raw<T, VEC> x[ITER];
+    Raw<U, VEC> g[ITER];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      x[i] = xn[i];
+      g[i] = gn[i];
+    }
+    if (kAhead) fetch(row + groups);
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
+      float xv[VEC], gv[VEC], w[VEC];
+      x[i].values(xv);
+      g[i].values(gv);
+      load_weights<VEC>(ws + (i * TPR + t) * VEC, w);        // (zero behind the row, and so is the gradient)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const int k = i * VEC + e;
-        const bool in = (i * TPR + t) * VEC + e < p.E;
-        const float xh = in ? (x[k] - mu) * rstd : 0.f, d = in ? g[k] : 0.f;
-        dw[k] = fmaf(d, xh, dw[k]);
-        db[k] += d;
-        x[k] = xh;
-        g[k] = d * w[k];
-        s[0] += g[k];
-        s[1] = fmaf(g[k], xh, s[1]);
+        const float xh = (xv[e] - mu) * rstd;
+        dw[i * VEC + e] = fmaf(gv[e], xh, dw[i * VEC + e]);
+        db[i * VEC + e] += gv[e];
+        const float gw = gv[e] * w[e];
+        s[0] += gw;
+        s[1] = fmaf(gw, xh, s[1]);
       }
     }
     group_sum<TPR>(s, red, phase);
@@ -180,46 +280,43 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_bwd_kernel(const LnPara
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * TPR + t) * VEC;
+      float xv[VEC], gv[VEC], w[VEC];
+      x[i].values(xv);
+      g[i].values(gv);
+      load_weights<VEC>(ws + c, w);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x[i * VEC + e] = rstd * (g[i * VEC + e] - m0 - x[i * VEC + e] * m1);
-      if (c < p.E) store_run<T, VEC>(dxr + c, x + i * VEC);
+      for (int e = 0; e < VEC; ++e) xv[e] = rstd * (gv[e] * w[e] - m0 - (xv[e] - mu) * rstd * m1);
+      if (c < p.E) store_run<T, VEC>(dxr + c, xv);
     }
   }
   if (p.part == nullptr) return;
-  // the groups' sums of this CTA, one group after the other
   float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.E;
   if constexpr (TPR == kLnThreads) {
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int c = (i * TPR + t) * VEC + e;
-        if (c < p.E) {
-          out[c] = dw[i * VEC + e];
-          out[p.E + c] = db[i * VEC + e];
-        }
+    for (int i = 0; i < R; ++i) {
+      const int c = (i / VEC * TPR + t) * VEC + i % VEC;
+      if (c < p.E) {
+        out[c] = dw[i];
+        out[p.E + c] = db[i];
       }
     }
   } else {
-    __shared__ float acc[2][TPR * R];
-    const int mine = threadIdx.x / TPR;
-    for (int k = 0; k < kLnThreads / TPR; ++k) {
-      if (mine == k) {
+    // the groups' sums side by side (the weights are no longer read), added up in the groups' order
+    __syncthreads();
+    float* mine = ws + threadIdx.x / TPR * 2 * C;
 #pragma unroll
-        for (int i = 0; i < ITER; ++i) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int c = (i * TPR + t) * VEC + e;
-            acc[0][c] = (k == 0 ? 0.f : acc[0][c]) + dw[i * VEC + e];
-            acc[1][c] = (k == 0 ? 0.f : acc[1][c]) + db[i * VEC + e];
-          }
-        }
-      }
-      __syncthreads();
+    for (int i = 0; i < R; ++i) {
+      const int c = (i / VEC * TPR + t) * VEC + i % VEC;
+      mine[c] = dw[i];
+      mine[C + c] = db[i];
     }
-    for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
-      out[c] = acc[0][c];
-      out[p.E + c] = acc[1][c];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * p.E; c += kLnThreads) {
+      const float* col = ws + (c < p.E ? c : C + c - p.E);
+      float a = 0.f;
+#pragma unroll
+      for (int k = 0; k < kLnThreads / TPR; ++k) a += col[k * 2 * C];
+      out[c] = a;
     }
   }
 }
@@ -291,40 +388,47 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_wide_bwd_kernel(const L
   }
 }
 
-// dw[c] = sum over the CTAs' rows of the workspace: eight lanes of rows for 32 columns, added up in order
-__global__ void __launch_bounds__(256) layer_norm_sum_kernel(const float* part, int parts, int E, void* dw, int dw_dtype,
-                                                             void* db, int db_dtype) {
-  __shared__ float s[8][33];
+// dw[c] = sum over the CTAs' rows of the workspace: 32 lanes of rows for 32 columns, added up in order
+__global__ void __launch_bounds__(1024) layer_norm_sum_kernel(const float* part, int parts, int E, void* dw, int dw_dtype,
+                                                              void* db, int db_dtype) {
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;                   // column of [dw | db]
   float a = 0.f;
   if (c < 2 * E)
-    for (int k = r; k < parts; k += 8) a += part[static_cast<int64_t>(k) * 2 * E + c];
+    for (int k = r; k < parts; k += 32) a += part[static_cast<int64_t>(k) * 2 * E + c];
   s[r][lane] = a;
   __syncthreads();
-  if (r == 0 && c < 2 * E) {
-    a = 0.f;
+  // column `r` of the block: its 32 partial sums in the lanes of one warp
+  a = s[lane][r];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a += s[k][lane];
-    if (c < E) {
-      if (dw != nullptr) store_from_f32(dw, dw_dtype, c, a);
+  for (int off = 16; off > 0; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off);
+  const int col = blockIdx.x * 32 + r;
+  if (lane == 0 && col < 2 * E) {
+    if (col < E) {
+      if (dw != nullptr) store_from_f32(dw, dw_dtype, col, a);
     } else if (db != nullptr) {
-      store_from_f32(db, db_dtype, c - E, a);
+      store_from_f32(db, db_dtype, col - E, a);
     }
   }
 }
 
 // Which kernel serves a row: runs of 8 elements where every row starts on 16 bytes and E is a multiple of 8, single
-// elements otherwise; a warp a row up to 32 elements a thread, then a CTA, then the form that reads the row again.
+// elements otherwise.  Forward, 16-bit rows: a warp a row up to 1024 values (65536 x 768: 41 us, two warps 51 us); fp32
+// rows, twice the registers: one run a thread (4099 x 1280: 12.6 us, two runs 15.7 us).  Backward: as many threads as
+// leave two runs (x, dy, dw and db of 16 values) to each; a warp a row with three runs spilled at two CTAs per SM (76
+// against 105 us at 65536 x 768).  Beyond 8192 values the form that reads the row again.
 struct LnForm {
   int vec, tpr, iter;       // iter = 0: the form for wide rows
 };
-LnForm ln_form(int E, bool vec8) {
+LnForm ln_form(int E, bool vec8, bool bwd, bool wide) {
   LnForm f;
   f.vec = vec8 ? 8 : 1;
-  f.tpr = E <= 1024 ? 32 : kLnThreads;
+  if (f.vec == 8 && !bwd && wide) f.tpr = E <= 256 ? 32 : E <= 512 ? 64 : E <= 1024 ? 128 : kLnThreads;
+  else if (f.vec == 8) f.tpr = E <= (bwd ? 512 : 1024) ? 32 : E <= 1024 ? 64 : E <= 2048 ? 128 : kLnThreads;
+  else f.tpr = E <= 1024 ? 32 : E <= 4096 ? 128 : kLnThreads;
   const int n = (E + f.vec * f.tpr - 1) / (f.vec * f.tpr);
-  if (f.vec == 8) f.iter = n <= 1 ? 1 : n <= 2 ? 2 : n <= 3 ? 3 : n <= 4 ? 4 : 0;
+  if (f.vec == 8) f.iter = n <= 4 ? n : 0;
   else f.iter = n <= 8 ? 8 : n <= 32 ? 32 : 0;
   return f;
 }
@@ -337,14 +441,16 @@ constexpr int kLnFwdCtas = 4, kLnBwdCtas = 2;     // resident CTAs per SM
 
 template <typename T, typename U, bool BWD>
 int ln_launch(const LnParams& p, const LnForm& f, int grid, cudaStream_t st) {
-#define SWV_LN(V, I, R)                                                            \
-  if (f.vec == V && f.iter == I && f.tpr == R) {                                    \
-    if constexpr (BWD) layer_norm_bwd_kernel<T, U, V, I, R><<<grid, kLnThreads, 0, st>>>(p); \
-    else layer_norm_fwd_kernel<T, U, V, I, R><<<grid, kLnThreads, 0, st>>>(p);      \
+#define SWV_LN(V, I, R)                                                                                      \
+  if (f.vec == V && f.iter == I && f.tpr == R) {                                                             \
+    constexpr int kSmem = 2 * V * I * (BWD ? kLnThreads : R) * 4;                                                               \
+    auto k = BWD ? layer_norm_bwd_kernel<T, U, V, I, R> : layer_norm_fwd_kernel<T, U, V, I, R>;              \
+    if (kSmem > 40 * 1024) SWV_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)); \
+    k<<<grid, kLnThreads, kSmem, st>>>(p);                                                                   \
   } else
-  SWV_LN(8, 1, 32) SWV_LN(8, 2, 32) SWV_LN(8, 3, 32) SWV_LN(8, 4, 32)
-  SWV_LN(8, 1, kLnThreads) SWV_LN(8, 2, kLnThreads) SWV_LN(8, 3, kLnThreads) SWV_LN(8, 4, kLnThreads)
-  SWV_LN(1, 8, 32) SWV_LN(1, 32, 32) SWV_LN(1, 8, kLnThreads) SWV_LN(1, 32, kLnThreads) {
+  SWV_LN(8, 1, 32) SWV_LN(8, 2, 32) SWV_LN(8, 3, 32) SWV_LN(8, 4, 32) SWV_LN(8, 1, 64) SWV_LN(8, 1, 128) SWV_LN(8, 1, kLnThreads) SWV_LN(8, 2, 64) SWV_LN(8, 2, 128) SWV_LN(8, 2, kLnThreads) SWV_LN(8, 3, kLnThreads)
+  SWV_LN(8, 4, kLnThreads)
+  SWV_LN(1, 8, 32) SWV_LN(1, 32, 32) SWV_LN(1, 32, 128) SWV_LN(1, 32, kLnThreads) {
     if constexpr (BWD) layer_norm_wide_bwd_kernel<T, U><<<grid, kLnThreads, 0, st>>>(p);
     else layer_norm_wide_fwd_kernel<T, U><<<grid, kLnThreads, 0, st>>>(p);
   }
@@ -387,7 +493,7 @@ int layer_norm_fwd_impl(const void* x, int64_t xs, int x_dtype, const void* w, i
   if (N == 0) return SWV_OK;
   if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return SWV_ERR_NULL;
   const bool vec = E % 8 == 0 && rows_vec8(x, xs, dtype_bytes(x_dtype)) && rows_vec8(y, ys, dtype_bytes(y_dtype));
-  const LnForm f = ln_form(E, vec);
+  const LnForm f = ln_form(E, vec, false, x_dtype == SWV_F32);
   LnParams p{};
   p.x = x; p.w = w; p.b = b; p.y = y; p.mean = mean; p.rstd = rstd;
   p.N = N; p.xs = xs; p.ys = ys; p.E = E; p.w_dtype = w_dtype; p.b_dtype = b_dtype; p.eps = eps;
@@ -414,7 +520,7 @@ int layer_norm_bwd_impl(const void* dy, int64_t dys, int y_dtype, const void* x,
   const bool sums = dw != nullptr || db != nullptr;
   const bool vec = E % 8 == 0 && rows_vec8(x, xs, dtype_bytes(x_dtype)) && rows_vec8(dy, dys, dtype_bytes(y_dtype)) &&
                    rows_vec8(dx, dxs, dtype_bytes(x_dtype));
-  const LnForm f = ln_form(E, vec);
+  const LnForm f = ln_form(E, vec, true, false);
   const int grid = N == 0 ? 0 : ln_grid(N, f.iter == 0 ? kLnThreads : f.tpr, kLnBwdCtas);
   if (sums && N > 0) {
     size_t need = static_cast<size_t>(grid) * 2 * E * sizeof(float);
@@ -432,7 +538,7 @@ int layer_norm_bwd_impl(const void* dy, int64_t dys, int y_dtype, const void* x,
     if (r != SWV_OK) return r;
   }
   if (sums) {                                             // (no rows: the sums are zero)
-    layer_norm_sum_kernel<<<(2 * E + 31) / 32, 256, 0, st>>>(p.part, grid, E, dw, dw_dtype, db, db_dtype);
+    layer_norm_sum_kernel<<<(2 * E + 31) / 32, 1024, 0, st>>>(p.part, grid, E, dw, dw_dtype, db, db_dtype);
     SWV_CUDA_OK(cudaGetLastError());
   }
   return SWV_OK;
