@@ -72,6 +72,42 @@ __device__ __forceinline__ void store_run(T* p, const float* v) {
   }
 }
 
+// A run of VEC elements as it lies in memory: half the registers of its fp32 values for 16-bit types.
+template <typename T, int VEC>
+struct Raw {
+  static constexpr int kWords = VEC * static_cast<int>(sizeof(T)) / 4 > 0 ? VEC * static_cast<int>(sizeof(T)) / 4 : 1;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC == 8) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p) + i / 4);      // read once
+        w[i] = a.x; w[i + 1] = a.y; w[i + 2] = a.z; w[i + 3] = a.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = __float_as_uint(*p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void values(float* v) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(w[i]);
+    } else if constexpr (VEC == 8) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+    } else {
+      float unused;
+      unpack2<T>(w[0], v[0], unused);
+    }
+  }
+};
+
 // one element of an array whose type is known at run time
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
   if (dtype == SWV_F32) return static_cast<const float*>(p)[i];

@@ -79,28 +79,28 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ 
     if (pair < p.pairs) rope_angle(p, t, pair, cs[i], sn[i]);      // (a unit can reach into the copied channels)
   }
   const int ca = HALVES ? u * PAIRS : 2 * u * PAIRS, cb = ca + p.pairs;
-  for (int h = h0; h < h1; h += 2) {
-    float a[2][2 * PAIRS];
+  constexpr int RUN = HALVES ? VEC : 2 * PAIRS;                    // elements of one access (8 or 1; adjacent pairs: 8 or 2)
+  constexpr int kRaw = RUN == 8 ? 8 : 1, kRuns = 2 * PAIRS / kRaw;
+  for (int h = h0; h < h1; h += 4) {                               // the loads of four heads are in flight together
+    Raw<T, kRaw> v[4][kRuns];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 4; ++k) {
       if (h + k >= h1) continue;
       const T* xh = x + (h + k) * p.xs_h;
-      if constexpr (HALVES) {
-        load_run<T, VEC>(xh + ca, a[k]);
-        load_run<T, VEC>(xh + cb, a[k] + PAIRS);
-      } else {
-        load_run<T, 2 * PAIRS>(xh + ca, a[k]);
-      }
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) v[k][r].load(xh + (HALVES ? (r < kRuns / 2 ? ca : cb - PAIRS) : ca) + r * kRaw);
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 4; ++k) {
       if (h + k >= h1) continue;
       T* yh = y + (h + k) * p.ys_h;
-      float o[2 * PAIRS];
+      float a[2 * PAIRS], o[2 * PAIRS];
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) v[k][r].values(a + r * kRaw);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
         const int ia = HALVES ? i : 2 * i, ib = HALVES ? PAIRS + i : 2 * i + 1;
-        const float va = a[k][ia], vb = a[k][ib];
+        const float va = a[ia], vb = a[ib];
         o[ia] = fmaf(va, cs[i], -vb * sn[i]);
         o[ib] = fmaf(vb, cs[i], va * sn[i]);
         if (!HALVES && u * PAIRS + i >= p.pairs) {                 // copied as they are (an infinity stays one)
@@ -127,8 +127,8 @@ int rope_axes_launch(RopeAxesParams& p, bool vec, bool halves, cudaStream_t st) 
   const int64_t threads = p.T * (turning + still);
   const int64_t blocks = (threads + 255) / 256;
   if (blocks > 0x7fffffff) return SWV_ERR_SHAPE;
-  // few tokens: the heads are divided until some four CTAs an SM are there, two heads (one step of the loop) at least
-  const int64_t want = 4ll * sm_count();
+  // few tokens: the heads are divided until some eight CTAs an SM are there, two heads at least
+  const int64_t want = 8ll * sm_count();
   const int64_t split = std::min<int64_t>(std::min<int64_t>((want + blocks - 1) / blocks, (p.H + 1) / 2), 65535);
   p.heads_per_cta = static_cast<int>((p.H + split - 1) / split);
   const dim3 grid(static_cast<unsigned>(blocks), (p.H + p.heads_per_cta - 1) / p.heads_per_cta);
