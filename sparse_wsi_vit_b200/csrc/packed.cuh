@@ -60,4 +60,58 @@ inline int packed_heads_at_once(int heads, int64_t rows, int D) {
   return static_cast<int>(n < 1 ? 1 : n > heads ? heads : n);
 }
 
+// Rows of D 16-bit values gathered in shared memory before they are written: a thread holds a whole row of a TMEM tile, and
+// 32 rows' stores of 16 bytes touch 32 lines each.  Chunks of 16 bytes change places with the row so that the threads'
+// stores meet different banks.
+template <int D>
+__device__ __forceinline__ uint32_t staged_at(uint32_t base, int row, int chunk) {
+  return base + row * (D * 2) + ((chunk ^ (row & 7)) << 4);
+}
+// 16 fp32 values of a row, from column 16 * c on, times f, as bf16
+template <int D>
+__device__ __forceinline__ void stage16(uint32_t base, int row, int c, const uint32_t (&o)[16], float f) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      w[q] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * q]) * f, __uint_as_float(o[8 * i + 2 * q + 1]) * f);
+    sts128(staged_at<D>(base, row, 2 * c + i), w[0], w[1], w[2], w[3]);
+  }
+}
+// Writes rows r0 .. r1 - 1 of the staged tile (one warp; `at(row)` is where a row goes), d <= D channels.
+template <int D, typename At>
+__device__ __forceinline__ void write_staged(uint32_t base, int r0, int r1, int d, At at) {
+  constexpr int kLanes = D / 8;                                // lanes a row
+  const int lane = threadIdx.x & 31, chunk = lane % kLanes;
+  for (int r = r0 + lane / kLanes; r < r1; r += 32 / kLanes)
+    if (chunk * 8 < d) *reinterpret_cast<uint4*>(at(r) + chunk * 8) = lds128(staged_at<D>(base, r, chunk));
+}
+
+// pairs of fp32 values in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c, float d) {
+  asm("{\n\t.reg .b64 v, s, e;\n\tmov.b64 v, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 e, {%5, %6};\n\t"
+      "fma.rn.f32x2 v, v, s, e;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "=f"(x), "=f"(y)
+      : "f"(a), "f"(b), "f"(m), "f"(c), "f"(d));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 v, s;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tadd.rn.f32x2 v, v, s;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 v, s;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tmul.rn.f32x2 v, v, s;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+
+// Whether a kernel is launched with the registers that its warpgroups share out (an increase beyond them would wait for
+// ever): asked once per kernel.
+template <typename K>
+bool registers_suffice(K kernel, int threads, int shared_out) {
+  cudaFuncAttributes a;
+  return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && a.numRegs * threads >= shared_out;
+}
+
 }  // namespace swv

@@ -44,6 +44,8 @@ struct PackedFwdParams {
 };
 
 constexpr int kFwdThreads = 384;
+constexpr int kFwdRegsControl = 80, kFwdRegsSoftmax = 208;      // of 384 x 168 = 64512 at launch: 63488
+constexpr int kFwdRegs = 128 * kFwdRegsControl + 256 * kFwdRegsSoftmax;
 
 template <int D>
 struct FwdCfg {
@@ -69,17 +71,6 @@ constexpr size_t fwd_smem() { return 1024 + FwdCfg<D>::kOffCtl + sizeof(FwdCtl) 
 
 __device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
-__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float sc, float add) {
-  asm("{\n\t.reg .b64 v, s, d;\n\tmov.b64 v, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 d, {%5, %5};\n\t"
-      "fma.rn.f32x2 v, v, s, d;\n\tmov.b64 {%0, %1}, v;\n\t}"
-      : "=f"(x), "=f"(y)
-      : "f"(a), "f"(b), "f"(sc), "f"(add));
-}
-__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
-  asm("{\n\t.reg .b64 v, s;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tadd.rn.f32x2 v, v, s;\n\tmov.b64 {%0, %1}, v;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(b));
-}
 __device__ __forceinline__ float max_of3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -142,9 +133,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const uint32_t tmem_base = ctl->tmem_base;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
 
-  // Registers: launched with 384 x 168 = 64512; 128 x 80 + 256 x 208 = 63488 after the exchange.
   if (warp < 4) {
-  reg_dec<80>();
+  reg_dec<kFwdRegsControl>();
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -152,7 +142,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
       for (int t = 0; t < 2; ++t) {
-        if (tokens(t) <= 0) continue;
+        if (blocks(t) == 0) continue;                        // (its rows, zeros, may be staged there at once)
         mbar_expect_tx(&ctl->q_full[t], p.tok * p.group * D * 2);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
@@ -260,7 +250,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   }
   } else {
     // ----------------------------------------------------------------- softmax
-    reg_inc<208>();
+    reg_inc<kFwdRegsSoftmax>();
     const int t = (warp - 4) >> 2;
     const int nt = blocks(t), nother = blocks(1 - t);
     const int quarter = warp & 3;
@@ -359,7 +349,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             float x0, x1;
-            fma2(x0, x1, __uint_as_float(s[v * 16 + i]), __uint_as_float(s[v * 16 + i + 1]), sc, neg_m);
+            fma2(x0, x1, __uint_as_float(s[v * 16 + i]), __uint_as_float(s[v * 16 + i + 1]), sc, neg_m, neg_m);
             x0 = ex2_approx(x0);
             x1 = ex2_approx(x1);
             add2(l0, l1, x0, x1);
@@ -415,7 +405,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (row_ok && p.lse != nullptr)
           p.lse[static_cast<int64_t>(head) * p.Tq + token] = l == 0.f ? ninf : (m_used + log2f(l)) * 0.6931471805599453f;
-        uint16_t* orow = static_cast<uint16_t*>(p.o) + token * p.os_t + head * p.os_h;
+        // (the tile's Q is no longer needed: its last scores are done)
+        const uint32_t stage = smem_u32(smem + t * Cfg::kTileBytes);
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {
           uint32_t o[16];
@@ -426,16 +417,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] = 0u;
           }
-#pragma unroll
-          for (int i = 0; i < 16; i += 8) {
-            if (!row_ok || c * 16 + i >= p.d) continue;
-            uint32_t w4[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              w4[q] = pack_bf16x2(__uint_as_float(o[i + 2 * q]) * inv, __uint_as_float(o[i + 2 * q + 1]) * inv);
-            *reinterpret_cast<uint4*>(orow + c * 16 + i) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-          }
+          stage16<D>(stage, row, c, o, inv);
         }
+        __syncwarp();
+        uint16_t* out = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(u.t0 + t * p.tok) * p.os_t +
+                        static_cast<int64_t>(kvh) * p.group * p.os_h;
+        write_staged<D>(stage, quarter * 32, min(rows, quarter * 32 + 32), p.d,
+                        [&](int r) { return out + (r / p.group) * p.os_t + (r % p.group) * p.os_h; });
       }
     }
   }
@@ -488,6 +476,8 @@ __global__ void __launch_bounds__(256) packed_attn_join_kernel(const PackedJoin*
 template <int D>
 int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PackedFwdParams& p,
                const PackedHeader& h, const int32_t* plan, cudaStream_t st) {
+  static const bool fits = registers_suffice(packed_attn_fwd_kernel<D>, kFwdThreads, kFwdRegs);
+  if (!fits) return SWV_ERR_CUDA;
   SWV_CUDA_OK(cudaFuncSetAttribute(packed_attn_fwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(fwd_smem<D>())));
   packed_attn_fwd_kernel<D><<<static_cast<unsigned>(p.n_units) * p.Hkv, kFwdThreads, fwd_smem<D>(), st>>>(tq, tk, tv, p);

@@ -13,8 +13,8 @@
 //   kDkv : lanes = keys;    streamed: Q (ring A), dO (ring B)     S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
 //   kDq  : lanes = queries; streamed: K (ring A), V (ring B)      S = Q K^T,   dP = dO V^T,   dQ += dS K
 // warp 0: TMA producer; warp 1: issues the products; warp 2: lse and delta of the streamed rows (kDkv); warp 3: zeroes the
-// streamed rows behind the sequence's end (they are summed over, and 0 x NaN would reach the sums); warps 4..11: eight
-// warps turn a tile's S and dP into P and dS, (row quarter, half of the columns) each.  P and dS go back into TMEM as bf16 pairs over the
+// streamed rows behind the sequence's end (they are summed over, and 0 x NaN would reach the sums); warps 4..19: sixteen
+// warps turn a tile's S and dP into P and dS, (row quarter, 32 of the columns) each.  P and dS go back into TMEM as bf16 pairs over the
 // columns that the warp read, as the A operand of the gradient products (16-bit operands: 2^-9 of each entry, independent).
 // TMEM: kDkv  S [0,128), dP [128,256), dV [256,256+D), dK [256+D,256+2D)
 //       kDq   S twice [0,256), dP [256,384), dQ [384,384+D)
@@ -34,12 +34,15 @@ int packed_plan_header(const int32_t* plan_host, PackedHeader* h);
 namespace {
 
 enum { kDkv = 0, kDq = 1 };
-constexpr int kBwdThreads = 384;
+constexpr int kBwdWarps = 16;                  // warps that turn a tile's products into P and dS, 32 columns each
+constexpr int kBwdThreads = 128 + 32 * kBwdWarps;
+constexpr int kBwdRegsControl = 64, kBwdRegsTerms = 104;        // of 640 x 96 = 61440 at launch: all
+constexpr int kBwdRegs = 128 * kBwdRegsControl + 32 * kBwdWarps * kBwdRegsTerms;
 
 struct PackedBwdParams {
   const PackedUnit* units;
   int n_units, group, tok, Tq, d, Hkv, heads_at_once;
-  const float2* stats;          // [Hkv][Tq][group] {lse in powers of two, delta}; +inf where a row sees no key
+  const float2* stats;          // [Hkv][Tq][group] {-lse in powers of two, -delta}; -inf where a row sees no key
   void *g1, *g2;                // kDkv: dK, dV; kDq: dQ
   int64_t g1_t, g1_h, g2_t, g2_h;
   float scale, scale_log2;
@@ -59,7 +62,7 @@ struct BwdCfg {
 };
 struct BwdCtl {
   uint64_t lane_full, a_full[4], a_empty[4], b_full[4], b_empty[4], tail_a, tail_b;
-  uint64_t s_full[2], dp_full, p_ready, ds_ready, p_done, ds_done, all_done, stat_full[2], stat_empty[2];
+  uint64_t s_full[2], dp_full, p_ready, ds_ready, p_done, ds_done, all_done, stat_full[2], stat_empty[2], staged;
   uint32_t tmem_base, abort_flag;
 };
 template <int D, int MODE>
@@ -118,14 +121,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ctl->s_full[s], 1);
       mbar_init(&ctl->stat_full[s], 1);
-      mbar_init(&ctl->stat_empty[s], 8);
+      mbar_init(&ctl->stat_empty[s], kBwdWarps);
     }
     mbar_init(&ctl->dp_full, 1);
-    mbar_init(&ctl->p_ready, 8);
-    mbar_init(&ctl->ds_ready, 8);
+    mbar_init(&ctl->p_ready, kBwdWarps);
+    mbar_init(&ctl->ds_ready, kBwdWarps);
     mbar_init(&ctl->p_done, 1);
     mbar_init(&ctl->ds_done, 1);
     mbar_init(&ctl->all_done, 1);
+    mbar_init(&ctl->staged, kBwdWarps);
     ctl->abort_flag = 0;
     fence_barrier_init();
   }
@@ -149,6 +153,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     return false;
   };
 
+  if (warp < 4) {
+  reg_dec<kBwdRegsControl>();
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -207,7 +213,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint64_t db = smem_desc_sw128(b, kTile * 128);
 #pragma unroll
         for (int ks = 0; ks < kTile / 16; ++ks) 
-          umma_f16_ts(col, a_col + (ks >> 2) * 64 + (ks & 3) * 8, db + ks * 128, kIdescG, !first || ks > 0);
+          umma_f16_ts(col, a_col + (ks >> 1) * 32 + (ks & 1) * 8, db + ks * 128, kIdescG, !first || ks > 0);
       };
       if constexpr (MODE == kDkv) {
         for (int j = 0; ok && j < n; ++j) {
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = i * 32 + lane;
-          f[i] = r < rows ? __ldg(src + r) : make_float2(__int_as_float(0x7f800000), 0.f);
+          f[i] = r < rows ? __ldg(src + r) : make_float2(-__int_as_float(0x7f800000), 0.f);
         }
         bool ok = j < 2 || wait(&ctl->stat_empty[j & 1], ((j >> 1) & 1) ^ 1, kDevWaitPReady);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -299,7 +305,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (lane == 0) mbar_arrive(&ctl->stat_full[j & 1]);
       }
     }
-  } else if (warp == 3) {
+  } else {
     if (tail) {
       bool ok = wait(&ctl->tail_a, 0, kDevWaitTmaFull) && (MODE == kDq || wait(&ctl->tail_b, 0, kDevWaitTmaFull));
       if (__all_sync(0xffffffffu, ok)) {
@@ -314,33 +320,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
     }
+  }
   } else {
-    // ------------------------------- eight warps: (row quarter, half of the columns)
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const int row = quarter * 32 + lane, c0 = half * 64;
+    // ------------------------------- sixteen warps: (row quarter, 32 of the columns)
+    reg_inc<kBwdRegsTerms>();
+    const int quarter = warp & 3, grp = (warp - 4) >> 2;
+    const int row = quarter * 32 + lane, c0 = grp * 32;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const float c2 = p.scale_log2;
     bool ok = true;
-    float lse2 = 0.f, delta = 0.f;
+    float neg_lse = 0.f, neg_delta = 0.f;
     int limit = 0;                                             // kDq: keys the row sees from block b0 on
     const int rows = MODE == kDkv ? u.n : u.n * p.group;
     const bool row_ok = row < rows;
     const int tk = MODE == kDkv ? row : row / p.group;         // token of the lane side
     if (MODE == kDq && row_ok) {
       const float2 f = __ldg(p.stats + (static_cast<int64_t>(kvh) * p.Tq + u.t0) * p.group + row);
-      lse2 = f.x;
-      delta = f.y;
+      neg_lse = f.x;
+      neg_delta = f.y;
       limit = min(u.len, u.off + tk + 1) - u.b0 * kTile;
     }
     for (int j = 0; j < n; ++j) {
-      const uint32_t s_col = tmem_base + lane_off + (MODE == kDq ? (j & 1) * 128 : 0);
-      const uint32_t dp_col = tmem_base + lane_off + kColDp;
-      ok = wait(MODE == kDq ? &ctl->s_full[j & 1] : &ctl->s_full[0], MODE == kDq ? (j >> 1) & 1 : j & 1, kDevWaitAccFull) &&
-           (MODE == kDq || wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitAccFull));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      const float* st = stats + (j & 1) * 2 * kTile;
+      const uint32_t s_col = tmem_base + lane_off + (MODE == kDq ? (j & 1) * 128 : 0) + c0;
+      const uint32_t dp_col = tmem_base + lane_off + kColDp + c0;
       // the columns that the row sees: keys before its limit, or queries from `lo` on
       int lo = 0, hi;
       if (MODE == kDq) {
@@ -350,36 +352,39 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         lo = min(max(u.off + row - tok0, 0), step) * p.group;
         hi = min(step, u.len - tok0) * p.group;
       }
-      uint32_t vis[2] = {column_bits(lo, hi, c0), column_bits(lo, hi, c0 + 32)};
-      const bool all = __all_sync(0xffffffffu, (vis[0] & vis[1]) == 0xffffffffu);
-      float pr[64];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      const uint32_t vis = column_bits(lo, hi, c0);
+      const bool all = __all_sync(0xffffffffu, vis == 0xffffffffu);
+      ok = wait(MODE == kDq ? &ctl->s_full[j & 1] : &ctl->s_full[0], MODE == kDq ? (j >> 1) & 1 : j & 1, kDevWaitAccFull) &&
+           (MODE == kDq || wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitAccFull));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const float* st = stats + (j & 1) * 2 * kTile + c0;
+      float pr[32];
+      {
         uint32_t s[32];
-        tmem_ld32(s_col + c0 + c * 32, s);
+        tmem_ld32(s_col, s);
         tc_wait_ld();
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          float4 l = make_float4(lse2, lse2, lse2, lse2);
-          if (MODE == kDkv) l = *reinterpret_cast<const float4*>(st + c0 + c * 32 + i);
-          const float lv[4] = {l.x, l.y, l.z, l.w};
+          float4 l = make_float4(neg_lse, neg_lse, neg_lse, neg_lse);
+          if (MODE == kDkv) l = *reinterpret_cast<const float4*>(st + i);
+          fma2(pr[i], pr[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), c2, l.x, l.y);
+          fma2(pr[i + 2], pr[i + 3], __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]), c2, l.z, l.w);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) pr[c * 32 + i + e] = ex2_approx(fmaf(__uint_as_float(s[i + e]), c2, -lv[e]));
+          for (int e = 0; e < 4; ++e) pr[i + e] = ex2_approx(pr[i + e]);
         }
         if (!all) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (!((vis[c] >> i) & 1u)) pr[c * 32 + i] = 0.f;
+            if (!((vis >> i) & 1u)) pr[i] = 0.f;
         }
       }
       if (MODE == kDkv) {
+        uint32_t w[16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(pr[c * 16 + 2 * i], pr[c * 16 + 2 * i + 1]);
-          tmem_st8(s_col + c0 + c * 8, w);
-        }
+        for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(pr[2 * i], pr[2 * i + 1]);
+        tmem_st16(s_col, w);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -389,29 +394,33 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      uint32_t w[32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      uint32_t w[16];
+      {
         uint32_t x[32];
-        tmem_ld32(dp_col + c0 + c * 32, x);
+        tmem_ld32(dp_col, x);
         tc_wait_ld();
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          float4 dl = make_float4(delta, delta, delta, delta);
-          if (MODE == kDkv) dl = *reinterpret_cast<const float4*>(st + kTile + c0 + c * 32 + i);
-          const float dv[4] = {dl.x, dl.y, dl.z, dl.w};
+          float4 dl = make_float4(neg_delta, neg_delta, neg_delta, neg_delta);
+          if (MODE == kDkv) dl = *reinterpret_cast<const float4*>(st + kTile + i);
           float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y[e] = pr[c * 32 + i + e] * (__uint_as_float(x[i + e]) - dv[e]);
+          for (int e = 0; e < 4; ++e) y[e] = __uint_as_float(x[i + e]);
+          add2(y[0], y[1], dl.x, dl.y);
+          add2(y[2], y[3], dl.z, dl.w);
+          mul2(y[0], y[1], pr[i], pr[i + 1]);
+          mul2(y[2], y[3], pr[i + 2], pr[i + 3]);
+          if (!all) {
             // (a selection: what lies behind the sequence may be infinite)
-            if (!all && !((vis[c] >> (i + e)) & 1u)) y[e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!((vis >> (i + e)) & 1u)) y[e] = 0.f;
           }
-          w[c * 16 + i / 2] = pack_bf16x2(y[0], y[1]);
-          w[c * 16 + i / 2 + 1] = pack_bf16x2(y[2], y[3]);
+          w[i / 2] = pack_bf16x2(y[0], y[1]);
+          w[i / 2 + 1] = pack_bf16x2(y[2], y[3]);
         }
       }
-      tmem_st32((MODE == kDkv ? dp_col : s_col) + c0, w);      // dS over dP (kDkv) or over S (kDq)
+      tmem_st16(MODE == kDkv ? dp_col : s_col, w);             // dS over dP (kDkv) or over S (kDq)
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -423,20 +432,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (ok && n > 0) ok = wait(&ctl->all_done, 0, kDevWaitPvDone);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
+    // The gradients: kDkv groups 0 and 1 take the halves of dV, 2 and 3 those of dK; kDq each a quarter of dQ.
+    constexpr int kCols = MODE == kDkv ? D / 2 : D / 4;
+    constexpr int kWidth = MODE == kDkv ? 2 * D : D;
+    const uint32_t col = tmem_base + lane_off + kColG + grp * kCols;
+    const bool is_dv = MODE == kDkv && grp < 2;
+    const bool divided = u.slot >= 0;
+    // (the lane side's tiles are no longer needed: dV or dQ over the first, dK over the second)
+    const uint32_t stage = smem_u32(smem) + (MODE == kDkv && !is_dv ? TB : 0);
+    const int ch0 = MODE == kDkv ? (grp & 1) * kCols : grp * kCols;
     if (ok) {
-      // the gradients' columns: kDkv half 0 writes dV, half 1 dK; kDq each half of dQ's columns
-      constexpr int kCols = MODE == kDkv ? D : D / 2;
-      const uint32_t col = tmem_base + lane_off + kColG + half * kCols;
-      const bool divided = u.slot >= 0;
-      const bool is_dv = MODE == kDkv && half == 0;
       const float f = is_dv ? 1.f : p.scale;
-      const int64_t token = u.t0 + tk;
-      const int head = MODE == kDkv ? kvh : kvh * p.group + row % p.group;
-      uint16_t* out = is_dv ? static_cast<uint16_t*>(p.g2) + token * p.g2_t + head * p.g2_h
-                            : static_cast<uint16_t*>(p.g1) + token * p.g1_t + head * p.g1_h;
-      constexpr int kWidth = MODE == kDkv ? 2 * D : D;
-      float* part = p.part + ((static_cast<int64_t>(divided ? u.slot : 0) * p.Hkv + kvh) * kTile + row) * kWidth + half * kCols;
-      const int ch0 = MODE == kDkv ? 0 : half * kCols;         // first channel
+      float* part = p.part + ((static_cast<int64_t>(divided ? u.slot : 0) * p.Hkv + kvh) * kTile + row) * kWidth + grp * kCols;
 #pragma unroll 1
       for (int c = 0; c < kCols / 16; ++c) {
         uint32_t o[16];
@@ -447,22 +454,32 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = 0u;
         }
-        if (!row_ok) continue;
-        if (divided) {
+        if (!divided) {
+          stage16<D>(stage, row, ch0 / 16 + c, o, f);
+        } else if (row_ok) {
 #pragma unroll
           for (int i = 0; i < 16; i += 4)
             *reinterpret_cast<uint4*>(part + c * 16 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i += 8) {
-            if (ch0 + c * 16 + i >= p.d) continue;
-            uint32_t w4[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              w4[q] = pack_bf16x2(__uint_as_float(o[i + 2 * q]) * f, __uint_as_float(o[i + 2 * q + 1]) * f);
-            *reinterpret_cast<uint4*>(out + ch0 + c * 16 + i) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-          }
         }
+      }
+    }
+    if (ok && !divided) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->staged);
+      ok = wait(&ctl->staged, 0, kDevWaitAccEmpty);
+      ok = __all_sync(0xffffffffu, ok);
+      // sixteen warps write eight rows each of every gradient
+      const int r0 = (warp - 4) * 8, r1 = min(rows, r0 + 8);
+      if (ok && MODE == kDkv) {
+        uint16_t* dv = static_cast<uint16_t*>(p.g2) + static_cast<int64_t>(u.t0) * p.g2_t + static_cast<int64_t>(kvh) * p.g2_h;
+        uint16_t* dk = static_cast<uint16_t*>(p.g1) + static_cast<int64_t>(u.t0) * p.g1_t + static_cast<int64_t>(kvh) * p.g1_h;
+        write_staged<D>(smem_u32(smem), r0, r1, p.d, [&](int r) { return dv + r * p.g2_t; });
+        write_staged<D>(smem_u32(smem) + TB, r0, r1, p.d, [&](int r) { return dk + r * p.g1_t; });
+      } else if (ok) {
+        uint16_t* dq = static_cast<uint16_t*>(p.g1) + static_cast<int64_t>(u.t0) * p.g1_t +
+                       static_cast<int64_t>(kvh) * p.group * p.g1_h;
+        write_staged<D>(smem_u32(smem), r0, r1, p.d,
+                        [&](int r) { return dq + (r / p.group) * p.g1_t + (r % p.group) * p.g1_h; });
       }
     }
   }
@@ -476,7 +493,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   }
 }
 
-// delta = dO . O per row, and lse in powers of two; half a warp a row.
+// -delta = -dO . O per row, and -lse in powers of two; half a warp a row.
 __global__ void __launch_bounds__(256) packed_attn_delta_kernel(const __nv_bfloat16* o, int64_t os_t, int64_t os_h,
                                                                 const __nv_bfloat16* g, int64_t gs_t, int64_t gs_h,
                                                                 const float* lse, float2* stats, int64_t rows, int Tq,
@@ -507,7 +524,7 @@ __global__ void __launch_bounds__(256) packed_attn_delta_kernel(const __nv_bfloa
   if (sub == 0) {
     const float l = lse[static_cast<int64_t>(head) * Tq + t];
     const float inf = __int_as_float(0x7f800000);
-    stats[(static_cast<int64_t>(kvh) * Tq + t) * group + hg] = make_float2(l == -inf ? inf : l * 1.4426950408889634f, a);
+    stats[(static_cast<int64_t>(kvh) * Tq + t) * group + hg] = make_float2(l == -inf ? -inf : l * -1.4426950408889634f, -a);
   }
 }
 
@@ -542,6 +559,8 @@ template <int D, int MODE>
 int launch_bwd(const CUtensorMap& l1, const CUtensorMap& l2, const CUtensorMap& a, const CUtensorMap& b,
                const PackedBwdParams& p, const PackedJoin* joins, int n_join, cudaStream_t st) {
   if (p.n_units == 0) return SWV_OK;
+  static const bool fits = registers_suffice(packed_attn_bwd_kernel<D, MODE>, kBwdThreads, kBwdRegs);
+  if (!fits) return SWV_ERR_CUDA;
   SWV_CUDA_OK(cudaFuncSetAttribute(packed_attn_bwd_kernel<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(bwd_smem<D, MODE>())));
   packed_attn_bwd_kernel<D, MODE>
