@@ -14,9 +14,11 @@
 //   kDq  : lanes = queries; streamed: K (ring A), V (ring B)      S = Q K^T,   dP = dO V^T,   dQ += dS K
 // warp 0: TMA producer; warp 1: issues the products; warp 2: lse and delta of the streamed rows (kDkv); warp 3: zeroes the
 // streamed rows behind the sequence's end (they are summed over, and 0 x NaN would reach the sums); warps 4..19: sixteen
-// warps turn a tile's S and dP into P and dS, (row quarter, 32 of the columns) each.  P and dS go back into TMEM as bf16 pairs over the
+// warps turn a tile's S and dP into P and dS, (row quarter, 32 of the columns) each.  kDkv writes both over dP once that is in
+// registers, so the next scores are formed while P is computed (P over S: 603 us where this takes {T} at 8192 causal tokens,
+// 16 heads of 128 sharing two key heads).  P and dS go back into TMEM as bf16 pairs over the
 // columns that the warp read, as the A operand of the gradient products (16-bit operands: 2^-9 of each entry, independent).
-// TMEM: kDkv  S [0,128), dP [128,256), dV [256,256+D), dK [256+D,256+2D)
+// TMEM: kDkv  S [0,128), dP [128,256) (D = 64: two tiles, [128,384)), then dV and dK
 //       kDq   S twice [0,256), dP [256,384), dQ [384,384+D)
 #include <algorithm>
 #include <cmath>
@@ -57,12 +59,17 @@ struct BwdCfg {
   static constexpr int kB = D == 64 ? 4 : (MODE == kDkv ? 2 : 1);
   static constexpr int kOffA = 2 * kTileBytes;
   static constexpr int kOffB = kOffA + kA * kTileBytes;
-  static constexpr int kOffStats = kOffB + kB * kTileBytes;             // [2][2][128] floats
-  static constexpr int kOffCtl = kOffStats + 2 * 2 * kTile * 4;
+  // kDkv: two tiles of 128 rows of 128 bytes (see the warp that fills them)
+  static constexpr int kOffOnes = kOffB + kB * kTileBytes;
+  static constexpr int kOffStats = kOffOnes + (MODE == kDkv ? kTile * 128 : 0);
+  static constexpr int kOffCtl = kOffStats + (MODE == kDkv ? kTile * 128 : 0);
+  static constexpr int kY = MODE == kDkv && D == 64 ? 2 : 1;            // dP tiles in TMEM
+  static constexpr uint32_t kColDp = MODE == kDkv ? 128 : 256;
+  static constexpr uint32_t kColG = kColDp + kY * 128;
 };
 struct BwdCtl {
   uint64_t lane_full, a_full[4], a_empty[4], b_full[4], b_empty[4], tail_a, tail_b;
-  uint64_t s_full[2], dp_full, p_ready, ds_ready, p_done, ds_done, all_done, stat_full[2], stat_empty[2], staged;
+  uint64_t s_full[2], s_read, dp_full[2], ds_ready[2], ds_done, all_done, stat_full[2], stat_empty[2], staged;
   uint32_t tmem_base, abort_flag;
 };
 template <int D, int MODE>
@@ -91,13 +98,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   constexpr int NA = Cfg::kA, NB = Cfg::kB, TB = Cfg::kTileBytes;
   constexpr uint32_t kIdescS = make_idesc(/*bf16*/ 1, kTile, kTile, 0, 0);
   constexpr uint32_t kIdescG = make_idesc(/*bf16*/ 1, kTile, D, 0, /*B is MN-major*/ 1);
-  constexpr uint32_t kColDp = MODE == kDkv ? 128 : 256;
-  constexpr uint32_t kColG = MODE == kDkv ? 256 : 384;
+  constexpr int kY = Cfg::kY;
+  constexpr uint32_t kColDp = Cfg::kColDp, kColG = Cfg::kColG;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   BwdCtl* ctl = reinterpret_cast<BwdCtl*>(smem + Cfg::kOffCtl);
-  float* stats = reinterpret_cast<float*>(smem + Cfg::kOffStats);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   int kvh;
@@ -121,12 +127,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ctl->s_full[s], 1);
       mbar_init(&ctl->stat_full[s], 1);
-      mbar_init(&ctl->stat_empty[s], kBwdWarps);
+      mbar_init(&ctl->stat_empty[s], 1);
+      mbar_init(&ctl->dp_full[s], 1);
+      mbar_init(&ctl->ds_ready[s], kBwdWarps);
     }
-    mbar_init(&ctl->dp_full, 1);
-    mbar_init(&ctl->p_ready, kBwdWarps);
-    mbar_init(&ctl->ds_ready, kBwdWarps);
-    mbar_init(&ctl->p_done, 1);
+    mbar_init(&ctl->s_read, kBwdWarps);
     mbar_init(&ctl->ds_done, 1);
     mbar_init(&ctl->all_done, 1);
     mbar_init(&ctl->staged, kBwdWarps);
@@ -137,9 +142,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
   }
-  if (MODE == kDkv && per < kTile) {
+  if (MODE == kDkv) {
     // rows that no load fills: they are summed over as zeros
-    for (int s = 0; s < NA + NB; ++s) zero_rows<D>(smem_u32(smem + Cfg::kOffA + s * TB), per, threadIdx.x, kBwdThreads);
+    if (per < kTile)
+      for (int s = 0; s < NA + NB; ++s) zero_rows<D>(smem_u32(smem + Cfg::kOffA + s * TB), per, threadIdx.x, kBwdThreads);
+    // row r of the tile of ones: {1, 1, 1, 0, ...} in its first 16 channels
+    for (int i = threadIdx.x; i < kTile * 8; i += kBwdThreads) {
+      const int r = i >> 3, chunk = (i & 7) ^ (r & 7);
+      sts128(smem_u32(smem + Cfg::kOffOnes) + i * 16, chunk == 0 ? 0x3f803f80u : 0u, chunk == 0 ? 0x3f80u : 0u, 0u, 0u);
+      sts128(smem_u32(smem + Cfg::kOffStats) + i * 16, 0u, 0u, 0u, 0u);
+    }
     fence_proxy_async_smem();
   }
   tc_fence_before();
@@ -200,6 +212,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // -------------------------------------------------------------- MMA issuer
     if (lane == 0 && n > 0) {
       const uint32_t l1 = smem_u32(smem), l2 = l1 + TB, ra = l1 + Cfg::kOffA, rb = l1 + Cfg::kOffB;
+      // col += 1 x (row statistic of the streamed side): 16 more channels, see the warp that fills them
+      auto plus_stat = [&](uint32_t col, int channels16) {
+        umma_f16_ss(col, smem_desc_sw128(l1 + Cfg::kOffOnes), smem_desc_sw128(l1 + Cfg::kOffStats) + channels16 * 2, kIdescS, 1);
+      };
       bool ok = wait(&ctl->lane_full, 0, kDevWaitQ);
       auto product = [&](uint32_t col, uint32_t a, uint32_t b) {          // both operands along the channels
         const uint64_t da = smem_desc_sw128(a), db = smem_desc_sw128(b);
@@ -216,39 +232,43 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           umma_f16_ts(col, a_col + (ks >> 1) * 32 + (ks & 1) * 8, db + ks * 128, kIdescG, !first || ks > 0);
       };
       if constexpr (MODE == kDkv) {
-        for (int j = 0; ok && j < n; ++j) {
-          const int sa = j % NA, sb = j % NB;
-          ok = wait(&ctl->a_full[sa], (j / NA) & 1, kDevWaitTmaFull) &&
-               (j == 0 || wait(&ctl->p_done, (j - 1) & 1, kDevWaitPvDone));          // P(j-1) lies where S(j) goes
-          if (!ok) break;
+        auto scores = [&](int j) {
+          if (!wait(&ctl->a_full[j % NA], (j / NA) & 1, kDevWaitTmaFull) ||
+              !wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitTmaFull) ||
+              (j > 0 && !wait(&ctl->s_read, (j - 1) & 1, kDevWaitAccEmpty)))
+            return false;
           tc_fence_after();
-          product(tmem_base, l1, ra + sa * TB);
+          product(tmem_base, l1, ra + (j % NA) * TB);
+          plus_stat(tmem_base, (j & 1) * 2);
           umma_commit(&ctl->s_full[0]);
-          if (j > 0) {
-            ok = wait(&ctl->ds_ready, (j - 1) & 1, kDevWaitPReady);
-            if (!ok) break;
-            tc_fence_after();
-            gradient(tmem_base + kColG + D, tmem_base + kColDp, ra + ((j - 1) % NA) * TB, j == 1);
-            umma_commit(&ctl->a_empty[(j - 1) % NA]);
-            umma_commit(&ctl->ds_done);
-          }
-          ok = wait(&ctl->b_full[sb], (j / NB) & 1, kDevWaitTmaFull) &&
-               (j == 0 || wait(&ctl->ds_done, (j - 1) & 1, kDevWaitPvDone));
+          return true;
+        };
+        auto inner = [&](int j) {
+          // P and dS of tile j - kY lay where dP(j) goes
+          if (!wait(&ctl->b_full[j % NB], (j / NB) & 1, kDevWaitTmaFull) ||
+              (j >= kY && !wait(&ctl->ds_done, (j - kY) & 1, kDevWaitPvDone)))
+            return false;
+          tc_fence_after();
+          const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
+          product(col, l2, rb + (j % NB) * TB);
+          plus_stat(col, (j & 1) * 2 + 1);
+          umma_commit(&ctl->stat_empty[j & 1]);
+          umma_commit(&ctl->dp_full[j & 1]);
+          return true;
+        };
+        ok = ok && scores(0) && inner(0);
+        for (int j = 0; ok && j < n; ++j) {
+          ok = (j + 1 == n || scores(j + 1)) && (j + 1 == n || kY == 1 || inner(j + 1)) &&
+               wait(&ctl->ds_ready[j & 1], (j >> 1) & 1, kDevWaitPReady);
           if (!ok) break;
           tc_fence_after();
-          product(tmem_base + kColDp, l2, rb + sb * TB);
-          umma_commit(&ctl->dp_full);
-          ok = wait(&ctl->p_ready, j & 1, kDevWaitPReady);
-          if (!ok) break;
-          tc_fence_after();
-          gradient(tmem_base + kColG, tmem_base, rb + sb * TB, j == 0);
-          umma_commit(&ctl->b_empty[sb]);
-          umma_commit(&ctl->p_done);
-        }
-        if (ok && wait(&ctl->ds_ready, (n - 1) & 1, kDevWaitPReady)) {
-          tc_fence_after();
-          gradient(tmem_base + kColG + D, tmem_base + kColDp, ra + ((n - 1) % NA) * TB, n == 1);
-          umma_commit(&ctl->all_done);
+          const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
+          gradient(tmem_base + kColG, col, rb + (j % NB) * TB, j == 0);
+          umma_commit(&ctl->b_empty[j % NB]);
+          gradient(tmem_base + kColG + D, col + 16, ra + (j % NA) * TB, j == 0);
+          umma_commit(&ctl->a_empty[j % NA]);
+          umma_commit(j + 1 < n ? &ctl->ds_done : &ctl->all_done);
+          if (kY == 1 && j + 1 < n) ok = inner(j + 1);
         }
       } else {
         auto scores = [&](int j) {
@@ -269,9 +289,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tc_fence_after();
           product(tmem_base + kColDp, l2, rb + (j % NB) * TB);
           umma_commit(&ctl->b_empty[j % NB]);
-          umma_commit(&ctl->dp_full);
+          umma_commit(&ctl->dp_full[j & 1]);
           if (j + 1 < n) ok = scores(j + 1);
-          ok = ok && wait(&ctl->ds_ready, j & 1, kDevWaitPReady);
+          ok = ok && wait(&ctl->ds_ready[j & 1], (j >> 1) & 1, kDevWaitPReady);
           if (!ok) break;
           tc_fence_after();
           gradient(tmem_base + kColG, tmem_base + (j & 1) * 128, ra + (j % NA) * TB, j == 0);
@@ -281,8 +301,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
   } else if (warp == 2) {
-    // --------------------------- lse and delta of the streamed rows, two tiles ahead at most
+    // Row statistics of the streamed queries (kDkv).  S - lse / scale and dP - delta are formed by the products themselves: a
+    // tile of ones times the statistic, as three bf16 terms whose sum has all 24 bits (the columns' values read from
+    // shared memory by every thread cost 65 of 419 us at 3 bags of 12 heads of 64).  Channels of the 128-byte rows: two tiles' lse
+    // and delta in 16 each, of which three are used.
     if (MODE == kDkv) {
+      const uint32_t tile = smem_u32(smem + Cfg::kOffStats);
+      const float per_score = 1.f / p.scale_log2;
       for (int j = 0; j < n; ++j) {
         const int tok0 = (u.b0 + j) * step;
         const int rows = min(step, u.len - tok0) * p.group;
@@ -291,16 +316,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = i * 32 + lane;
-          f[i] = r < rows ? __ldg(src + r) : make_float2(-__int_as_float(0x7f800000), 0.f);
+          f[i] = r < rows ? __ldg(src + r) : make_float2(0.f, 0.f);
         }
-        bool ok = j < 2 || wait(&ctl->stat_empty[j & 1], ((j >> 1) & 1) ^ 1, kDevWaitPReady);
+        bool ok = j < 2 || wait(&ctl->stat_empty[j & 1], ((j >> 1) & 1) ^ 1, kDevWaitAccEmpty);
         if (!__all_sync(0xffffffffu, ok)) break;
-        float* st = stats + (j & 1) * 2 * kTile;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          st[i * 32 + lane] = f[i].x;
-          st[kTile + i * 32 + lane] = f[i].y;
+          const int r = i * 32 + lane;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float x = k == 0 ? f[i].x * per_score : f[i].y;
+            const uint32_t hi = __float_as_uint(x) & 0xffff0000u;
+            const bool finite = fabsf(x) < __int_as_float(0x7f800000);
+            const float y = finite ? x - __uint_as_float(hi) : 0.f;      // (an infinity is one term; NaN stays in the first)
+            const uint32_t mid = __float_as_uint(y) & 0xffff0000u;
+            const uint32_t lo = __float_as_uint(y - __uint_as_float(mid));
+            const int chunk = ((j & 1) * 2 + k) * 2;
+            sts128(tile + r * 128 + ((chunk ^ (r & 7)) << 4), ((x == x ? hi : 0x7fc00000u) >> 16) | mid, lo >> 16, 0u, 0u);
+          }
         }
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->stat_full[j & 1]);
       }
@@ -342,7 +377,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     for (int j = 0; j < n; ++j) {
       const uint32_t s_col = tmem_base + lane_off + (MODE == kDq ? (j & 1) * 128 : 0) + c0;
-      const uint32_t dp_col = tmem_base + lane_off + kColDp + c0;
+      const uint32_t dp_col = tmem_base + lane_off + kColDp + (j % kY) * 128 + c0;
       // the columns that the row sees: keys before its limit, or queries from `lo` on
       int lo = 0, hi;
       if (MODE == kDq) {
@@ -354,25 +389,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       const uint32_t vis = column_bits(lo, hi, c0);
       const bool all = __all_sync(0xffffffffu, vis == 0xffffffffu);
-      ok = wait(MODE == kDq ? &ctl->s_full[j & 1] : &ctl->s_full[0], MODE == kDq ? (j >> 1) & 1 : j & 1, kDevWaitAccFull) &&
-           (MODE == kDq || wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitAccFull));
+      ok = wait(MODE == kDq ? &ctl->s_full[j & 1] : &ctl->s_full[0], MODE == kDq ? (j >> 1) & 1 : j & 1, kDevWaitAccFull);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const float* st = stats + (j & 1) * 2 * kTile + c0;
       float pr[32];
       {
         uint32_t s[32];
         tmem_ld32(s_col, s);
         tc_wait_ld();
+        if (MODE == kDkv) {                                    // S(j+1) may go there
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->s_read);
+        }
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float4 l = make_float4(neg_lse, neg_lse, neg_lse, neg_lse);
-          if (MODE == kDkv) l = *reinterpret_cast<const float4*>(st + i);
-          fma2(pr[i], pr[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), c2, l.x, l.y);
-          fma2(pr[i + 2], pr[i + 3], __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]), c2, l.z, l.w);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pr[i + e] = ex2_approx(pr[i + e]);
+        for (int i = 0; i < 32; i += 2) {                      // (kDkv: the scores hold -lse already)
+          fma2(pr[i], pr[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), c2, neg_lse, neg_lse);
+          pr[i] = ex2_approx(pr[i]);
+          pr[i + 1] = ex2_approx(pr[i + 1]);
         }
         if (!all) {
 #pragma unroll
@@ -380,17 +415,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             if (!((vis >> i) & 1u)) pr[i] = 0.f;
         }
       }
-      if (MODE == kDkv) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(pr[2 * i], pr[2 * i + 1]);
-        tmem_st16(s_col, w);
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->p_ready);
-      }
-      ok = wait(&ctl->dp_full, j & 1, kDevWaitAccFull);
+      ok = wait(&ctl->dp_full[j & 1], (j >> 1) & 1, kDevWaitAccFull);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -399,35 +424,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint32_t x[32];
         tmem_ld32(dp_col, x);
         tc_wait_ld();
+        if (MODE == kDkv) {                                    // P over the first half of the warp's own columns of dP
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float4 dl = make_float4(neg_delta, neg_delta, neg_delta, neg_delta);
-          if (MODE == kDkv) dl = *reinterpret_cast<const float4*>(st + kTile + i);
-          float y[4];
+          for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(pr[2 * i], pr[2 * i + 1]);
+          tmem_st16(dp_col, w);
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = __uint_as_float(x[i + e]);
-          add2(y[0], y[1], dl.x, dl.y);
-          add2(y[2], y[3], dl.z, dl.w);
-          mul2(y[0], y[1], pr[i], pr[i + 1]);
-          mul2(y[2], y[3], pr[i + 2], pr[i + 3]);
+        for (int i = 0; i < 32; i += 2) {
+          float y0 = __uint_as_float(x[i]), y1 = __uint_as_float(x[i + 1]);
+          if (MODE == kDq) add2(y0, y1, neg_delta, neg_delta);  // (kDkv: -delta is in dP already)
+          mul2(y0, y1, pr[i], pr[i + 1]);
           if (!all) {
             // (a selection: what lies behind the sequence may be infinite)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!((vis >> (i + e)) & 1u)) y[e] = 0.f;
+            if (!((vis >> i) & 1u)) y0 = 0.f;
+            if (!((vis >> (i + 1)) & 1u)) y1 = 0.f;
           }
-          w[i / 2] = pack_bf16x2(y[0], y[1]);
-          w[i / 2 + 1] = pack_bf16x2(y[2], y[3]);
+          w[i / 2] = pack_bf16x2(y0, y1);
         }
       }
-      tmem_st16(MODE == kDkv ? dp_col : s_col, w);             // dS over dP (kDkv) or over S (kDq)
+      tmem_st16(MODE == kDkv ? dp_col + 16 : s_col, w);        // dS over the second half of them (kDkv) or over S (kDq)
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&ctl->ds_ready);
-        if (MODE == kDkv) mbar_arrive(&ctl->stat_empty[j & 1]);
-      }
+      if (lane == 0) mbar_arrive(&ctl->ds_ready[j & 1]);
     }
     if (ok && n > 0) ok = wait(&ctl->all_done, 0, kDevWaitPvDone);
     ok = __all_sync(0xffffffffu, ok);
