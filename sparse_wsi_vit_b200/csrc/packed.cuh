@@ -88,6 +88,10 @@ __device__ __forceinline__ void write_staged(uint32_t base, int r0, int r1, int 
     if (chunk * 8 < d) *reinterpret_cast<uint4*>(at(r) + chunk * 8) = lds128(staged_at<D>(base, r, chunk));
 }
 
+// At the head of a rarely taken branch: without it the compiler turns the branch's selections into instructions that every
+// pass executes (half of all, in the loops of the attention kernels).
+#define KEEP_BRANCH() asm volatile("" ::: "memory")
+
 // pairs of fp32 values in one instruction
 __device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c, float d) {
   asm("{\n\t.reg .b64 v, s, e;\n\tmov.b64 v, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\tmov.b64 e, {%5, %6};\n\t"

@@ -298,6 +298,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (live) {
         const int vis = limit - j * kTile;                   // the first `vis` columns are seen
         if (__any_sync(0xffffffffu, vis < kTile)) {
+          KEEP_BRANCH();
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t w = first_bits(vis - c * 32);

@@ -14,12 +14,11 @@
 //   kDq  : lanes = queries; streamed: K (ring A), V (ring B)      S = Q K^T,   dP = dO V^T,   dQ += dS K
 // warp 0: TMA producer; warp 1: issues the products; warp 2: lse and delta of the streamed rows (kDkv); warp 3: zeroes the
 // streamed rows behind the sequence's end (they are summed over, and 0 x NaN would reach the sums); warps 4..19: sixteen
-// warps turn a tile's S and dP into P and dS, (row quarter, 32 of the columns) each.  kDkv writes both over dP once that is in
-// registers, so the next scores are formed while P is computed (P over S: 603 us where this takes {T} at 8192 causal tokens,
-// 16 heads of 128 sharing two key heads).  P and dS go back into TMEM as bf16 pairs over the
-// columns that the warp read, as the A operand of the gradient products (16-bit operands: 2^-9 of each entry, independent).
+// warps turn a tile's S and dP into P and dS, (row quarter, 32 of the columns) each.  P (kDkv) and dS go back into TMEM as bf16
+// pairs over the columns of dP that the warp has read, as the A operand of the gradient products (16-bit operands: each entry is
+// off by at most 2^-8); S's columns are free as soon as it is in registers, so the next tile's products are formed meanwhile.
 // TMEM: kDkv  S [0,128), dP [128,256) (D = 64: two tiles, [128,384)), then dV and dK
-//       kDq   S twice [0,256), dP [256,384), dQ [384,384+D)
+//       kDq   S [0,128), dP twice [128,384), dQ [384,384+D)
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -63,13 +62,12 @@ struct BwdCfg {
   static constexpr int kOffOnes = kOffB + kB * kTileBytes;
   static constexpr int kOffStats = kOffOnes + (MODE == kDkv ? kTile * 128 : 0);
   static constexpr int kOffCtl = kOffStats + (MODE == kDkv ? kTile * 128 : 0);
-  static constexpr int kY = MODE == kDkv && D == 64 ? 2 : 1;            // dP tiles in TMEM
-  static constexpr uint32_t kColDp = MODE == kDkv ? 128 : 256;
-  static constexpr uint32_t kColG = kColDp + kY * 128;
+  static constexpr int kY = MODE == kDkv && D == 128 ? 1 : 2;           // dP tiles in TMEM
+  static constexpr uint32_t kColDp = 128, kColG = kColDp + kY * 128;
 };
 struct BwdCtl {
   uint64_t lane_full, a_full[4], a_empty[4], b_full[4], b_empty[4], tail_a, tail_b;
-  uint64_t s_full[2], s_read, dp_full[2], ds_ready[2], ds_done, all_done, stat_full[2], stat_empty[2], staged;
+  uint64_t s_full, s_read, dp_full[2], ds_ready[2], ds_done, all_done, stat_full[2], stat_empty[2], staged;
   uint32_t tmem_base, abort_flag;
 };
 template <int D, int MODE>
@@ -125,12 +123,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(&ctl->tail_a, 1);
     mbar_init(&ctl->tail_b, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&ctl->s_full[s], 1);
       mbar_init(&ctl->stat_full[s], 1);
       mbar_init(&ctl->stat_empty[s], 1);
       mbar_init(&ctl->dp_full[s], 1);
       mbar_init(&ctl->ds_ready[s], kBwdWarps);
     }
+    mbar_init(&ctl->s_full, 1);
     mbar_init(&ctl->s_read, kBwdWarps);
     mbar_init(&ctl->ds_done, 1);
     mbar_init(&ctl->all_done, 1);
@@ -231,16 +229,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         for (int ks = 0; ks < kTile / 16; ++ks) 
           umma_f16_ts(col, a_col + (ks >> 1) * 32 + (ks & 1) * 8, db + ks * 128, kIdescG, !first || ks > 0);
       };
-      if constexpr (MODE == kDkv) {
+      {
         auto scores = [&](int j) {
           if (!wait(&ctl->a_full[j % NA], (j / NA) & 1, kDevWaitTmaFull) ||
-              !wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitTmaFull) ||
+              (MODE == kDkv && !wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitTmaFull)) ||
               (j > 0 && !wait(&ctl->s_read, (j - 1) & 1, kDevWaitAccEmpty)))
             return false;
           tc_fence_after();
           product(tmem_base, l1, ra + (j % NA) * TB);
-          plus_stat(tmem_base, (j & 1) * 2);
-          umma_commit(&ctl->s_full[0]);
+          if (MODE == kDkv) plus_stat(tmem_base, (j & 1) * 2);
+          umma_commit(&ctl->s_full);
           return true;
         };
         auto inner = [&](int j) {
@@ -251,8 +249,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tc_fence_after();
           const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
           product(col, l2, rb + (j % NB) * TB);
-          plus_stat(col, (j & 1) * 2 + 1);
-          umma_commit(&ctl->stat_empty[j & 1]);
+          if (MODE == kDkv) {
+            plus_stat(col, (j & 1) * 2 + 1);
+            umma_commit(&ctl->stat_empty[j & 1]);
+          } else {
+            umma_commit(&ctl->b_empty[j % NB]);
+          }
           umma_commit(&ctl->dp_full[j & 1]);
           return true;
         };
@@ -263,40 +265,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (!ok) break;
           tc_fence_after();
           const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
-          gradient(tmem_base + kColG, col, rb + (j % NB) * TB, j == 0);
-          umma_commit(&ctl->b_empty[j % NB]);
-          gradient(tmem_base + kColG + D, col + 16, ra + (j % NA) * TB, j == 0);
+          if (MODE == kDkv) {
+            gradient(tmem_base + kColG, col, rb + (j % NB) * TB, j == 0);
+            umma_commit(&ctl->b_empty[j % NB]);
+          }
+          gradient(tmem_base + kColG + (MODE == kDkv ? D : 0), col + 16, ra + (j % NA) * TB, j == 0);
           umma_commit(&ctl->a_empty[j % NA]);
           umma_commit(j + 1 < n ? &ctl->ds_done : &ctl->all_done);
           if (kY == 1 && j + 1 < n) ok = inner(j + 1);
-        }
-      } else {
-        auto scores = [&](int j) {
-          // dS(j-2) lay where S(j) goes
-          if (!wait(&ctl->a_full[j % NA], (j / NA) & 1, kDevWaitTmaFull) ||
-              (j >= 2 && !wait(&ctl->ds_done, j & 1, kDevWaitPvDone)))
-            return false;
-          tc_fence_after();
-          product(tmem_base + (j & 1) * 128, l1, ra + (j % NA) * TB);
-          umma_commit(&ctl->s_full[j & 1]);
-          return true;
-        };
-        if (ok) ok = scores(0);
-        for (int j = 0; ok && j < n; ++j) {
-          // (dP(j-1) has been read: its dS was ready before dQ took it)
-          ok = wait(&ctl->b_full[j % NB], (j / NB) & 1, kDevWaitTmaFull);
-          if (!ok) break;
-          tc_fence_after();
-          product(tmem_base + kColDp, l2, rb + (j % NB) * TB);
-          umma_commit(&ctl->b_empty[j % NB]);
-          umma_commit(&ctl->dp_full[j & 1]);
-          if (j + 1 < n) ok = scores(j + 1);
-          ok = ok && wait(&ctl->ds_ready[j & 1], (j >> 1) & 1, kDevWaitPReady);
-          if (!ok) break;
-          tc_fence_after();
-          gradient(tmem_base + kColG, tmem_base + (j & 1) * 128, ra + (j % NA) * TB, j == 0);
-          umma_commit(&ctl->a_empty[j % NA]);
-          umma_commit(j + 1 < n ? &ctl->ds_done : &ctl->all_done);
         }
       }
     }
@@ -376,7 +352,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       limit = min(u.len, u.off + tk + 1) - u.b0 * kTile;
     }
     for (int j = 0; j < n; ++j) {
-      const uint32_t s_col = tmem_base + lane_off + (MODE == kDq ? (j & 1) * 128 : 0) + c0;
+      const uint32_t s_col = tmem_base + lane_off + c0;
       const uint32_t dp_col = tmem_base + lane_off + kColDp + (j % kY) * 128 + c0;
       // the columns that the row sees: keys before its limit, or queries from `lo` on
       int lo = 0, hi;
@@ -389,7 +365,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       const uint32_t vis = column_bits(lo, hi, c0);
       const bool all = __all_sync(0xffffffffu, vis == 0xffffffffu);
-      ok = wait(MODE == kDq ? &ctl->s_full[j & 1] : &ctl->s_full[0], MODE == kDq ? (j >> 1) & 1 : j & 1, kDevWaitAccFull);
+      ok = wait(&ctl->s_full, j & 1, kDevWaitAccFull);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -398,11 +374,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint32_t s[32];
         tmem_ld32(s_col, s);
         tc_wait_ld();
-        if (MODE == kDkv) {                                    // S(j+1) may go there
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->s_read);
-        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->s_read);              // S(j+1) may go there
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {                      // (kDkv: the scores hold -lse already)
           fma2(pr[i], pr[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), c2, neg_lse, neg_lse);
@@ -410,6 +384,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           pr[i + 1] = ex2_approx(pr[i + 1]);
         }
         if (!all) {
+          KEEP_BRANCH();
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (!((vis >> i) & 1u)) pr[i] = 0.f;
@@ -424,6 +399,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint32_t x[32];
         tmem_ld32(dp_col, x);
         tc_wait_ld();
+        if (!all) {                                            // (what lies behind the sequence may be infinite)
+          KEEP_BRANCH();
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((vis >> i) & 1u)) x[i] = 0u;
+        }
         if (MODE == kDkv) {                                    // P over the first half of the warp's own columns of dP
 #pragma unroll
           for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(pr[2 * i], pr[2 * i + 1]);
@@ -434,15 +415,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           float y0 = __uint_as_float(x[i]), y1 = __uint_as_float(x[i + 1]);
           if (MODE == kDq) add2(y0, y1, neg_delta, neg_delta);  // (kDkv: -delta is in dP already)
           mul2(y0, y1, pr[i], pr[i + 1]);
-          if (!all) {
-            // (a selection: what lies behind the sequence may be infinite)
-            if (!((vis >> i) & 1u)) y0 = 0.f;
-            if (!((vis >> (i + 1)) & 1u)) y1 = 0.f;
-          }
           w[i / 2] = pack_bf16x2(y0, y1);
         }
       }
-      tmem_st16(MODE == kDkv ? dp_col + 16 : s_col, w);        // dS over the second half of them (kDkv) or over S (kDq)
+      tmem_st16(dp_col + 16, w);                               // dS over the second half of them
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
