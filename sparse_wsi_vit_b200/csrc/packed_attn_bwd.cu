@@ -12,8 +12,9 @@
 // One kernel for both sides.  The lane side (128 rows) stays in shared memory, the streamed side passes through two rings:
 //   kDkv : lanes = keys;    streamed: Q (ring A), dO (ring B)     S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
 //   kDq  : lanes = queries; streamed: K (ring A), V (ring B)      S = Q K^T,   dP = dO V^T,   dQ += dS K
-// warp 0: TMA producer; warp 1: issues the products; warp 2: lse and delta of the streamed rows (kDkv); warp 3: zeroes the
-// streamed rows behind the sequence's end (they are summed over, and 0 x NaN would reach the sums); warps 4..19: sixteen
+// warp 0: TMA producer; warp 1: issues S and dP; warp 2: lse and delta of the streamed rows (kDkv); warp 3: issues the
+// gradient products, and zeroes the streamed rows behind the sequence's end (they are summed over, and 0 x NaN would reach
+// the sums); warps 4..19: sixteen
 // warps turn a tile's S and dP into P and dS, (row quarter, 32 of the columns) each.  P (kDkv) and dS go back into TMEM as bf16
 // pairs over the columns of dP that the warp has read, as the A operand of the gradient products (16-bit operands: each entry is
 // off by at most 2^-8); S's columns are free as soon as it is in registers, so the next tile's products are formed meanwhile.
@@ -67,7 +68,7 @@ struct BwdCfg {
 };
 struct BwdCtl {
   uint64_t lane_full, a_full[4], a_empty[4], b_full[4], b_empty[4], tail_a, tail_b;
-  uint64_t s_full, s_read, dp_full[2], ds_ready[2], ds_done, all_done, stat_full[2], stat_empty[2], staged;
+  uint64_t s_full, s_read, dp_full[2], ds_ready[2], ds_done[2], all_done, stat_full[2], stat_empty[2], staged;
   uint32_t tmem_base, abort_flag;
 };
 template <int D, int MODE>
@@ -127,10 +128,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&ctl->stat_empty[s], 1);
       mbar_init(&ctl->dp_full[s], 1);
       mbar_init(&ctl->ds_ready[s], kBwdWarps);
+      mbar_init(&ctl->ds_done[s], 1);
     }
     mbar_init(&ctl->s_full, 1);
     mbar_init(&ctl->s_read, kBwdWarps);
-    mbar_init(&ctl->ds_done, 1);
     mbar_init(&ctl->all_done, 1);
     mbar_init(&ctl->staged, kBwdWarps);
     ctl->abort_flag = 0;
@@ -207,14 +208,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // -------------------------------------------------------------- MMA issuer
+    // ------------------------------------------------- issues S and dP of every tile
     if (lane == 0 && n > 0) {
       const uint32_t l1 = smem_u32(smem), l2 = l1 + TB, ra = l1 + Cfg::kOffA, rb = l1 + Cfg::kOffB;
-      // col += 1 x (row statistic of the streamed side): 16 more channels, see the warp that fills them
-      auto plus_stat = [&](uint32_t col, int channels16) {
-        umma_f16_ss(col, smem_desc_sw128(l1 + Cfg::kOffOnes), smem_desc_sw128(l1 + Cfg::kOffStats) + channels16 * 2, kIdescS, 1);
-      };
-      bool ok = wait(&ctl->lane_full, 0, kDevWaitQ);
       auto product = [&](uint32_t col, uint32_t a, uint32_t b) {          // both operands along the channels
         const uint64_t da = smem_desc_sw128(a), db = smem_desc_sw128(b);
 #pragma unroll
@@ -223,57 +219,34 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           umma_f16_ss(col, da + off, db + off, kIdescS, ks > 0);
         }
       };
-      auto gradient = [&](uint32_t col, uint32_t a_col, uint32_t b, bool first) {   // the 128 streamed rows are summed over
-        const uint64_t db = smem_desc_sw128(b, kTile * 128);
-#pragma unroll
-        for (int ks = 0; ks < kTile / 16; ++ks) 
-          umma_f16_ts(col, a_col + (ks >> 1) * 32 + (ks & 1) * 8, db + ks * 128, kIdescG, !first || ks > 0);
+      // col += 1 x (row statistic of the streamed side): 16 more channels, see the warp that fills them
+      auto plus_stat = [&](uint32_t col, int channels16) {
+        umma_f16_ss(col, smem_desc_sw128(l1 + Cfg::kOffOnes), smem_desc_sw128(l1 + Cfg::kOffStats) + channels16 * 2, kIdescS, 1);
       };
-      {
-        auto scores = [&](int j) {
-          if (!wait(&ctl->a_full[j % NA], (j / NA) & 1, kDevWaitTmaFull) ||
-              (MODE == kDkv && !wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitTmaFull)) ||
-              (j > 0 && !wait(&ctl->s_read, (j - 1) & 1, kDevWaitAccEmpty)))
-            return false;
-          tc_fence_after();
-          product(tmem_base, l1, ra + (j % NA) * TB);
-          if (MODE == kDkv) plus_stat(tmem_base, (j & 1) * 2);
-          umma_commit(&ctl->s_full);
-          return true;
-        };
-        auto inner = [&](int j) {
-          // P and dS of tile j - kY lay where dP(j) goes
-          if (!wait(&ctl->b_full[j % NB], (j / NB) & 1, kDevWaitTmaFull) ||
-              (j >= kY && !wait(&ctl->ds_done, (j - kY) & 1, kDevWaitPvDone)))
-            return false;
-          tc_fence_after();
-          const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
-          product(col, l2, rb + (j % NB) * TB);
-          if (MODE == kDkv) {
-            plus_stat(col, (j & 1) * 2 + 1);
-            umma_commit(&ctl->stat_empty[j & 1]);
-          } else {
-            umma_commit(&ctl->b_empty[j % NB]);
-          }
-          umma_commit(&ctl->dp_full[j & 1]);
-          return true;
-        };
-        ok = ok && scores(0) && inner(0);
-        for (int j = 0; ok && j < n; ++j) {
-          ok = (j + 1 == n || scores(j + 1)) && (j + 1 == n || kY == 1 || inner(j + 1)) &&
-               wait(&ctl->ds_ready[j & 1], (j >> 1) & 1, kDevWaitPReady);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
-          if (MODE == kDkv) {
-            gradient(tmem_base + kColG, col, rb + (j % NB) * TB, j == 0);
-            umma_commit(&ctl->b_empty[j % NB]);
-          }
-          gradient(tmem_base + kColG + (MODE == kDkv ? D : 0), col + 16, ra + (j % NA) * TB, j == 0);
-          umma_commit(&ctl->a_empty[j % NA]);
-          umma_commit(j + 1 < n ? &ctl->ds_done : &ctl->all_done);
-          if (kY == 1 && j + 1 < n) ok = inner(j + 1);
+      bool ok = wait(&ctl->lane_full, 0, kDevWaitQ);
+      for (int j = 0; ok && j < n; ++j) {
+        ok = wait(&ctl->a_full[j % NA], (j / NA) & 1, kDevWaitTmaFull) &&
+             (MODE == kDq || wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitTmaFull)) &&
+             (j == 0 || wait(&ctl->s_read, (j - 1) & 1, kDevWaitAccEmpty));
+        if (!ok) break;
+        tc_fence_after();
+        product(tmem_base, l1, ra + (j % NA) * TB);
+        if (MODE == kDkv) plus_stat(tmem_base, (j & 1) * 2);
+        umma_commit(&ctl->s_full);
+        // P and dS of tile j - kY lay where dP(j) goes
+        ok = wait(&ctl->b_full[j % NB], (j / NB) & 1, kDevWaitTmaFull) &&
+             (j < kY || wait(&ctl->ds_done[(j - kY) & 1], ((j - kY) >> 1) & 1, kDevWaitPvDone));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
+        product(col, l2, rb + (j % NB) * TB);
+        if (MODE == kDkv) {
+          plus_stat(col, (j & 1) * 2 + 1);
+          umma_commit(&ctl->stat_empty[j & 1]);
+        } else {
+          umma_commit(&ctl->b_empty[j % NB]);
         }
+        umma_commit(&ctl->dp_full[j & 1]);
       }
     }
   } else if (warp == 2) {
@@ -317,9 +290,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
     }
   } else {
-    if (tail) {
-      bool ok = wait(&ctl->tail_a, 0, kDevWaitTmaFull) && (MODE == kDq || wait(&ctl->tail_b, 0, kDevWaitTmaFull));
-      if (__all_sync(0xffffffffu, ok)) {
+    // -------------- zeroes the rows behind the sequence's end in the last tile, and issues the gradient products
+    bool ok = n > 0;
+    auto clean = [&]() {
+      bool r = wait(&ctl->tail_a, 0, kDevWaitTmaFull) && (MODE == kDq || wait(&ctl->tail_b, 0, kDevWaitTmaFull));
+      r = __all_sync(0xffffffffu, r);
+      if (r) {
         const int sa = (n - 1) % NA, sb = (n - 1) % NB;
         zero_rows<D>(smem_u32(smem + Cfg::kOffA + sa * TB), last_rows, lane, 32);
         if (MODE == kDkv) zero_rows<D>(smem_u32(smem + Cfg::kOffB + sb * TB), last_rows, lane, 32);
@@ -330,6 +306,35 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (MODE == kDkv) mbar_arrive(&ctl->b_full[sb]);
         }
       }
+      return r;
+    };
+    const uint32_t ra = smem_u32(smem) + Cfg::kOffA, rb = smem_u32(smem) + Cfg::kOffB;
+    auto gradient = [&](uint32_t col, uint32_t a_col, uint32_t b, bool first) {     // the 128 streamed rows are summed over
+      const uint64_t db = smem_desc_sw128(b, kTile * 128);
+#pragma unroll
+      for (int ks = 0; ks < kTile / 16; ++ks)
+        umma_f16_ts(col, a_col + (ks >> 1) * 32 + (ks & 1) * 8, db + ks * 128, kIdescG, !first || ks > 0);
+    };
+    // The last tile lands while tile n - 2 is worked on at the latest: its loads wait for the stages of tiles n - 1 - NA
+    // and n - 1 - NB, which the products of tile n - 2 no longer need.
+    for (int j = 0; ok && j < n; ++j) {
+      if (tail && j == max(n - 2, 0)) ok = clean();
+      if (!ok) break;
+      ok = wait(&ctl->ds_ready[j & 1], (j >> 1) & 1, kDevWaitPReady);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) {
+        tc_fence_after();
+        const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
+        gradient(tmem_base + kColG + (MODE == kDkv ? D : 0), col + 16, ra + (j % NA) * TB, j == 0);   // (dK first: Q's stage
+        umma_commit(&ctl->a_empty[j % NA]);                                                           // is wanted sooner)
+        if (MODE == kDkv) {
+          gradient(tmem_base + kColG, col, rb + (j % NB) * TB, j == 0);
+          umma_commit(&ctl->b_empty[j % NB]);
+        }
+        umma_commit(j + 1 < n ? &ctl->ds_done[j & 1] : &ctl->all_done);
+      }
+      __syncwarp();
     }
   }
   } else {
