@@ -62,7 +62,6 @@ struct FwdCtl {
   uint64_t q_full[2];
   uint64_t full[8], empty[8];
   uint64_t s_full[2], s_read[2], p_full[2][2], pv_done[2];
-  uint64_t exp_done[2][4];                  // a warp's exponentials of a tile are through
   uint64_t tail_full;                       // the last value block of the sequence, before it is cleaned
   uint32_t tmem_base, abort_flag;
 };
@@ -113,7 +112,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       mbar_init(&ctl->p_full[t][0], 4);
       mbar_init(&ctl->p_full[t][1], 4);
       mbar_init(&ctl->pv_done[t], 1);
-      for (int q = 0; q < 4; ++q) mbar_init(&ctl->exp_done[t][q], 1);
     }
     for (int s = 0; s < NST; ++s) {
       mbar_init(&ctl->full[s], 1);
@@ -252,7 +250,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     // ----------------------------------------------------------------- softmax
     reg_inc<kFwdRegsSoftmax>();
     const int t = (warp - 4) >> 2;
-    const int nt = blocks(t), nother = blocks(1 - t);
+    const int nt = blocks(t);
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int rows = tokens(t) * p.group;
@@ -264,7 +262,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const uint32_t s_col = tmem_base + lane_off + (t % Cfg::kSlots) * kTile;
     const uint32_t p_col = tmem_base + lane_off + Cfg::kColP + t * 64;
     const uint32_t o_col = tmem_base + lane_off + Cfg::kColO + t * D;
-    const bool other_live = quarter * 32 < tokens(1 - t) * p.group;
     const float sc = p.scale_log2;
     const float ninf = -__int_as_float(0x7f800000);
     float m_used = ninf;
@@ -336,13 +333,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         // A row that sees no key has probabilities of zero; one whose scores are all -inf comes out NaN (-inf + inf).
         const float neg_m = limit > 0 ? -m_used : 0.f;
-        // The two tiles take turns at the exponentials, A(0), B(0), A(1), ...: in step with each other they would both
-        // wait for the tensor cores and then share the exponential unit.  (The warps of a quarter share a scheduler.)
-        const int turn = j - 1 + t;                          // the other tile's block whose turn was before this one's
-        if (other_live && turn >= 0 && turn < nother && !mbar_wait_bounded(&ctl->exp_done[1 - t][quarter], turn & 1, abort_flag)) {
-          record_status(p.status, kDevWaitPReady);
-          ok = false;
-        }
         float l0 = 0.f, l1 = 0.f;
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
@@ -357,7 +347,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             packed[i >> 1] = pack_bf16x2(x0, x1);
           }
           tmem_st8(p_col + v * 8, packed);
-          if (v == 7 && lane == 0) mbar_arrive(&ctl->exp_done[t][quarter]);
           if (v == 4 || v == 7) {          // the first half is handed over under the next 16 columns' exponentials
             tc_wait_st();
             tc_fence_before();
