@@ -427,39 +427,59 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   }
 }
 
-// Joins the sums of divided units, one warp per row: o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, the parts in order.
+// Joins the sums of divided units, one warp per row: o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.  The parts'
+// (m, l) lie in the lanes, 32 parts at a time, their rows are added up in the parts' order with eight loads in flight.
 template <int D>
 __global__ void __launch_bounds__(256) packed_attn_join_kernel(const PackedJoin* joins, const PackedFwdParams p) {
+  constexpr int V = D / 32;                                    // channels a lane
   const PackedJoin jn = joins[blockIdx.x];
   const int kvh = blockIdx.y, lane = threadIdx.x & 31;
   const float ninf = -__int_as_float(0x7f800000);
-  const int rows = jn.n * p.group;                           // rows of both tiles, tile B's from row tok * group on
+  const int rows = jn.n * p.group;                             // rows of both tiles, tile B's from row tok * group on
+  const int64_t step = static_cast<int64_t>(p.Hkv) * (2 * kTile);
   for (int i = blockIdx.z * 8 + (threadIdx.x >> 5); i < rows; i += gridDim.z * 8) {
     const int per = p.tok * p.group;
-    const int r = (i / per) * kTile + i % per;
-    const int64_t r0 = (static_cast<int64_t>(jn.slot) * p.Hkv + kvh) * (2 * kTile) + r;
-    const int64_t step = static_cast<int64_t>(p.Hkv) * (2 * kTile);
-    float m = ninf, l = 0.f;
-    for (int k = 0; k < jn.parts; ++k) m = fmaxf(m, p.part_ml[r0 + k * step].x);
-    float acc[D / 32];
+    const int64_t r0 = (static_cast<int64_t>(jn.slot) * p.Hkv + kvh) * (2 * kTile) + (i / per) * kTile + i % per;
+    float m = ninf;
+    for (int k = lane; k < jn.parts; k += 32) m = fmaxf(m, p.part_ml[r0 + k * step].x);
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
-    for (int k = 0; k < jn.parts; ++k) {
-      const float2 ml = p.part_ml[r0 + k * step];
-      const float f = ml.x == m ? 1.f : ex2_approx(ml.x - m);
-      l = fmaf(ml.y, f, l);
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    float l = 0.f, acc[V];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(p.part_o[(r0 + k * step) * D + c * 32 + lane], f, acc[c]);
+    for (int c = 0; c < V; ++c) acc[c] = 0.f;
+    for (int k0 = 0; k0 < jn.parts; k0 += 32) {
+      float f = 0.f;
+      if (k0 + lane < jn.parts) {
+        const float2 ml = p.part_ml[r0 + (k0 + lane) * step];
+        f = ml.x == m ? 1.f : ex2_approx(ml.x - m);
+        l = fmaf(ml.y, f, l);
+      }
+      const int here = min(32, jn.parts - k0);
+#pragma unroll 8
+      for (int k = 0; k < here; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        const float* src = p.part_o + (r0 + (k0 + k) * step) * D + lane * V;
+        float v[V];
+        if constexpr (V == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+        else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+        for (int c = 0; c < V; ++c) acc[c] = fmaf(v[c], fk, acc[c]);
+      }
     }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     const int head = kvh * p.group + i % p.group;
     const int64_t token = jn.t0 + i / p.group;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (lane == 0 && p.lse != nullptr)
       p.lse[static_cast<int64_t>(head) * p.Tq + token] = l == 0.f ? ninf : (m + log2f(l)) * 0.6931471805599453f;
-    __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.o) + token * p.os_t + head * p.os_h;
+    if (lane * V >= p.d) continue;                             // (d is a multiple of 8)
+    uint32_t w[V / 2];
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-      if (c * 32 + lane < p.d) orow[c * 32 + lane] = __float2bfloat16_rn(acc[c] * inv);
+    for (int c = 0; c < V / 2; ++c) w[c] = pack_bf16x2(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+    uint16_t* out = static_cast<uint16_t*>(p.o) + token * p.os_t + head * p.os_h + lane * V;
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(out) = w[0];
   }
 }
 

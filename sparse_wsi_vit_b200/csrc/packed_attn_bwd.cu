@@ -540,17 +540,31 @@ __global__ void __launch_bounds__(256) packed_attn_bwd_join_kernel(const PackedJ
     const float* part = p.part + ((static_cast<int64_t>(jn.slot) * p.Hkv + kvh) * kTile + r) * kWidth;
     const int64_t token = jn.t0 + (MODE == kDkv ? r : r / p.group);
     const int head = MODE == kDkv ? kvh : kvh * p.group + r % p.group;
+    constexpr int V = D / 32;                                  // channels a lane of each gradient
 #pragma unroll
-    for (int c = 0; c < kWidth / 32; ++c) {
-      const int ch = c * 32 + lane;
-      float a = 0.f;
-      for (int k = 0; k < jn.parts; ++k) a += part[k * step + ch];
-      const bool is_dv = MODE == kDkv && ch < D;
-      const int cd = MODE == kDkv ? ch % D : ch;
-      if (cd >= p.d) continue;
-      __nv_bfloat16* out = is_dv ? static_cast<__nv_bfloat16*>(p.g2) + token * p.g2_t + head * p.g2_h
-                                 : static_cast<__nv_bfloat16*>(p.g1) + token * p.g1_t + head * p.g1_h;
-      out[cd] = __float2bfloat16_rn(is_dv ? a : a * p.scale);
+    for (int g = 0; g < kWidth / D; ++g) {
+      float a[V];
+#pragma unroll
+      for (int c = 0; c < V; ++c) a[c] = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < jn.parts; ++k) {
+        const float* src = part + k * step + g * D + lane * V;
+        float v[V];
+        if constexpr (V == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+        else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+        for (int c = 0; c < V; ++c) a[c] += v[c];
+      }
+      if (lane * V >= p.d) continue;                           // (d is a multiple of 8)
+      const bool is_dv = MODE == kDkv && g == 0;
+      const float f = is_dv ? 1.f : p.scale;
+      uint16_t* out = (is_dv ? static_cast<uint16_t*>(p.g2) + token * p.g2_t + head * p.g2_h
+                             : static_cast<uint16_t*>(p.g1) + token * p.g1_t + head * p.g1_h) + lane * V;
+      uint32_t w[V / 2];
+#pragma unroll
+      for (int c = 0; c < V / 2; ++c) w[c] = pack_bf16x2(a[2 * c] * f, a[2 * c + 1] * f);
+      if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(out) = w[0];
     }
   }
 }
