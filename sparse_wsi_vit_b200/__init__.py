@@ -11,6 +11,7 @@ from .modules import DeepSeekSparseAttention, DSAViTBlock, DSAViTSlideEncoder, I
 from .static_modules import (BlockSparse2DViTBlock, BlockSparse2DViTSlideEncoder, BlockSparseAttention2D,
                              StaticSparseAttention, StaticSparseViTBlock, StaticSparseViTSlideEncoder)
 from .packed import PackedPlan, RopeAxes, layer_norm, packed_attention, rope_axes
+from .packed_modules import PackedAttention, PackedBags, PackedViTBlock, PackedViTSlideEncoder
 from . import ingest, patterns, training
 
 __all__ = [
@@ -18,5 +19,6 @@ __all__ = [
     "dsa_attention_masked", "dsa_indexer_topk", "dsa_sparse_attention", "DeepSeekSparseAttention",
     "DSAViTBlock", "DSAViTSlideEncoder", "IndexerProjection", "block_sparse_attention", "rope2d", "patterns", "ingest", "training",
     "PackedPlan", "RopeAxes", "layer_norm", "packed_attention", "rope_axes",
+    "PackedAttention", "PackedBags", "PackedViTBlock", "PackedViTSlideEncoder",
     "BlockSparseAttention2D", "BlockSparse2DViTBlock", "BlockSparse2DViTSlideEncoder", "StaticSparseAttention", "StaticSparseViTBlock", "StaticSparseViTSlideEncoder",
 ]

@@ -1,6 +1,8 @@
 // Work tables of the packed attention kernels: built on the host from the sequences' lengths, read by the kernels on
 // the device.  One int32 array holds all of them; its first 32 words say where each one lies.
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 
 namespace swv {
@@ -110,12 +112,20 @@ __device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {
       : "f"(a), "f"(b));
 }
 
-// Whether a kernel is launched with the registers that its warpgroups share out (an increase beyond them would wait for
-// ever): asked once per kernel.
+// Prepares a kernel on the current device, once: its shared memory, and whether it is launched with the registers that
+// its warpgroups share out (an increase beyond them would wait for ever).
 template <typename K>
-bool registers_suffice(K kernel, int threads, int shared_out) {
+int prepare_kernel(K kernel, std::atomic<uint64_t>& done, int threads, int shared_out, size_t smem) {
+  int dev = 0;
+  SWV_CUDA_OK(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return SWV_OK;
   cudaFuncAttributes a;
-  return cudaFuncGetAttributes(&a, kernel) == cudaSuccess && a.numRegs * threads >= shared_out;
+  SWV_CUDA_OK(cudaFuncGetAttributes(&a, kernel));
+  if (a.numRegs * threads < shared_out) return SWV_ERR_CUDA;
+  SWV_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return SWV_OK;
 }
 
 }  // namespace swv

@@ -486,10 +486,9 @@ __global__ void __launch_bounds__(256) packed_attn_join_kernel(const PackedJoin*
 template <int D>
 int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PackedFwdParams& p,
                const PackedHeader& h, const int32_t* plan, cudaStream_t st) {
-  static const bool fits = registers_suffice(packed_attn_fwd_kernel<D>, kFwdThreads, kFwdRegs);
-  if (!fits) return SWV_ERR_CUDA;
-  SWV_CUDA_OK(cudaFuncSetAttribute(packed_attn_fwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(fwd_smem<D>())));
+  static std::atomic<uint64_t> prepared{0};
+  const int rc = prepare_kernel(packed_attn_fwd_kernel<D>, prepared, kFwdThreads, kFwdRegs, fwd_smem<D>());
+  if (rc != SWV_OK) return rc;
   packed_attn_fwd_kernel<D><<<static_cast<unsigned>(p.n_units) * p.Hkv, kFwdThreads, fwd_smem<D>(), st>>>(tq, tk, tv, p);
   SWV_CUDA_OK(cudaGetLastError());
   if (h.n_fwd_join > 0) {

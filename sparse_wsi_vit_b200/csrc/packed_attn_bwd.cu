@@ -573,10 +573,9 @@ template <int D, int MODE>
 int launch_bwd(const CUtensorMap& l1, const CUtensorMap& l2, const CUtensorMap& a, const CUtensorMap& b,
                const PackedBwdParams& p, const PackedJoin* joins, int n_join, cudaStream_t st) {
   if (p.n_units == 0) return SWV_OK;
-  static const bool fits = registers_suffice(packed_attn_bwd_kernel<D, MODE>, kBwdThreads, kBwdRegs);
-  if (!fits) return SWV_ERR_CUDA;
-  SWV_CUDA_OK(cudaFuncSetAttribute(packed_attn_bwd_kernel<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(bwd_smem<D, MODE>())));
+  static std::atomic<uint64_t> prepared{0};
+  const int rc = prepare_kernel(packed_attn_bwd_kernel<D, MODE>, prepared, kBwdThreads, kBwdRegs, bwd_smem<D, MODE>());
+  if (rc != SWV_OK) return rc;
   packed_attn_bwd_kernel<D, MODE>
       <<<static_cast<unsigned>(p.n_units) * p.Hkv, kBwdThreads, bwd_smem<D, MODE>(), st>>>(l1, l2, a, b, p);
   SWV_CUDA_OK(cudaGetLastError());

@@ -13,6 +13,7 @@ calls that the kernels do not serve.  The reference's dense ViT-5 has the same p
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -72,15 +73,22 @@ def _norm_fwd(x, weight, bias, eps, out_dtype, want_stats):
     E, dev = x.shape[-1], x.device
     x2 = _rows2d(x)
     N = x2.shape[0]
-    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    y = x.new_empty(x.shape, dtype=out_dtype)
     stats = mean = rstd = None
     if want_stats:
-        stats = torch.empty(2 * N, dtype=torch.float32, device=dev)      # mean, rstd
+        stats = x.new_empty(2 * N, dtype=torch.float32)      # mean, rstd
         mean = stats.data_ptr()
         rstd = mean + 4 * N
     _call(lib.swv_layer_norm_fwd, "swv_layer_norm_fwd", dev, x2.data_ptr(), x2.stride(0), _DTYPES[x.dtype], _ptr(weight),
           _code(weight), _ptr(bias), _code(bias), y.data_ptr(), E, _DTYPES[out_dtype], mean, rstd, N, E, eps)
     return y, stats
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_bwd_bytes(N, E):
+    n = ctypes.c_size_t()
+    check(lib.swv_layer_norm_bwd_bytes(N, E, ctypes.byref(n)), "swv_layer_norm_bwd_bytes")
+    return n.value
 
 
 class LayerNormFunction(torch.autograd.Function):
@@ -100,18 +108,18 @@ class LayerNormFunction(torch.autograd.Function):
         E, dev = x.shape[-1], x.device
         x2, dy2 = _rows2d(x), _rows2d(dy)
         N = x2.shape[0]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dx = x.new_empty(x.shape)
         _, want_w, want_b, _, _ = ctx.needs_input_grad
-        dw = torch.empty(E, dtype=weight.dtype, device=dev) if want_w else None
-        db = torch.empty(E, dtype=ctx.bias_dtype, device=dev) if want_b else None
-        ws, nws = None, ctypes.c_size_t()
+        dw = weight.new_empty(E) if want_w else None
+        db = x.new_empty(E, dtype=ctx.bias_dtype) if want_b else None
+        ws, nws = None, 0
         if want_w or want_b:
-            check(lib.swv_layer_norm_bwd_bytes(N, E, ctypes.byref(nws)), "swv_layer_norm_bwd_bytes")
-            ws = torch.empty(nws.value, dtype=torch.uint8, device=dev)
+            nws = _norm_bwd_bytes(N, E)
+            ws = x.new_empty(nws, dtype=torch.uint8)
         mean = stats.data_ptr()
         _call(lib.swv_layer_norm_bwd, "swv_layer_norm_bwd", dev, dy2.data_ptr(), dy2.stride(0), _DTYPES[dy.dtype],
               x2.data_ptr(), x2.stride(0), _DTYPES[x.dtype], _ptr(weight), _code(weight), mean, mean + 4 * N, dx.data_ptr(), E,
-              _ptr(dw), _code(dw), _ptr(db), _code(db), N, E, _ptr(ws), nws.value)
+              _ptr(dw), _code(dw), _ptr(db), _code(db), N, E, _ptr(ws), nws)
         return dx, dw, db, None, None
 
 
@@ -184,7 +192,7 @@ def _rope_apply(x, positions, rope, inverse, out=None):
     T, H, hd = x.shape
     if x.stride(2) != 1:
         x = x.contiguous()
-    y = torch.empty((T, H, hd), dtype=x.dtype, device=x.device) if out is None else out
+    y = x.new_empty((T, H, hd)) if out is None else out
     _call(lib.swv_rope_axes_apply, "swv_rope_axes_apply", x.device, x.data_ptr(), _I3(*x.stride()), y.data_ptr(),
           _I3(*y.stride()), _DTYPES[x.dtype], positions.data_ptr(), _POS_CODES[positions.dtype], positions.stride(0),
           *rope._call, inverse, T, H, hd)
@@ -267,12 +275,16 @@ class PackedPlan:
         self._call = (self._host.ctypes.data, self._table.data_ptr())
         self._bytes = {}
 
-    def _workspace_bytes(self, D):
-        if D not in self._bytes:
+    def _workspace_bytes(self, D, Tq=None):
+        """Forward (Tq None) or backward workspace for head dimension D and buffers of Tq query rows."""
+        if (D, Tq) not in self._bytes:
             n = ctypes.c_size_t()
-            check(lib.swv_packed_attn_bytes(self._host.ctypes.data, D, ctypes.byref(n)), "swv_packed_attn_bytes")
-            self._bytes[D] = n.value
-        return self._bytes[D]
+            if Tq is None:
+                check(lib.swv_packed_attn_bytes(self._call[0], D, ctypes.byref(n)), "swv_packed_attn_bytes")
+            else:
+                check(lib.swv_packed_attn_bwd_bytes(self._call[0], Tq, D, ctypes.byref(n)), "swv_packed_attn_bwd_bytes")
+            self._bytes[D, Tq] = n.value
+        return self._bytes[D, Tq]
 
 
 def _rows_ok(t):
@@ -312,16 +324,16 @@ def _attn_fwd(q, k, v, plan, scale, want_lse, out=None):
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     o = out
     if o is None:
-        o = torch.empty((Tq, H, D), dtype=torch.bfloat16, device=dev)
+        o = q.new_empty((Tq, H, D))
         if plan.q_tokens < Tq:
             o[plan.q_tokens:].zero_()                     # rows behind the last sequence
     lse = None
     if want_lse:
-        lse = torch.empty((H, Tq), dtype=torch.float32, device=dev)
+        lse = q.new_empty((H, Tq), dtype=torch.float32)
         if plan.q_tokens < Tq:
             lse[:, plan.q_tokens:].fill_(-float("inf"))
     nws = plan._workspace_bytes(D)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
     _call(lib.swv_packed_attn_fwd, "swv_packed_attn_fwd", dev, q.data_ptr(), _I3(*q.stride()), k.data_ptr(),
           _I3(*k.stride()), v.data_ptr(), _I3(*v.stride()), o.data_ptr(), _I3(*o.stride()), _ptr(lse), *plan._call, Tq,
           k.shape[0], D, scale, _ptr(ws), nws, status_word(dev).data_ptr())
@@ -347,20 +359,19 @@ class PackedAttentionFunction(torch.autograd.Function):
         plan, dev, D = ctx.plan, q.device, q.shape[2]
         q, k, v, d_out = _aligned(q), _aligned(k), _aligned(v), _aligned(d_out)
         Tq, Tk = q.shape[0], k.shape[0]
-        dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         if plan.q_tokens < Tq:                            # rows behind the last sequence
             dq[plan.q_tokens:].zero_()
         if plan.k_tokens < Tk:
             dk[plan.k_tokens:].zero_()
             dv[plan.k_tokens:].zero_()
-        n = ctypes.c_size_t()
-        check(lib.swv_packed_attn_bwd_bytes(plan._call[0], Tq, D, ctypes.byref(n)), "swv_packed_attn_bwd_bytes")
-        ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        nws = plan._workspace_bytes(D, Tq)
+        ws = q.new_empty(nws, dtype=torch.uint8)
         dqs, dks = _I3(*dq.stride()), _I3(*dk.stride())
         _call(lib.swv_packed_attn_bwd, "swv_packed_attn_bwd", dev, d_out.data_ptr(), _I3(*d_out.stride()), q.data_ptr(),
               _I3(*q.stride()), k.data_ptr(), _I3(*k.stride()), v.data_ptr(), _I3(*v.stride()), o.data_ptr(), dqs,
               lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dks, *plan._call, Tq, Tk, D, ctx.scale,
-              ws.data_ptr(), n.value, status_word(dev).data_ptr())
+              ws.data_ptr(), nws, status_word(dev).data_ptr())
         return dq, dk, dv, None, None
 
 

@@ -17,9 +17,12 @@ import torch.nn.functional as F
 def slide_step(network, batch, multiclass: bool = True, use_bce_loss: bool = False):
     """Forward + loss of one batch dict {"input", "coords", "label"[, "class_weight"]} exactly as the
     reference's ``_step`` computes it (wsi_attn_wrapper.py:75-110).  ``input`` may be a (B, N, F) tensor
-    or, for a ragged batch (``ingest.ragged_collate``), a list of (N_i, F) tensors.  Returns (loss, preds, logits)."""
+    or, for a ragged batch (``ingest.ragged_collate``), a list of (N_i, F) tensors (one pass for an encoder that packs
+    them, else slide by slide).  Returns (loss, preds, logits)."""
     inputs, coords, labels = batch["input"], batch.get("coords"), batch["label"]
-    if isinstance(inputs, (list, tuple)):
+    if isinstance(inputs, (list, tuple)) and getattr(network, "packs_bags", False):
+        logits = network(list(inputs), coords)["logits"]              # one packed pass over all slides
+    elif isinstance(inputs, (list, tuple)):
         logits = torch.cat([network(x, None if coords is None else coords[i])["logits"] for i, x in enumerate(inputs)])
     else:
         logits = network(inputs, coords)["logits"]
