@@ -53,7 +53,11 @@ __device__ __forceinline__ PackedUnit packed_unit(const PackedUnit* units, int n
   const int r = blockIdx.x - g * n_units * at_once;
   const int here = min(at_once, heads - g * at_once);
   head = g * at_once + r % here;
-  return units[r / here];
+  union { int4 v[2]; PackedUnit u; } x;
+  const int4* src = reinterpret_cast<const int4*>(units + r / here);
+  x.v[0] = __ldg(src);
+  x.v[1] = __ldg(src + 1);
+  return x.u;
 }
 // Heads whose two streamed tensors (`rows` rows of the longest sequence) fill half of the L2.
 inline int packed_heads_at_once(int heads, int64_t rows, int D) {
@@ -69,16 +73,16 @@ template <int D>
 __device__ __forceinline__ uint32_t staged_at(uint32_t base, int row, int chunk) {
   return base + row * (D * 2) + ((chunk ^ (row & 7)) << 4);
 }
-// 16 fp32 values of a row, from column 16 * c on, times f, as bf16
-template <int D>
-__device__ __forceinline__ void stage16(uint32_t base, int row, int c, const uint32_t (&o)[16], float f) {
+// N (16 or 32) fp32 values of a row, from column N * c on, times f, as bf16
+template <int D, int N>
+__device__ __forceinline__ void stage_columns(uint32_t base, int row, int c, const uint32_t* o, float f) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < N / 8; ++i) {
     uint32_t w[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       w[q] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * q]) * f, __uint_as_float(o[8 * i + 2 * q + 1]) * f);
-    sts128(staged_at<D>(base, row, 2 * c + i), w[0], w[1], w[2], w[3]);
+    sts128(staged_at<D>(base, row, N / 8 * c + i), w[0], w[1], w[2], w[3]);
   }
 }
 // Writes rows r0 .. r1 - 1 of the staged tile (one warp; `at(row)` is where a row goes), d <= D channels.
@@ -86,6 +90,7 @@ template <int D, typename At>
 __device__ __forceinline__ void write_staged(uint32_t base, int r0, int r1, int d, At at) {
   constexpr int kLanes = D / 8;                                // lanes a row
   const int lane = threadIdx.x & 31, chunk = lane % kLanes;
+#pragma unroll 4
   for (int r = r0 + lane / kLanes; r < r1; r += 32 / kLanes)
     if (chunk * 8 < d) *reinterpret_cast<uint4*>(at(r) + chunk * 8) = lds128(staged_at<D>(base, r, chunk));
 }
@@ -93,6 +98,11 @@ __device__ __forceinline__ void write_staged(uint32_t base, int r0, int r1, int 
 // At the head of a rarely taken branch: without it the compiler turns the branch's selections into instructions that every
 // pass executes (half of all, in the loops of the attention kernels).
 #define KEEP_BRANCH() asm volatile("" ::: "memory")
+
+// Row r < 128 of a tile as (token, head of the group): r / group by a multiplication (inverse = ceil(2^16 / group): the error
+// r * (inverse * group - 2^16) < 128 * 128 never reaches the next quotient).
+__device__ __forceinline__ int row_token(int r, int inverse) { return (r * inverse) >> 16; }
+inline int group_inverse(int group) { return (65536 + group - 1) / group; }
 
 // pairs of fp32 values in one instruction
 __device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c, float d) {

@@ -31,7 +31,7 @@ namespace {
 
 struct PackedFwdParams {
   const PackedUnit* units;
-  int n_units, group, tok;      // tok = 128 / group query tokens a tile
+  int n_units, group, group_inv, tok;      // tok = 128 / group query tokens a tile
   int Tq, d;                    // d <= D channels
   void* o;                      // bf16
   int64_t os_t, os_h;
@@ -91,19 +91,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   FwdCtl* ctl = reinterpret_cast<FwdCtl*>(smem + Cfg::kOffCtl);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 0) {                            // (fetched while the barriers are made)
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
   int kvh;
   const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
-  const int n = u.b1 - u.b0;
-  // tokens and key blocks of tile t: its last token sees the fewest keys of no later tile
-  auto tokens = [&](int t) { return min(p.tok, u.n - t * p.tok); };
-  auto blocks = [&](int t) {
-    const int tk = tokens(t);
-    if (tk <= 0) return 0;
-    const int sees = max(0, min(u.len, u.off + t * p.tok + tk));
-    return min(n, max(0, (sees + kTile - 1) / kTile - u.b0));
-  };
-  const bool tail = n > 0 && u.b1 * kTile > u.len;   // the last block holds rows behind the sequence
-
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&ctl->q_full[t], 1);
@@ -125,6 +119,17 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
   }
+  const int n = u.b1 - u.b0;
+  // tokens and key blocks of tile t: its last token sees the fewest keys of no later tile
+  auto tokens = [&](int t) { return min(p.tok, u.n - t * p.tok); };
+  auto blocks = [&](int t) {
+    const int tk = tokens(t);
+    if (tk <= 0) return 0;
+    const int sees = max(0, min(u.len, u.off + t * p.tok + tk));
+    return min(n, max(0, (sees + kTile - 1) / kTile - u.b0));
+  };
+  const bool tail = n > 0 && u.b1 * kTile > u.len;   // the last block holds rows behind the sequence
+
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -136,9 +141,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
-      tma_prefetch_desc(&tm_q);
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
       for (int t = 0; t < 2; ++t) {
         if (blocks(t) == 0) continue;                        // (its rows, zeros, may be staged there at once)
         mbar_expect_tx(&ctl->q_full[t], p.tok * p.group * D * 2);
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const int rows = tokens(t) * p.group;
     const bool live = quarter * 32 < rows;
     const bool row_ok = row < rows;
-    const int tk = row / p.group;                            // token of the tile
+    const int tk = row_token(row, p.group_inv);                            // token of the tile
     const int limit = row_ok ? min(u.len, u.off + t * p.tok + tk + 1) - u.b0 * kTile : 0;   // keys it sees from block b0 on
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_col = tmem_base + lane_off + (t % Cfg::kSlots) * kTile;
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
     if (ok && live) {
-      const int head = kvh * p.group + row % p.group;
+      const int head = kvh * p.group + row - tk * p.group;
       const int64_t token = u.t0 + t * p.tok + tk;
       if (u.slot >= 0) {
         const int64_t r = (static_cast<int64_t>(u.slot) * p.Hkv + kvh) * (2 * kTile) + t * kTile + row;
@@ -398,22 +400,25 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         // (the tile's Q is no longer needed: its last scores are done)
         const uint32_t stage = smem_u32(smem + t * Cfg::kTileBytes);
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t o[16];
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
           if (nt > 0) {
-            tmem_ld16(o_col + c * 16, o);
+            tmem_ld32(o_col + c * 32, o);
             tc_wait_ld();
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = 0u;
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
           }
-          stage16<D>(stage, row, c, o, inv);
+          stage_columns<D, 32>(stage, row, c, o, inv);
         }
         __syncwarp();
         uint16_t* out = static_cast<uint16_t*>(p.o) + static_cast<int64_t>(u.t0 + t * p.tok) * p.os_t +
                         static_cast<int64_t>(kvh) * p.group * p.os_h;
         write_staged<D>(stage, quarter * 32, min(rows, quarter * 32 + 32), p.d,
-                        [&](int r) { return out + (r / p.group) * p.os_t + (r % p.group) * p.os_h; });
+                        [&](int r) {
+                          const int w = row_token(r, p.group_inv);
+                          return out + w * p.os_t + (r - w * p.group) * p.os_h;
+                        });
       }
     }
   }
@@ -581,6 +586,7 @@ int packed_attn_fwd_impl(const void* q, const int64_t* qs, const void* k, const 
   }
   PackedFwdParams p{};
   p.group = h.H / h.Hkv;
+  p.group_inv = group_inverse(p.group);
   p.tok = kTile / p.group;
   p.units = reinterpret_cast<const PackedUnit*>(plan + h.fwd_off);
   p.n_units = h.n_fwd;

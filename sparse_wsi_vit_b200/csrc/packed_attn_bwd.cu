@@ -43,7 +43,7 @@ constexpr int kBwdRegs = 128 * kBwdRegsControl + 32 * kBwdWarps * kBwdRegsTerms;
 
 struct PackedBwdParams {
   const PackedUnit* units;
-  int n_units, group, tok, Tq, d, Hkv, heads_at_once;
+  int n_units, group, group_inv, tok, Tq, d, Hkv, heads_at_once;
   const float2* stats;          // [Hkv][Tq][group] {-lse in powers of two, -delta}; -inf where a row sees no key
   void *g1, *g2;                // kDkv: dK, dV; kDq: dQ
   int64_t g1_t, g1_h, g2_t, g2_h;
@@ -105,14 +105,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   BwdCtl* ctl = reinterpret_cast<BwdCtl*>(smem + Cfg::kOffCtl);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 0) {                            // (fetched while the barriers are made)
+    tma_prefetch_desc(&tm_l1);
+    tma_prefetch_desc(&tm_l2);
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_b);
+  }
   int kvh;
   const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
-  const int n = u.b1 - u.b0;
-  const int per = MODE == kDkv ? p.tok * p.group : kTile;      // streamed rows a tile
-  const int step = MODE == kDkv ? p.tok : kTile;               // streamed tokens a tile
-  const int last_rows = min(step, u.len - (u.b1 - 1) * step) * (MODE == kDkv ? p.group : 1);
-  const bool tail = n > 0 && last_rows < per;                  // the last tile holds rows behind the sequence
-
   if (threadIdx.x == 0) {
     mbar_init(&ctl->lane_full, 1);
     for (int s = 0; s < 4; ++s) {
@@ -141,6 +141,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
   }
+  const int n = u.b1 - u.b0;
+  const int per = MODE == kDkv ? p.tok * p.group : kTile;      // streamed rows a tile
+  const int step = MODE == kDkv ? p.tok : kTile;               // streamed tokens a tile
+  const int last_rows = min(step, u.len - (u.b1 - 1) * step) * (MODE == kDkv ? p.group : 1);
+  const bool tail = n > 0 && last_rows < per;                  // the last tile holds rows behind the sequence
+
   if (MODE == kDkv) {
     // rows that no load fills: they are summed over as zeros
     if (per < kTile)
@@ -169,10 +175,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
-      tma_prefetch_desc(&tm_l1);
-      tma_prefetch_desc(&tm_l2);
-      tma_prefetch_desc(&tm_a);
-      tma_prefetch_desc(&tm_b);
       mbar_expect_tx(&ctl->lane_full, 2 * (MODE == kDkv ? TB : p.tok * p.group * D * 2));
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     int limit = 0;                                             // kDq: keys the row sees from block b0 on
     const int rows = MODE == kDkv ? u.n : u.n * p.group;
     const bool row_ok = row < rows;
-    const int tk = MODE == kDkv ? row : row / p.group;         // token of the lane side
+    const int tk = MODE == kDkv ? row : row_token(row, p.group_inv);         // token of the lane side
     if (MODE == kDq && row_ok) {
       const float2 f = __ldg(p.stats + (static_cast<int64_t>(kvh) * p.Tq + u.t0) * p.group + row);
       neg_lse = f.x;
@@ -444,22 +446,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (ok) {
       const float f = is_dv ? 1.f : p.scale;
       float* part = p.part + ((static_cast<int64_t>(divided ? u.slot : 0) * p.Hkv + kvh) * kTile + row) * kWidth + grp * kCols;
+      constexpr int kStep = kCols < 32 ? kCols : 32;           // (kDq at D = 64: 16 columns a warp)
 #pragma unroll 1
-      for (int c = 0; c < kCols / 16; ++c) {
-        uint32_t o[16];
+      for (int c = 0; c < kCols / kStep; ++c) {
+        uint32_t o[32];
         if (n > 0) {
-          tmem_ld16(col + c * 16, o);
+          if constexpr (kStep == 32) tmem_ld32(col + c * 32, o);
+          else tmem_ld16(col, *reinterpret_cast<uint32_t(*)[16]>(o));
           tc_wait_ld();
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = 0u;
+          for (int i = 0; i < kStep; ++i) o[i] = 0u;
         }
         if (!divided) {
-          stage16<D>(stage, row, ch0 / 16 + c, o, f);
+          stage_columns<D, kStep>(stage, row, ch0 / kStep + c, o, f);
         } else if (row_ok) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<uint4*>(part + c * 16 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < kStep; i += 4)
+            *reinterpret_cast<uint4*>(part + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
     }
@@ -479,7 +483,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint16_t* dq = static_cast<uint16_t*>(p.g1) + static_cast<int64_t>(u.t0) * p.g1_t +
                        static_cast<int64_t>(kvh) * p.group * p.g1_h;
         write_staged<D>(smem_u32(smem), r0, r1, p.d,
-                        [&](int r) { return dq + (r / p.group) * p.g1_t + (r % p.group) * p.g1_h; });
+                        [&](int r) {
+                          const int w = row_token(r, p.group_inv);
+                          return dq + w * p.g1_t + (r - w * p.group) * p.g1_h;
+                        });
       }
     }
   }
@@ -644,6 +651,7 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
 
   PackedBwdParams p{};
   p.group = h.H / h.Hkv;
+  p.group_inv = group_inverse(p.group);
   p.tok = kTile / p.group;
   p.Tq = static_cast<int>(Tq); p.d = D; p.Hkv = h.Hkv;
   p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
