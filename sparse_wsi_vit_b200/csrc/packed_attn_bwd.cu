@@ -18,8 +18,6 @@
 // warps turn a tile's S and dP into P and dS, (row quarter, 32 of the columns) each.  P (kDkv) and dS go back into TMEM as bf16
 // pairs over the columns of dP that the warp has read, as the A operand of the gradient products (16-bit operands: each entry is
 // off by at most 2^-8); S's columns are free as soon as it is in registers, so the next tile's products are formed meanwhile.
-// TMEM: kDkv  S [0,128), dP [128,256) (D = 64: two tiles, [128,384)), then dV and dK
-//       kDq   S [0,128), dP twice [128,384), dQ [384,384+D)
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -63,8 +61,14 @@ struct BwdCfg {
   static constexpr int kOffOnes = kOffB + kB * kTileBytes;
   static constexpr int kOffStats = kOffOnes + (MODE == kDkv ? kTile * 128 : 0);
   static constexpr int kOffCtl = kOffStats + (MODE == kDkv ? kTile * 128 : 0);
-  static constexpr int kY = MODE == kDkv && D == 128 ? 1 : 2;           // dP tiles in TMEM
-  static constexpr uint32_t kColDp = 128, kColG = kColDp + kY * 128;
+  // TMEM.  Where two accumulators of 128 columns leave room for two tiles only (kTurns), a tile's S and dP take turns in one of
+  // them: dP is formed there once S has been read, while P is computed, and P and dS go over it.  Otherwise S has a tile of its
+  // own and dP two.  (One tile for S, one for dP: dP(j+1) waits for the gradients of tile j, which cost 500 us where this
+  // takes {T} at 8192 causal tokens, 16 heads of 128 sharing two key heads.)
+  static constexpr bool kTurns = MODE == kDkv && D == 128;
+  static constexpr uint32_t kColG = kTurns ? 256 : 384;
+  __device__ static uint32_t s_tile(int j) { return kTurns ? (j & 1) * 128 : 0; }
+  __device__ static uint32_t dp_tile(int j) { return kTurns ? (j & 1) * 128 : 128 + (j & 1) * 128; }
 };
 struct BwdCtl {
   uint64_t lane_full, a_full[4], a_empty[4], b_full[4], b_empty[4], tail_a, tail_b;
@@ -97,8 +101,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   constexpr int NA = Cfg::kA, NB = Cfg::kB, TB = Cfg::kTileBytes;
   constexpr uint32_t kIdescS = make_idesc(/*bf16*/ 1, kTile, kTile, 0, 0);
   constexpr uint32_t kIdescG = make_idesc(/*bf16*/ 1, kTile, D, 0, /*B is MN-major*/ 1);
-  constexpr int kY = Cfg::kY;
-  constexpr uint32_t kColDp = Cfg::kColDp, kColG = Cfg::kColG;
+  constexpr uint32_t kColG = Cfg::kColG;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -229,18 +232,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int j = 0; ok && j < n; ++j) {
         ok = wait(&ctl->a_full[j % NA], (j / NA) & 1, kDevWaitTmaFull) &&
              (MODE == kDq || wait(&ctl->stat_full[j & 1], (j >> 1) & 1, kDevWaitTmaFull)) &&
-             (j == 0 || wait(&ctl->s_read, (j - 1) & 1, kDevWaitAccEmpty));
+             (Cfg::kTurns ? j < 2 || wait(&ctl->ds_done[j & 1], ((j >> 1) & 1) ^ 1, kDevWaitPvDone)      // dS(j-2) lay there
+                          : j == 0 || wait(&ctl->s_read, (j - 1) & 1, kDevWaitAccEmpty));                // S(j-1)
         if (!ok) break;
         tc_fence_after();
-        product(tmem_base, l1, ra + (j % NA) * TB);
-        if (MODE == kDkv) plus_stat(tmem_base, (j & 1) * 2);
+        product(tmem_base + Cfg::s_tile(j), l1, ra + (j % NA) * TB);
+        if (MODE == kDkv) plus_stat(tmem_base + Cfg::s_tile(j), (j & 1) * 2);
         umma_commit(&ctl->s_full);
-        // P and dS of tile j - kY lay where dP(j) goes
         ok = wait(&ctl->b_full[j % NB], (j / NB) & 1, kDevWaitTmaFull) &&
-             (j < kY || wait(&ctl->ds_done[(j - kY) & 1], ((j - kY) >> 1) & 1, kDevWaitPvDone));
+             (Cfg::kTurns ? wait(&ctl->s_read, j & 1, kDevWaitAccEmpty)                                  // S(j) lay there
+                          : j < 2 || wait(&ctl->ds_done[j & 1], ((j >> 1) & 1) ^ 1, kDevWaitPvDone));    // dS(j-2)
         if (!ok) break;
         tc_fence_after();
-        const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
+        const uint32_t col = tmem_base + Cfg::dp_tile(j);
         product(col, l2, rb + (j % NB) * TB);
         if (MODE == kDkv) {
           plus_stat(col, (j & 1) * 2 + 1);
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (!ok) break;
       if (lane == 0) {
         tc_fence_after();
-        const uint32_t col = tmem_base + kColDp + (j % kY) * 128;
+        const uint32_t col = tmem_base + Cfg::dp_tile(j);
         gradient(tmem_base + kColG + (MODE == kDkv ? D : 0), col + 16, ra + (j % NA) * TB, j == 0);   // (dK first: Q's stage
         umma_commit(&ctl->a_empty[j % NA]);                                                           // is wanted sooner)
         if (MODE == kDkv) {
@@ -359,8 +363,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       limit = min(u.len, u.off + tk + 1) - u.b0 * kTile;
     }
     for (int j = 0; j < n; ++j) {
-      const uint32_t s_col = tmem_base + lane_off + c0;
-      const uint32_t dp_col = tmem_base + lane_off + kColDp + (j % kY) * 128 + c0;
+      const uint32_t s_col = tmem_base + lane_off + Cfg::s_tile(j) + c0;
+      const uint32_t dp_col = tmem_base + lane_off + Cfg::dp_tile(j) + c0;
       // the columns that the row sees: keys before its limit, or queries from `lo` on
       int lo = 0, hi;
       if (MODE == kDq) {
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->s_read);              // S(j+1) may go there
+        if (lane == 0) mbar_arrive(&ctl->s_read);              // S(j+1) or dP(j) may go there
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {                      // (kDkv: the scores hold -lse already)
           fma2(pr[i], pr[i + 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]), c2, neg_lse, neg_lse);
