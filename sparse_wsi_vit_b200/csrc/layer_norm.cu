@@ -193,9 +193,12 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_nor
   Raw<U, VEC> gn[ITER];
 #pragma unroll
   for (int i = 0; i < R; ++i) dw[i] = db[i] = 0.f;
+  float mu_next, rstd_next;
   auto fetch = [&](int64_t r) {
     const T* xr = static_cast<const T*>(p.x) + r * p.xs;
     const U* dyr = static_cast<const U*>(p.dy) + r * p.dys;
+    mu_next = r < p.N ? p.mean[r] : 0.f;
+    rstd_next = r < p.N ? p.rstd[r] : 0.f;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * TPR + t) * VEC;
@@ -211,8 +214,8 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_nor
   if (kAhead) fetch(row);
   stage_weights<VEC, ITER, TPR>(p, ws, false);
   for (; row < p.N; row += groups) {
-    const float mu = p.mean[row], rstd = p.rstd[row];
     if (!kAhead) fetch(row);
+    const float mu = mu_next, rstd = rstd_next;
     Raw<T, VEC> x[ITER];
     Raw<U, VEC> g[ITER];
 #pragma unroll

@@ -64,7 +64,7 @@ struct BwdCfg {
   // TMEM.  Where two accumulators of 128 columns leave room for two tiles only (kTurns), a tile's S and dP take turns in one of
   // them: dP is formed there once S has been read, while P is computed, and P and dS go over it.  Otherwise S has a tile of its
   // own and dP two.  (One tile for S, one for dP: dP(j+1) waits for the gradients of tile j, which cost 500 us where this
-  // takes {T} at 8192 causal tokens, 16 heads of 128 sharing two key heads.)
+  // takes 473 at 8192 causal tokens, 16 heads of 128 sharing two key heads.)
   static constexpr bool kTurns = MODE == kDkv && D == 128;
   static constexpr uint32_t kColG = kTurns ? 256 : 384;
   __device__ static uint32_t s_tile(int j) { return kTurns ? (j & 1) * 128 : 0; }
