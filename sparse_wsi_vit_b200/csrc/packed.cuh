@@ -8,6 +8,7 @@
 namespace swv {
 
 constexpr int kPlanMagic = 0x53575031;
+constexpr float kMinScale = 8.673617379884035e-19f;       // 2^-60; lse / scale and scale x score stay in fp32's range
 constexpr int kPlanHeader = 32;           // words
 
 struct PackedHeader {                     // words 0..31 of a plan
@@ -136,6 +137,13 @@ int prepare_kernel(K kernel, std::atomic<uint64_t>& done, int threads, int share
   SWV_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   if (dev < 64) done.fetch_or(bit, std::memory_order_release);
   return SWV_OK;
+}
+
+// The producer ends by waiting for its last copies (with the limit of one wait each): a CTA that gave up does not leave its
+// shared memory to copies in flight; otherwise they have landed long since.
+__device__ __forceinline__ void drain_copy(uint64_t* bar, uint32_t parity) {
+  volatile uint32_t never = 0;
+  (void)mbar_wait_bounded(bar, parity, &never);
 }
 
 }  // namespace swv

@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         for (int c = 0; c < D / 64; ++c)
           tma_load_4d(smem + t * Cfg::kTileBytes + c * (kTile * 128), &tm_q, &ctl->q_full[t], c * 64, 0, u.t0 + t * p.tok, kvh);
       }
-      for (int it = 0; it < 2 * n; ++it) {
+      int it = 0;
+      for (; it < 2 * n; ++it) {
         const int s = it % NST;
         if (!mbar_wait_bounded(&ctl->empty[s], ((it / NST) & 1) ^ 1, abort_flag)) {
           record_status(p.status, kDevWaitStageEmpty);
@@ -162,6 +163,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         for (int c = 0; c < D / 64; ++c)
           tma_load_3d(smem + Cfg::kOffRing + s * Cfg::kTileBytes + c * (kTile * 128), (it & 1) ? &tm_v : &tm_k, bar,
                       c * 64, key0, kvh);
+      }
+      for (int t = 0; t < 2; ++t)
+        if (blocks(t) > 0) drain_copy(&ctl->q_full[t], 0);
+      for (int i = max(0, it - NST); i < it; ++i) {
+        const bool cut = tail && i == 2 * n - 1;
+        drain_copy(cut ? &ctl->tail_full : &ctl->full[i % NST], cut ? 0 : (i / NST) & 1);
       }
     }
   } else if (warp <= 2) {
@@ -564,7 +571,7 @@ int packed_attn_fwd_impl(const void* q, const int64_t* qs, const void* k, const 
   int rc = packed_plan_header(plan_host, &h);
   if (rc != SWV_OK) return rc;
   if (Tq < h.Tq || Tk < h.Tk || Tq > 0x7fffffff || Tk > 0x7fffffff) return SWV_ERR_SHAPE;
-  if (!(scale > 0.f) || !std::isfinite(scale)) return SWV_ERR_SHAPE;
+  if (!(scale >= kMinScale && scale <= 1.f / kMinScale)) return SWV_ERR_SHAPE;
   if (D < 8 || D % 8 != 0 || D > 128) return SWV_ERR_UNSUPPORTED;
   if (h.n_fwd == 0) return SWV_OK;                           // no query
   if (!q || !o || !plan || !status) return SWV_ERR_NULL;
@@ -576,7 +583,7 @@ int packed_attn_fwd_impl(const void* q, const int64_t* qs, const void* k, const 
   }
   if (!packed_aligned(q, qs, 2) || !packed_aligned(k, ks, 2) || !packed_aligned(v, vs, 2) || !packed_aligned(o, os, 2))
     return SWV_ERR_ALIGN;
-  if (static_cast<int64_t>(h.n_fwd) * h.Hkv > 0x7fffffff || h.Hkv > 65535) return SWV_ERR_TOO_LARGE;
+  if (static_cast<int64_t>(h.n_fwd) * h.Hkv > 0x7fffffff || h.Hkv > 65535) return SWV_ERR_UNSUPPORTED;
   size_t need = 0;
   packed_attn_bytes_impl(plan_host, D, &need);
   if (need > 0) {

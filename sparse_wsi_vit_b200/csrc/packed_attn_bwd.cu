@@ -189,6 +189,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tma_load_4d(smem + TB + c * (kTile * 128), &tm_l2, &ctl->lane_full, c * 64, 0, u.t0, kvh);
         }
       }
+      int loads[2] = {0, 0};                                    // of ring A and ring B
       for (int j = 0; j < n; ++j) {
         const int at = u.s0 + (u.b0 + j) * step;
         // (the stages of the tail are declared full by the warp that cleans them)
@@ -202,6 +203,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           uint8_t* dst = smem + (r == 0 ? Cfg::kOffA : Cfg::kOffB) + s * TB;
           uint64_t* bar = !cut ? full : r == 0 ? &ctl->tail_a : (MODE == kDkv ? &ctl->tail_b : full);
           mbar_expect_tx(bar, per * D * 2);
+          ++loads[r];
           const CUtensorMap* tm = r == 0 ? &tm_a : &tm_b;
 #pragma unroll
           for (int c = 0; c < D / 64; ++c) {
@@ -210,6 +212,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
         }
         if (*abort_flag != 0u) break;
+      }
+      drain_copy(&ctl->lane_full, 0);
+      for (int r = 0; r < 2; ++r) {
+        const int N = r == 0 ? NA : NB;
+        for (int j = max(0, loads[r] - N); j < loads[r]; ++j) {
+          const bool cut = tail && j == n - 1 && (r == 0 || MODE == kDkv);
+          uint64_t* bar = cut ? (r == 0 ? &ctl->tail_a : &ctl->tail_b) : r == 0 ? &ctl->a_full[j % N] : &ctl->b_full[j % N];
+          drain_copy(bar, cut ? 0 : (j / N) & 1);
+        }
       }
     }
   } else if (warp == 1) {
@@ -633,7 +644,7 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   int rc = packed_plan_header(plan_host, &h);
   if (rc != SWV_OK) return rc;
   if (Tq < h.Tq || Tk < h.Tk || Tq > 0x7fffffff || Tk > 0x7fffffff) return SWV_ERR_SHAPE;
-  if (!(scale > 0.f) || !std::isfinite(scale)) return SWV_ERR_SHAPE;
+  if (!(scale >= kMinScale && scale <= 1.f / kMinScale)) return SWV_ERR_SHAPE;
   if (D < 8 || D % 8 != 0 || D > 128) return SWV_ERR_UNSUPPORTED;
   if (h.Tq == 0 && h.Tk == 0) return SWV_OK;
   if (!plan || !status || !workspace) return SWV_ERR_NULL;
@@ -648,7 +659,7 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   if ((h.Tq > 0 && !packed_aligned(dq, dqs, 2)) ||
       (h.Tk > 0 && (!packed_aligned(dk, dks, 2) || !packed_aligned(dv, dvs, 2))))
     return SWV_ERR_ALIGN;
-  if (static_cast<int64_t>(std::max(h.n_dq, h.n_dkv)) * h.Hkv > 0x7fffffff || h.Hkv > 65535) return SWV_ERR_TOO_LARGE;
+  if (static_cast<int64_t>(std::max(h.n_dq, h.n_dkv)) * h.Hkv > 0x7fffffff || h.Hkv > 65535) return SWV_ERR_UNSUPPORTED;
   const BwdSizes sz = bwd_sizes(h, Tq, D);
   if (workspace_bytes < sz.stats + sz.dq + sz.dkv) return SWV_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return SWV_ERR_ALIGN;

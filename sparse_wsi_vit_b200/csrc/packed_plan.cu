@@ -93,7 +93,7 @@ int check(int n_seq, const int64_t* ql, const int64_t* kl, int H, int Hkv, int64
     *Tq += ql[i];
     *Tk += kl[i];
     // token indices, key limits and their sums stay within 32 bits
-    if (*Tq > (1 << 29) || *Tk > (1 << 29)) return SWV_ERR_TOO_LARGE;
+    if (*Tq > (1 << 29) || *Tk > (1 << 29)) return SWV_ERR_UNSUPPORTED;
   }
   return SWV_OK;
 }
@@ -184,7 +184,7 @@ int packed_plan_impl(int n_seq, const int64_t* q_lens, const int64_t* k_lens, in
       memcpy(plan, out.data(), out.size() * 4);
     }
   } catch (...) {                                 // (host memory ran out)
-    return SWV_ERR_TOO_LARGE;
+    return SWV_ERR_UNSUPPORTED;
   }
   return SWV_OK;
 }

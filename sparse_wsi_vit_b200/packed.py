@@ -18,7 +18,7 @@ import functools
 import numpy as np
 import torch
 
-from ._lib import SwvError, check, dtype_code, lib
+from ._lib import SwvError, check, lib
 from .ops import _CHECK, _require_cuda, check_status, status_word
 
 _POS_CODES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
@@ -47,6 +47,20 @@ def _same_device(first, *ts):
     for t in ts:
         if t is not None and t.device != dev:
             raise SwvError("all tensors of a call must be on one device")
+
+
+def _check_out(out, like, inputs, same=None):
+    """An output buffer of the caller: no part of an autograd graph, and no memory of the inputs (``same``: or exactly
+    that one).  Its version is raised, so that a graph that has saved it notices."""
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise SwvError("out must have the result's shape, type and device")
+    if out.requires_grad:
+        raise SwvError("out must not require a gradient")
+    if same is None or out.data_ptr() != same.data_ptr() or out.stride() != same.stride():
+        mine = out.untyped_storage().data_ptr()
+        if any(t.untyped_storage().data_ptr() == mine for t in inputs):
+            raise SwvError("out must not share memory with the inputs")
+    torch.autograd.graph.increment_version(out)
 
 
 # --------------------------------------------------------------------------- #
@@ -126,7 +140,8 @@ class LayerNormFunction(torch.autograd.Function):
 def _norm_param(t, name, x):
     if t.dim() != 1 or t.shape[0] != x.shape[-1]:
         raise SwvError(f"{name} has shape {tuple(t.shape)}, expected {(x.shape[-1],)}")
-    dtype_code(t.dtype)
+    if t.dtype not in _DTYPES:
+        raise SwvError(f"{name} is float32, bfloat16 or float16, not {t.dtype}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -139,7 +154,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     _same_device(x, weight, bias)
     dt = x.dtype
     out_dtype = out_dtype or dt
-    dtype_code(dt), dtype_code(out_dtype)
+    if dt not in _DTYPES or out_dtype not in _DTYPES:
+        raise SwvError(f"layer_norm takes float32, bfloat16 and float16, not {dt} -> {out_dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise SwvError("layer_norm needs a last dimension of one value or more")
     if out_dtype != dt and dt != torch.float32 and out_dtype != torch.float32:
@@ -179,8 +195,8 @@ class RopeAxes:
             raise SwvError(f"{len(scales)} scales for {len(sections)} axes")
         if ladder not in ("axis", "head") or pairing not in ("adjacent", "halves"):
             raise SwvError(f"ladder is 'axis' or 'head', pairing 'adjacent' or 'halves'; got {ladder!r}, {pairing!r}")
-        if not theta > 0:
-            raise SwvError("theta must be positive")
+        if not 0 < theta < float("inf") or not np.isfinite(scales).all():
+            raise SwvError("theta must be positive, and it and the scales finite")
         self.head_dim, self.sections, self.pairs, self.halves = int(head_dim), tuple(sections), R, pairing == "halves"
         power = [(sum(sections[:a]) + i) / R if ladder == "head" else i / n for a, n in enumerate(sections) for i in range(n)]
         self._axis = np.repeat(np.arange(len(sections)), sections).astype(np.uint8)
@@ -217,13 +233,14 @@ class RopeAxesFunction(torch.autograd.Function):
 def rope_axes(x, positions, rope, out=None):
     """Turns the heads ``x (T, H, head_dim)`` (fp32, bf16 or fp16) by ``positions (T, axes)`` (fp32, int32 or int64) as
     ``rope`` (a ``RopeAxes``) says.  The queries and keys of a fused projection turn in one call as its leading heads.
-    ``out``: where to write, ``x`` itself included (inference only)."""
+    ``out``: where to write, exactly ``x`` or memory of its own (inference only)."""
     _same_device(x, positions)
     if x.dim() != 3 or x.shape[2] != rope.head_dim:
         raise SwvError(f"x has shape {tuple(x.shape)}, expected (tokens, heads, {rope.head_dim})")
     if x.shape[1] < 1:
         raise SwvError("rope_axes needs one head or more")
-    dtype_code(x.dtype)
+    if x.dtype not in _DTYPES:
+        raise SwvError(f"rope_axes takes float32, bfloat16 and float16, not {x.dtype}")
     if positions.dtype not in _POS_CODES:
         raise SwvError(f"positions are float32, int32 or int64, not {positions.dtype}")
     if tuple(positions.shape) != (x.shape[0], len(rope.sections)):
@@ -234,27 +251,34 @@ def rope_axes(x, positions, rope, out=None):
     if out is not None:
         if grad:
             raise SwvError("rope_axes writes into `out` only where no gradient is asked for")
-        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
-            raise SwvError("out must have x's shape, type and device, and unit inner stride")
-        if x.stride(2) != 1 and out.data_ptr() != x.data_ptr():
-            x = x.contiguous()
+        if out.stride(2) != 1:
+            raise SwvError("out must have unit inner stride")
+        _check_out(out, x, (x, positions), same=x)
     return RopeAxesFunction.apply(x, positions, rope) if grad else _rope_apply(x, positions, rope, False, out)
 
 
 # --------------------------------------------------------------------------- #
 # packed attention
 # --------------------------------------------------------------------------- #
+def _lengths(x):
+    a = np.asarray(x).reshape(-1)
+    if a.size and a.dtype.kind not in "iu":
+        raise SwvError(f"lengths are whole numbers, not {a.dtype}")
+    return np.ascontiguousarray(a, dtype=np.int64)
+
+
 class PackedPlan:
     """The work tables of one packed batch, for any number of calls with its lengths (all layers of an encoder).
 
     ``q_lengths`` / ``k_lengths``: tokens of every sequence (k_lengths None: the same); ``heads`` query heads share
     ``kv_heads`` key / value heads evenly.  ``causal``: query i of a sequence sees the keys j <= i + lk - lq.
     Made on the host and copied to ``device`` once; a captured CUDA graph keeps using the plan it was captured with, so
-    the plan must outlive it."""
+    the plan must outlive it.  (Before a backward pass is captured, let go of eager graphs of the same leaves, as for any torch
+    operator: their gradient nodes belong to another stream.)"""
 
     def __init__(self, q_lengths, k_lengths=None, *, heads, kv_heads=None, causal=False, device="cuda"):
-        ql = np.ascontiguousarray(np.asarray(q_lengths, dtype=np.int64).reshape(-1))
-        kl = ql if k_lengths is None else np.ascontiguousarray(np.asarray(k_lengths, dtype=np.int64).reshape(-1))
+        ql = _lengths(q_lengths)
+        kl = ql if k_lengths is None else _lengths(k_lengths)
         if len(ql) != len(kl):
             raise SwvError(f"{len(ql)} query lengths and {len(kl)} key lengths")
         self.heads, self.kv_heads, self.causal = int(heads), int(heads if kv_heads is None else kv_heads), bool(causal)
@@ -273,7 +297,14 @@ class PackedPlan:
         self._host = words[: size.value // 4].copy()
         self._table = torch.from_numpy(self._host).to(self.device)      # (waits for the copy: any stream may use it)
         self._call = (self._host.ctypes.data, self._table.data_ptr())
+        self._stream = _raw_stream(self.device.index) if self.device.type == "cuda" else 0
         self._bytes = {}
+
+    def _used(self):
+        """The tables are read on the current stream: their memory is not given to others before that is through."""
+        if _raw_stream(self.device.index) != self._stream and not torch.cuda.is_current_stream_capturing():
+            self._table.record_stream(torch.cuda.current_stream(self.device))
+        return self._call
 
     def _workspace_bytes(self, D, Tq=None):
         """Forward (Tq None) or backward workspace for head dimension D and buffers of Tq query rows."""
@@ -335,7 +366,7 @@ def _attn_fwd(q, k, v, plan, scale, want_lse, out=None):
     nws = plan._workspace_bytes(D)
     ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
     _call(lib.swv_packed_attn_fwd, "swv_packed_attn_fwd", dev, q.data_ptr(), _I3(*q.stride()), k.data_ptr(),
-          _I3(*k.stride()), v.data_ptr(), _I3(*v.stride()), o.data_ptr(), _I3(*o.stride()), _ptr(lse), *plan._call, Tq,
+          _I3(*k.stride()), v.data_ptr(), _I3(*v.stride()), o.data_ptr(), _I3(*o.stride()), _ptr(lse), *plan._used(), Tq,
           k.shape[0], D, scale, _ptr(ws), nws, status_word(dev).data_ptr())
     return o, lse
 
@@ -370,7 +401,7 @@ class PackedAttentionFunction(torch.autograd.Function):
         dqs, dks = _I3(*dq.stride()), _I3(*dk.stride())
         _call(lib.swv_packed_attn_bwd, "swv_packed_attn_bwd", dev, d_out.data_ptr(), _I3(*d_out.stride()), q.data_ptr(),
               _I3(*q.stride()), k.data_ptr(), _I3(*k.stride()), v.data_ptr(), _I3(*v.stride()), o.data_ptr(), dqs,
-              lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dks, *plan._call, Tq, Tk, D, ctx.scale,
+              lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dks, *plan._used(), Tq, Tk, D, ctx.scale,
               ws.data_ptr(), nws, status_word(dev).data_ptr())
         return dq, dk, dv, None, None
 
@@ -385,13 +416,14 @@ def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
     sequence; with ``out`` (inference only) those are left as they were."""
     _attn_check(q, k, v, plan)
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise SwvError("scale must be positive and finite")
+    if not 2.0 ** -60 <= scale <= 2.0 ** 60:
+        raise SwvError("scale must be positive, between 2^-60 and 2^60")
     grad = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
     if out is not None:
         if grad:
             raise SwvError("packed_attention writes into `out` only where no gradient is asked for")
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not _rows_ok(out):
-            raise SwvError("out must have q's shape, type and device, and rows on 16 bytes")
+        _check_out(out, q, (q, k, v))
+        if not _rows_ok(out):
+            raise SwvError("out must have rows on 16 bytes")
     o, lse = PackedAttentionFunction.apply(q, k, v, plan, scale) if grad else _attn_fwd(q, k, v, plan, scale, return_lse, out)
     return (o, lse) if return_lse else o

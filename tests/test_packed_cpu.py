@@ -109,6 +109,10 @@ def test_plan_refusals(swv):
         swv.PackedPlan([4], heads=129, kv_heads=1, device="cpu")
     with pytest.raises(E):
         swv.PackedPlan([1 << 29, 1], heads=2, device="cpu")
+    with pytest.raises(E):
+        swv.PackedPlan([4.5], heads=2, device="cpu")
+    assert swv.PackedPlan([], heads=2, device="cpu").q_tokens == 0
+    assert swv.PackedPlan(torch.tensor([3, 4]), heads=2, device="cpu").q_tokens == 7
 
 
 def test_packed_attention_entry_points_refuse(swv):
@@ -133,6 +137,7 @@ def test_packed_attention_entry_points_refuse(swv):
     assert fwd(qs=odd) == -2 and fwd(q=ctypes.c_void_p(0x1008)) == -2
     assert fwd(Tq=299) == -4 and fwd(Tk=10) == -4
     assert fwd(scale=0.0) == -4 and fwd(scale=-1.0) == -4 and fwd(scale=float("nan")) == -4 and fwd(scale=float("inf")) == -4
+    assert fwd(scale=2.0 ** -61) == -4 and fwd(scale=2.0 ** 61) == -4
     assert fwd(D=12) == -8 and fwd(D=256) == -8
     assert L.swv_packed_attn_bwd_bytes(hp, 300, 64, ctypes.byref(n)) == 0 and n.value >= 4 * 300 * 8
     assert L.swv_packed_attn_bwd_bytes(hp, 200, 64, ctypes.byref(n)) == -4
@@ -179,7 +184,7 @@ def test_python_refusals_without_a_gpu(swv):
         swv.packed_attention(t, t, t, plan)
     for bad in (dict(sections=(5,)), dict(sections=()), dict(sections=(-1, 2)), dict(sections=(0, 0)),
                 dict(sections=(2, 2), scales=(1.0,)), dict(sections=(2,), ladder="x"), dict(sections=(2,), pairing="x"),
-                dict(sections=(2,), theta=0.0), dict(sections=(1,) * 9)):
+                dict(sections=(2,), theta=0.0), dict(sections=(2,), theta=float("inf")), dict(sections=(2,), scales=(float("nan"),)), dict(sections=(1,) * 9)):
         with pytest.raises(E):
             swv.RopeAxes(8, **bad)
     with pytest.raises(E):

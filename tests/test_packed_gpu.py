@@ -302,6 +302,69 @@ def test_attention_two_streams_share_a_plan(swv):
         assert all(torch.equal(x, w) for x in g)
 
 
+def test_offsets_beyond_32_bits(swv):
+    """Rows 2^27 elements apart (a long cache's token stride): offsets pass 2^31 elements and 2^32 bytes."""
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    ql = [20]
+    q, k, v, do = _qkv(ql, ql, 4, 2, 64, 30, fused=False)
+    buf = torch.empty(20, 1 << 27, dtype=torch.bfloat16, device="cuda")
+    far = lambda t, c: buf[:, c:c + t[0].numel()].view(t.shape).copy_(t)
+    fq, fk, fv, fo = far(q, 0), far(k, 1024), far(v, 2048), far(do, 4096)
+    plan = swv.PackedPlan(ql, heads=4, kv_heads=2, causal=True)
+    want = swv.packed_attention(q, k, v, plan)
+    assert fq.stride(0) == 1 << 27 and torch.equal(swv.packed_attention(fq, fk, fv, plan), want)
+    leaves, wide = ([t.detach().requires_grad_() for t in x] for x in ((q, k, v), (fq, fk, fv)))
+    for a, b in zip(torch.autograd.grad(swv.packed_attention(*leaves, plan), leaves, do),
+                    torch.autograd.grad(swv.packed_attention(*wide, plan), wide, fo)):
+        assert torch.equal(a, b)
+    x = buf[:, 8192:8192 + 256]
+    x.copy_(torch.randn(20, 256, device="cuda"))
+    assert torch.equal(swv.layer_norm(x), swv.layer_norm(x.contiguous()))
+    rope, pos = swv.RopeAxes(64, (16, 16)), torch.arange(40, device="cuda").view(20, 2)
+    assert torch.equal(swv.rope_axes(fq, pos, rope), swv.rope_axes(q, pos, rope))
+
+
+def test_attention_plan_on_a_side_stream(swv):
+    """A plan made on one stream, used on another and dropped at once: its tables are not handed to others too early."""
+    ql = [3000]
+    q, k, v, _ = _qkv(ql, ql, 4, 4, 64, 31)
+    want = swv.packed_attention(q, k, v, swv.PackedPlan(ql, heads=4))
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    got = []
+    for _ in range(10):
+        plan = swv.PackedPlan(ql, heads=4)
+        with torch.cuda.stream(st):
+            got.append(swv.packed_attention(q, k, v, plan))
+        n = plan._host.size
+        del plan
+        torch.zeros(n, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_out_buffers_are_checked(swv):
+    """`out` shares no memory with the inputs, is in no graph, and a graph that has saved it notices."""
+    E = swv._lib.SwvError
+    ql = [20]
+    q, k, v, _ = _qkv(ql, ql, 4, 2, 64, 32, fused=False)
+    plan = swv.PackedPlan(ql, heads=4, kv_heads=2)
+    for bad in (q, torch.empty_like(q).requires_grad_()):
+        with pytest.raises(E):
+            swv.packed_attention(q, k, v, plan, out=bad)
+    rope, pos = swv.RopeAxes(64, (16, 16)), torch.zeros(20, 2, device="cuda")
+    buf = torch.randn(21, 4, 64, device="cuda")
+    with pytest.raises(E):
+        swv.rope_axes(buf[:20], pos, rope, out=buf[1:])
+    x = torch.randn(20, 4, 64, device="cuda")
+    w = torch.randn(20, 4, 64, device="cuda", requires_grad=True)
+    y = (w * x).sum()                                  # saves x
+    swv.rope_axes(x, pos, rope, out=x)
+    with pytest.raises(RuntimeError):
+        y.backward()
+
+
 def test_attention_refusals(swv):
     E = swv._lib.SwvError
     ql = [20]
@@ -314,7 +377,7 @@ def test_attention_refusals(swv):
     wide = torch.randn(20, 2, 136, device="cuda").bfloat16()
     with pytest.raises(E):
         swv.packed_attention(wide, wide, wide, swv.PackedPlan(ql, heads=2))
-    for s in (0.0, -1.0, math.inf, math.nan):
+    for s in (0.0, -1.0, math.inf, math.nan, 2.0 ** -61, 2.0 ** 61):
         with pytest.raises(E):
             swv.packed_attention(q, k, v, plan, scale=s)
     with pytest.raises(E):
