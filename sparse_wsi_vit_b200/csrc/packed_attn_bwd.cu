@@ -647,7 +647,7 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   if (!(scale >= kMinScale && scale <= 1.f / kMinScale)) return SWV_ERR_SHAPE;
   if (D < 8 || D % 8 != 0 || D > 128) return SWV_ERR_UNSUPPORTED;
   if (h.Tq == 0 && h.Tk == 0) return SWV_OK;
-  if (!plan || !status || !workspace) return SWV_ERR_NULL;
+  if (!plan || !status) return SWV_ERR_NULL;
   if (h.Tq > 0 && (!d_out || !q || !o || !lse || !dq)) return SWV_ERR_NULL;
   if (h.Tk > 0 && (!k || !v || !dk || !dv)) return SWV_ERR_NULL;
   // one side empty: the maps need some memory, nothing reads it
@@ -660,7 +660,8 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
       (h.Tk > 0 && (!packed_aligned(dk, dks, 2) || !packed_aligned(dv, dvs, 2))))
     return SWV_ERR_ALIGN;
   if (static_cast<int64_t>(std::max(h.n_dq, h.n_dkv)) * h.Hkv > 0x7fffffff || h.Hkv > 65535) return SWV_ERR_UNSUPPORTED;
-  const BwdSizes sz = bwd_sizes(h, Tq, D);
+  const BwdSizes sz = bwd_sizes(h, h.Tq == 0 ? 0 : Tq, D);
+  if (!workspace && sz.stats + sz.dq + sz.dkv > 0) return SWV_ERR_NULL;
   if (workspace_bytes < sz.stats + sz.dq + sz.dkv) return SWV_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return SWV_ERR_ALIGN;
 

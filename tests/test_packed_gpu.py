@@ -112,6 +112,7 @@ SHAPES = [
     ([1, 2, 5], [777, 64, 3000], 16, 2, 128, True), ([2, 2], [6007, 300], 6, 6, 64, False),     # few queries: divided keys
     ([70, 3, 128], [20, 5, 128], 10, 2, 80, True),                                             # rows that see nothing
     ([1000], [2500], 12, 4, 96, True), ([3000], [100], 2, 2, 64, False),                       # divided queries
+    ([0, 0], [7, 30], 2, 2, 64, False), ([5, 9], [0, 0], 2, 1, 64, True), ([0], [0], 2, 2, 64, False),    # a side without tokens
     ([200, 30], [0, 40], 2, 2, 64, False), ([0, 10], [30, 20], 3, 1, 128, False), ([40], None, 7, 1, 72, True),
     ([9], [400], 128, 1, 64, True), ([33], [70], 128, 2, 24, False), ([500, 600], None, 16, 2, 40, True),
     ([2048], None, 2, 2, 64, True), ([1025, 1023], None, 4, 4, 128, True),
