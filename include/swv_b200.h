@@ -437,7 +437,7 @@ int swv_rope_axes_apply(const void* x, const int64_t x_strides[3], void* y, cons
  *
  * swv_packed_plan turns the lengths (HOST arrays) into the kernels' work tables: one int32 HOST array that the caller
  * copies to the device; both copies are passed to every call.  *bytes (may be NULL) gets its size, also when `plan` is
- * NULL or too small (SWV_ERR_WORKSPACE).  At most 2^29 tokens.
+ * NULL or too small (SWV_ERR_WORKSPACE).  At most 2^29 tokens and 2^27 units of work (tiles of 128 rows).
  *
  *   q, o, dq, d_out (Tq,H,D), k, v, dk, dv (Tk,Hkv,D) bf16: strides (t,h,d), unit inner stride, rows on 16 bytes;
  *   D a multiple of 8 up to 128; Tq, Tk at least the plan's tokens: rows behind them are neither read nor written;

@@ -88,12 +88,17 @@ int check(int n_seq, const int64_t* ql, const int64_t* kl, int H, int Hkv, int64
   if (n_seq > 0 && (!ql || !kl)) return SWV_ERR_NULL;
   if (H / Hkv > kTile) return SWV_ERR_UNSUPPORTED;
   *Tq = *Tk = 0;
+  const int64_t tok = kTile / (H / Hkv);
+  int64_t units = 0;                              // of the three passes
   for (int i = 0; i < n_seq; ++i) {
     if (ql[i] < 0 || kl[i] < 0) return SWV_ERR_SHAPE;
     *Tq += ql[i];
     *Tk += kl[i];
     // token indices, key limits and their sums stay within 32 bits
     if (*Tq > (1 << 29) || *Tk > (1 << 29)) return SWV_ERR_UNSUPPORTED;
+    // and so do the tables' offsets in words (eight a unit; dividing adds few)
+    units += (ql[i] + 2 * tok - 1) / (2 * tok) + (ql[i] + tok - 1) / tok + (kl[i] + kTile - 1) / kTile;
+    if (units > (1 << 27)) return SWV_ERR_UNSUPPORTED;
   }
   return SWV_OK;
 }

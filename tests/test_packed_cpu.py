@@ -191,3 +191,13 @@ def test_python_refusals_without_a_gpu(swv):
         swv.RopeAxes(512, (200,))
     with pytest.raises(E):
         swv.rope_axes(torch.randn(2, 1, 8), torch.zeros(2, 1), swv.RopeAxes(8, (4,)))
+
+
+def test_plan_of_more_work_than_its_tables_address_is_refused(swv):
+    """2^29 tokens in tiles of one token (128 heads share a key head) are 2^29 units and more: word offsets of 32 bits do
+    not reach them.  Refused before anything is allocated, with and without a buffer for the plan."""
+    with pytest.raises(swv._lib.SwvError):
+        swv.PackedPlan([1 << 29], [1], heads=128, kv_heads=1, device="cpu")
+    n, one, size = (ctypes.c_int64 * 1)(1 << 29), (ctypes.c_int64 * 1)(1), ctypes.c_size_t()
+    lib = swv._lib.lib
+    assert lib.swv_packed_plan(1, n, one, 128, 1, 0, None, 0, ctypes.byref(size)) not in (0, -5)
