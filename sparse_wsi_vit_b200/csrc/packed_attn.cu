@@ -12,9 +12,9 @@
 //   warp 3      : zeroes the value rows behind the sequence's end in its last tile (they belong to the next sequence
 //                 or to nobody, and 0 x NaN would reach O)
 //   warps 4..7 and 8..11 : softmax of tile A and of tile B, one thread per row: the row's 128 scores are read into registers,
-//                 P is written as bf16 pairs, in two halves, so that P V
-//                 starts under the second half's exponentials.  P is rounded to bf16 because the product takes
-//                 16-bit operands (2^-9 of each, independent); l sums the unrounded values.
+//                 P is written as bf16 pairs, in two halves, so that P V starts under the second half's exponentials.
+//                 P is rounded to bf16 because the product takes 16-bit operands (each entry is off by at most 2^-8);
+//                 l sums the unrounded values.
 //                 The stabiliser is raised (and O in TMEM rescaled) only when a row's maximum exceeds it by 2^8.
 // The scores' slot is free as soon as they are in registers, so S = Q K(j+1)^T is formed while the exponentials of block j run
 // (D = 128 has one slot for both tiles in turn); P has columns of its own.
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     tmem_relinquish();
   }
   const int n = u.b1 - u.b0;
-  // tokens and key blocks of tile t: its last token sees the fewest keys of no later tile
+  // tokens and key blocks of tile t (its last token sees the most keys)
   auto tokens = [&](int t) { return min(p.tok, u.n - t * p.tok); };
   auto blocks = [&](int t) {
     const int tk = tokens(t);
@@ -415,6 +415,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          if (__any_sync(0xffffffffu, l == 0.f)) {             // a row that sees no key is zero, also where 0 x v is NaN
+            KEEP_BRANCH();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0u : o[i];
           }
           stage_columns<D, 32>(stage, row, c, o, inv);
         }

@@ -56,6 +56,12 @@ def _check_out(out, like, inputs, same=None):
         raise SwvError("out must have the result's shape, type and device")
     if out.requires_grad:
         raise SwvError("out must not require a gradient")
+    if not out.is_contiguous():
+        reach = 1                                         # elements that the dimensions inside span
+        for n, s in sorted(zip(out.shape, out.stride()), key=lambda d: d[1]):
+            if n > 1 and s < reach:
+                raise SwvError("out must not hold an element twice")
+            reach += (n - 1) * s
     if same is None or out.data_ptr() != same.data_ptr() or out.stride() != same.stride():
         mine = out.untyped_storage().data_ptr()
         if any(t.untyped_storage().data_ptr() == mine for t in inputs):
@@ -245,6 +251,8 @@ def rope_axes(x, positions, rope, out=None):
         raise SwvError(f"positions are float32, int32 or int64, not {positions.dtype}")
     if tuple(positions.shape) != (x.shape[0], len(rope.sections)):
         raise SwvError(f"positions have shape {tuple(positions.shape)}, expected {(x.shape[0], len(rope.sections))}")
+    if positions.requires_grad and torch.is_grad_enabled():
+        raise SwvError("positions have no gradient: detach them")
     if positions.stride(1) != 1 and positions.shape[1] > 1:
         positions = positions.contiguous()
     grad = torch.is_grad_enabled() and x.requires_grad
@@ -283,6 +291,8 @@ class PackedPlan:
             raise SwvError(f"{len(ql)} query lengths and {len(kl)} key lengths")
         self.heads, self.kv_heads, self.causal = int(heads), int(heads if kv_heads is None else kv_heads), bool(causal)
         device = torch.device(device)
+        if device.type == "cuda" and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise SwvError("make the plan before the capture: its tables are copied from the host")
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
         self.q_tokens, self.k_tokens = int(ql.sum()), int(kl.sum())
         size = ctypes.c_size_t()
@@ -413,7 +423,9 @@ def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
     projection are read as they are if their rows lie on 16 bytes); ``plan``: the batch's ``PackedPlan``; ``scale``
     defaults to 1 / sqrt(D).  Returns ``(Tq, heads, D)`` bf16, with ``return_lse`` also the rows' log-sum-exp (heads, Tq)
     fp32, which has no gradient.  A row that sees no key is zero (lse -inf), and so are rows behind the last
-    sequence; with ``out`` (inference only) those are left as they were."""
+    sequence; with ``out`` (inference only) those are left as they were.  A NaN or an infinity never leaves its sequence;
+    inside a causal one it can reach rows that do not see it (a masked pair is multiplied with zero): from a value row
+    the results, from any input the gradients."""
     _attn_check(q, k, v, plan)
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     if not 2.0 ** -60 <= scale <= 2.0 ** 60:

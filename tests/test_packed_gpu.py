@@ -602,3 +602,58 @@ def test_rope_axes_refusals(swv):
         swv.rope_axes(x.requires_grad_(), pos, rope, out=torch.empty_like(x))
     with pytest.raises(E):
         swv.rope_axes(x.detach(), pos, rope, out=torch.empty(4, 2, 8, device="cuda").bfloat16())
+
+
+def test_rope_axes_positions_have_no_gradient(swv):
+    """Positions that ask for a gradient are refused instead of getting none; without gradients they are taken."""
+    x, pos, rope = torch.randn(4, 2, 8, device="cuda"), torch.ones(4, 2, device="cuda"), swv.RopeAxes(8, (2, 2))
+    want = swv.rope_axes(x, pos, rope)
+    pos.requires_grad_()
+    with pytest.raises(swv._lib.SwvError):
+        swv.rope_axes(x, pos, rope)
+    with torch.no_grad():
+        assert torch.equal(swv.rope_axes(x, pos, rope), want)
+
+
+def test_out_buffers_hold_every_element_once(swv):
+    E = swv._lib.SwvError
+    rope, pos = swv.RopeAxes(64, (16, 16)), torch.zeros(20, 2, device="cuda")
+    x = torch.randn(20, 1, 64, device="cuda").expand(20, 4, 64)          # the heads share their memory
+    wide = torch.empty(20, 4, 128, device="cuda")
+    lapped = torch.empty(4000, device="cuda").as_strided((20, 4, 64), (64, 64, 1))
+    for t, bad in ((x, x), (x, lapped)):
+        with pytest.raises(E):
+            swv.rope_axes(t, pos, rope, out=bad)
+    assert torch.equal(swv.rope_axes(x, pos, rope, out=wide[..., :64]), swv.rope_axes(x, pos, rope))
+    heads_first = torch.empty(4, 20, 64, device="cuda").transpose(0, 1)  # another order of the dimensions
+    assert torch.equal(swv.rope_axes(x, pos, rope, out=heads_first), swv.rope_axes(x, pos, rope))
+    q, k, v, _ = _qkv([20], [20], 4, 2, 64, 32, fused=False)
+    with pytest.raises(E):
+        swv.packed_attention(q, k, v, swv.PackedPlan([20], heads=4, kv_heads=2), out=lapped.bfloat16().as_strided((20, 4, 64), (64, 64, 1)))
+
+
+def test_plan_inside_a_capture_is_refused(swv):
+    """Before the host copy that would end the capture; the capture goes on."""
+    x, w = torch.randn(8, 16, device="cuda"), torch.ones(16, device="cuda")
+    want = swv.layer_norm(x, w)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = swv.layer_norm(x, w)
+        with pytest.raises(swv._lib.SwvError):
+            swv.PackedPlan([8], heads=1)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_row_that_sees_no_key_is_zero_beside_nan_values(swv, D):
+    """Causal, 40 queries and 30 keys: the first ten rows see nothing and are zero although the values are NaN."""
+    q, k, v, _ = _qkv([40, 50], [30, 50], 4, 2, D, 33, fused=False)
+    plan = swv.PackedPlan([40, 50], [30, 50], heads=4, kv_heads=2, causal=True)
+    clean = swv.packed_attention(q, k, v, plan)
+    bad = v.clone()
+    bad[:30] = math.nan
+    o, lse = swv.packed_attention(q, k, bad, plan, return_lse=True)
+    assert not bool(o[:10].any()) and bool((lse[:, :10] == -math.inf).all())
+    assert bool(torch.isnan(o[10:40]).all()) and torch.equal(o[40:], clean[40:])
