@@ -96,8 +96,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  int kvh;
-  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&ctl->q_full[t], 1);
@@ -119,6 +117,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
   }
+  grid_wait();
+  int kvh;
+  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
   const int n = u.b1 - u.b0;
   // tokens and key blocks of tile t (its last token sees the most keys)
   auto tokens = [&](int t) { return min(p.tok, u.n - t * p.tok); };
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = ctl->tmem_base;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
+  grid_release();
 
   if (warp < 4) {
   reg_dec<kFwdRegsControl>();
@@ -449,6 +451,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 template <int D>
 __global__ void __launch_bounds__(256) packed_attn_join_kernel(const PackedJoin* joins, const PackedFwdParams p) {
   constexpr int V = D / 32;                                    // channels a lane
+  grid_wait();
   const PackedJoin jn = joins[blockIdx.x];
   const int kvh = blockIdx.y, lane = threadIdx.x & 31;
   const float ninf = -__int_as_float(0x7f800000);
@@ -506,14 +509,14 @@ int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
   static std::atomic<uint64_t> prepared{0};
   const int rc = prepare_kernel(packed_attn_fwd_kernel<D>, prepared, kFwdThreads, kFwdRegs, fwd_smem<D>());
   if (rc != SWV_OK) return rc;
-  packed_attn_fwd_kernel<D><<<static_cast<unsigned>(p.n_units) * p.Hkv, kFwdThreads, fwd_smem<D>(), st>>>(tq, tk, tv, p);
-  SWV_CUDA_OK(cudaGetLastError());
+  SWV_CUDA_OK(launch_after(packed_attn_fwd_kernel<D>, static_cast<unsigned>(p.n_units) * p.Hkv, kFwdThreads, fwd_smem<D>(), st,
+                           tq, tk, tv, p));
   if (h.n_fwd_join > 0) {
     // a row a warp where there are few rows; at most 16 CTAs a unit
     const int rows = std::min(2 * p.tok, p.Tq) * p.group;
     const dim3 grid(h.n_fwd_join, p.Hkv, std::min(16, (rows + 7) / 8));
-    packed_attn_join_kernel<D><<<grid, 256, 0, st>>>(reinterpret_cast<const PackedJoin*>(plan + h.fwd_join_off), p);
-    SWV_CUDA_OK(cudaGetLastError());
+    SWV_CUDA_OK(launch_after(packed_attn_join_kernel<D>, grid, 256, 0, st,
+                             reinterpret_cast<const PackedJoin*>(plan + h.fwd_join_off), p));
   }
   return SWV_OK;
 }

@@ -48,6 +48,7 @@ struct PackedBwdParams {
   float scale, scale_log2;
   float* part;                  // [slot][Hkv][128][D (kDq) or 2 D (kDkv: dV, dK)] sums of divided units, before the scale
   int* status;
+  int wait_first;               // kDq: not launched behind the keys' side
 };
 
 template <int D, int MODE>
@@ -114,8 +115,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tma_prefetch_desc(&tm_a);
     tma_prefetch_desc(&tm_b);
   }
-  int kvh;
-  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
   if (threadIdx.x == 0) {
     mbar_init(&ctl->lane_full, 1);
     for (int s = 0; s < 4; ++s) {
@@ -144,6 +143,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
   }
+  if (MODE == kDkv || p.wait_first) grid_wait();
+  int kvh;
+  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
   const int n = u.b1 - u.b0;
   const int per = MODE == kDkv ? p.tok * p.group : kTile;      // streamed rows a tile
   const int step = MODE == kDkv ? p.tok : kTile;               // streamed tokens a tile
@@ -167,6 +169,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = ctl->tmem_base;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
+  grid_release();                                              // (after the wait of every thread of the CTA)
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     if (mbar_wait_bounded(bar, parity, abort_flag)) return true;
     record_status(p.status, code);
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const bool row_ok = row < rows;
     const int tk = MODE == kDkv ? row : row_token(row, p.group_inv);         // token of the lane side
     if (MODE == kDq && row_ok) {
-      const float2 f = __ldg(p.stats + (static_cast<int64_t>(kvh) * p.Tq + u.t0) * p.group + row);
+      const float2 f = __ldcg(p.stats + (static_cast<int64_t>(kvh) * p.Tq + u.t0) * p.group + row);
       neg_lse = f.x;
       neg_delta = f.y;
       limit = min(u.len, u.off + tk + 1) - u.b0 * kTile;
@@ -513,6 +516,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     __syncwarp();
     tmem_dealloc(tmem_base, 512);
   }
+  if (MODE == kDq && blockIdx.x == gridDim.x - 1) grid_wait();   // the grid's end stands for the keys' side's too
 }
 
 // -delta = -dO . O per row, and -lse in powers of two; half a warp a row.
@@ -520,6 +524,8 @@ __global__ void __launch_bounds__(256) packed_attn_delta_kernel(const __nv_bfloa
                                                                 const __nv_bfloat16* g, int64_t gs_t, int64_t gs_h,
                                                                 const float* lse, float2* stats, int64_t rows, int Tq,
                                                                 int tokens, int group, int d) {
+  grid_wait();
+  grid_release();
   const int sub = threadIdx.x & 15;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
   if (r >= rows) return;                                       // (half warps leave together: the sums below stay inside one)
@@ -554,6 +560,8 @@ __global__ void __launch_bounds__(256) packed_attn_delta_kernel(const __nv_bfloa
 template <int D, int MODE>
 __global__ void __launch_bounds__(256) packed_attn_bwd_join_kernel(const PackedJoin* joins, const PackedBwdParams p) {
   constexpr int kWidth = MODE == kDkv ? 2 * D : D;
+  grid_wait();
+  grid_release();
   const PackedJoin jn = joins[blockIdx.x];
   const int kvh = blockIdx.y, lane = threadIdx.x & 31;
   const int rows = MODE == kDkv ? jn.n : jn.n * p.group;
@@ -593,19 +601,31 @@ __global__ void __launch_bounds__(256) packed_attn_bwd_join_kernel(const PackedJ
 
 template <int D, int MODE>
 int launch_bwd(const CUtensorMap& l1, const CUtensorMap& l2, const CUtensorMap& a, const CUtensorMap& b,
-               const PackedBwdParams& p, const PackedJoin* joins, int n_join, cudaStream_t st) {
+               const PackedBwdParams& p, cudaStream_t st) {
   if (p.n_units == 0) return SWV_OK;
   static std::atomic<uint64_t> prepared{0};
   const int rc = prepare_kernel(packed_attn_bwd_kernel<D, MODE>, prepared, kBwdThreads, kBwdRegs, bwd_smem<D, MODE>());
   if (rc != SWV_OK) return rc;
-  packed_attn_bwd_kernel<D, MODE>
-      <<<static_cast<unsigned>(p.n_units) * p.Hkv, kBwdThreads, bwd_smem<D, MODE>(), st>>>(l1, l2, a, b, p);
-  SWV_CUDA_OK(cudaGetLastError());
-  if (n_join > 0) {
-    packed_attn_bwd_join_kernel<D, MODE><<<dim3(n_join, p.Hkv, 16), 256, 0, st>>>(joins, p);
-    SWV_CUDA_OK(cudaGetLastError());
-  }
+  SWV_CUDA_OK(launch_after(packed_attn_bwd_kernel<D, MODE>, static_cast<unsigned>(p.n_units) * p.Hkv, kBwdThreads,
+                           bwd_smem<D, MODE>(), st, l1, l2, a, b, p));
   return SWV_OK;
+}
+template <int D, int MODE>
+int launch_join(const PackedBwdParams& p, const int32_t* joins, int n_join, cudaStream_t st) {
+  if (n_join > 0)
+    SWV_CUDA_OK(launch_after(packed_attn_bwd_join_kernel<D, MODE>, dim3(n_join, p.Hkv, 16), 256, 0, st,
+                             reinterpret_cast<const PackedJoin*>(joins), p));
+  return SWV_OK;
+}
+template <int D>
+int launch_sides(const CUtensorMap& tq, const CUtensorMap& tg, const CUtensorMap& tk, const CUtensorMap& tv,
+                 const PackedBwdParams& keys, const PackedBwdParams& queries, const PackedHeader& h, const int32_t* plan,
+                 cudaStream_t st) {
+  int rc = launch_bwd<D, kDkv>(tk, tv, tq, tg, keys, st);
+  if (rc == SWV_OK) rc = launch_bwd<D, kDq>(tq, tg, tk, tv, queries, st);
+  if (rc == SWV_OK) rc = launch_join<D, kDkv>(keys, plan + h.dkv_join_off, h.n_dkv_join, st);
+  if (rc == SWV_OK) rc = launch_join<D, kDq>(queries, plan + h.dq_join_off, h.n_dq_join, st);
+  return rc;
 }
 
 struct BwdSizes {
@@ -676,10 +696,9 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   p.stats = stats;
   if (h.Tq > 0) {
     const int64_t rows = static_cast<int64_t>(h.H) * h.Tq;
-    packed_attn_delta_kernel<<<static_cast<unsigned>((rows + 15) / 16), 256, 0, st>>>(
-        static_cast<const __nv_bfloat16*>(o), os[0], os[1], static_cast<const __nv_bfloat16*>(d_out), gs[0], gs[1], lse,
-        stats, rows, static_cast<int>(Tq), h.Tq, p.group, D);
-    SWV_CUDA_OK(cudaGetLastError());
+    SWV_CUDA_OK(launch_after(packed_attn_delta_kernel, static_cast<unsigned>((rows + 15) / 16), 256, 0, st,
+                             static_cast<const __nv_bfloat16*>(o), os[0], os[1], static_cast<const __nv_bfloat16*>(d_out),
+                             gs[0], gs[1], lse, stats, rows, static_cast<int>(Tq), h.Tq, p.group, D));
   }
   CUtensorMap tq, tg, tk, tv;
   if ((rc = packed_tmap(&tq, q, qs, Tq, h.Hkv, p.group, D, p.tok)) != SWV_OK) return rc;
@@ -695,19 +714,14 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   a.g1 = dk; a.g1_t = dks[0]; a.g1_h = dks[1];
   a.g2 = dv; a.g2_t = dvs[0]; a.g2_h = dvs[1];
   a.part = reinterpret_cast<float*>(w + sz.dq);
-  const PackedJoin* ja = reinterpret_cast<const PackedJoin*>(plan + h.dkv_join_off);
-  rc = D <= 64 ? launch_bwd<64, kDkv>(tk, tv, tq, tg, a, ja, h.n_dkv_join, st)
-               : launch_bwd<128, kDkv>(tk, tv, tq, tg, a, ja, h.n_dkv_join, st);
-  if (rc != SWV_OK) return rc;
   PackedBwdParams b = p;                                       // queries' side
   b.units = reinterpret_cast<const PackedUnit*>(plan + h.dq_off);
   b.n_units = h.n_dq;
   b.heads_at_once = packed_heads_at_once(h.Hkv, h.longest_k, D);
   b.g1 = dq; b.g1_t = dqs[0]; b.g1_h = dqs[1];
   b.part = reinterpret_cast<float*>(w);
-  const PackedJoin* jb = reinterpret_cast<const PackedJoin*>(plan + h.dq_join_off);
-  return D <= 64 ? launch_bwd<64, kDq>(tq, tg, tk, tv, b, jb, h.n_dq_join, st)
-                 : launch_bwd<128, kDq>(tq, tg, tk, tv, b, jb, h.n_dq_join, st);
+  b.wait_first = a.n_units == 0;
+  return D <= 64 ? launch_sides<64>(tq, tg, tk, tv, a, b, h, plan, st) : launch_sides<128>(tq, tg, tk, tv, a, b, h, plan, st);
 }
 
 }  // namespace swv
