@@ -116,6 +116,8 @@ __device__ __forceinline__ void load_weights(const float* ws, float* v) {
 
 template <typename T, typename U, int VEC, int ITER, int TPR>
 __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 24 ? 2 : sizeof(T) == 4 ? 3 : 4) layer_norm_fwd_kernel(const LnParams p) {
+  grid_wait();
+  grid_release();
   __shared__ float red[4 * (kLnThreads / 32)];
   extern __shared__ float ws[];
   constexpr int C = VEC * ITER * TPR;
@@ -179,6 +181,8 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 24 ? 2 : sizeof(T) ==
 
 template <typename T, typename U, int VEC, int ITER, int TPR>
 __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_norm_bwd_kernel(const LnParams p) {
+  grid_wait();
+  grid_release();
   __shared__ float red[4 * (kLnThreads / 32)];
   extern __shared__ float ws[];
   constexpr int R = ITER * VEC, C = R * TPR;
@@ -291,6 +295,8 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_nor
 // Rows that do not fit the registers: one CTA per row, which it reads again for each of its sums (from L2).
 template <typename T, typename U>
 __global__ void __launch_bounds__(kLnThreads) layer_norm_wide_fwd_kernel(const LnParams p) {
+  grid_wait();
+  grid_release();
   __shared__ float red[4 * (kLnThreads / 32)];
   int phase = 0;
   const float inv_e = 1.f / p.E;
@@ -324,6 +330,8 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_wide_fwd_kernel(const L
 // workspace without conflict.
 template <typename T, typename U>
 __global__ void __launch_bounds__(kLnThreads) layer_norm_wide_bwd_kernel(const LnParams p) {
+  grid_wait();
+  grid_release();
   __shared__ float red[4 * (kLnThreads / 32)];
   int phase = 0;
   const float inv_e = 1.f / p.E;
@@ -358,6 +366,7 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_wide_bwd_kernel(const L
 // dw[c] = sum over the CTAs' rows of the workspace: 32 lanes of rows for 32 columns, added up in order
 __global__ void __launch_bounds__(1024) layer_norm_sum_kernel(const float* part, int parts, int E, void* dw, int dw_dtype,
                                                               void* db, int db_dtype) {
+  grid_wait();
   __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, r = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;                   // column of [dw | db]
@@ -413,16 +422,15 @@ int ln_launch(const LnParams& p, const LnForm& f, int grid, cudaStream_t st) {
     constexpr int kSmem = 2 * V * I * (BWD ? kLnThreads : R) * 4;                                                               \
     auto k = BWD ? layer_norm_bwd_kernel<T, U, V, I, R> : layer_norm_fwd_kernel<T, U, V, I, R>;              \
     if (kSmem > 40 * 1024) SWV_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)); \
-    k<<<grid, kLnThreads, kSmem, st>>>(p);                                                                   \
+    SWV_CUDA_OK(launch_after(k, grid, kLnThreads, kSmem, st, p));                                            \
   } else
   SWV_LN(8, 1, 32) SWV_LN(8, 2, 32) SWV_LN(8, 3, 32) SWV_LN(8, 4, 32) SWV_LN(8, 1, 64) SWV_LN(8, 1, 128) SWV_LN(8, 1, kLnThreads) SWV_LN(8, 2, 64) SWV_LN(8, 2, 128) SWV_LN(8, 2, kLnThreads) SWV_LN(8, 3, kLnThreads)
   SWV_LN(8, 4, kLnThreads)
   SWV_LN(1, 8, 32) SWV_LN(1, 32, 32) SWV_LN(1, 32, 128) SWV_LN(1, 32, kLnThreads) {
-    if constexpr (BWD) layer_norm_wide_bwd_kernel<T, U><<<grid, kLnThreads, 0, st>>>(p);
-    else layer_norm_wide_fwd_kernel<T, U><<<grid, kLnThreads, 0, st>>>(p);
+    auto k = BWD ? layer_norm_wide_bwd_kernel<T, U> : layer_norm_wide_fwd_kernel<T, U>;
+    SWV_CUDA_OK(launch_after(k, grid, kLnThreads, 0, st, p));
   }
 #undef SWV_LN
-  SWV_CUDA_OK(cudaGetLastError());
   return SWV_OK;
 }
 
@@ -505,8 +513,7 @@ int layer_norm_bwd_impl(const void* dy, int64_t dys, int y_dtype, const void* x,
     if (r != SWV_OK) return r;
   }
   if (sums) {                                             // (no rows: the sums are zero)
-    layer_norm_sum_kernel<<<(2 * E + 31) / 32, 1024, 0, st>>>(p.part, grid, E, dw, dw_dtype, db, db_dtype);
-    SWV_CUDA_OK(cudaGetLastError());
+    SWV_CUDA_OK(launch_after(layer_norm_sum_kernel, (2 * E + 31) / 32, 1024, 0, st, p.part, grid, E, dw, dw_dtype, db, db_dtype));
   }
   return SWV_OK;
 }

@@ -47,6 +47,8 @@ __device__ __forceinline__ void rope_angle(const RopeAxesParams& p, int64_t t, i
 // VEC = 8: 16-byte aligned rows, hd a multiple of 8 and (halves) the number of pairs too; VEC = 1: any layout.
 template <typename T, int VEC, bool HALVES>
 __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ RopeAxesParams p) {
+  grid_wait();
+  grid_release();
   // units of a token: (halves) VEC pairs a unit, then the channels that are copied; (adjacent) max(VEC / 2, 1) pairs a unit
   constexpr int PAIRS = HALVES ? VEC : (VEC == 8 ? 4 : 1);
   const int turning = (p.pairs + PAIRS - 1) / PAIRS;
@@ -132,11 +134,9 @@ int rope_axes_launch(RopeAxesParams& p, bool vec, bool halves, cudaStream_t st) 
   const int64_t split = std::min<int64_t>(std::min<int64_t>((want + blocks - 1) / blocks, (p.H + 1) / 2), 65535);
   p.heads_per_cta = static_cast<int>((p.H + split - 1) / split);
   const dim3 grid(static_cast<unsigned>(blocks), (p.H + p.heads_per_cta - 1) / p.heads_per_cta);
-  if (vec && halves) rope_axes_kernel<T, 8, true><<<grid, 256, 0, st>>>(p);
-  else if (vec) rope_axes_kernel<T, 8, false><<<grid, 256, 0, st>>>(p);
-  else if (halves) rope_axes_kernel<T, 1, true><<<grid, 256, 0, st>>>(p);
-  else rope_axes_kernel<T, 1, false><<<grid, 256, 0, st>>>(p);
-  SWV_CUDA_OK(cudaGetLastError());
+  auto k = vec ? (halves ? rope_axes_kernel<T, 8, true> : rope_axes_kernel<T, 8, false>)
+               : (halves ? rope_axes_kernel<T, 1, true> : rope_axes_kernel<T, 1, false>);
+  SWV_CUDA_OK(launch_after(k, grid, 256, 0, st, p));
   return SWV_OK;
 }
 
