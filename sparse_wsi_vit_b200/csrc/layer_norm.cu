@@ -3,14 +3,15 @@
 //   mu = mean(x)   rstd = 1 / sqrt(mean((x - mu)^2) + eps)   xh = (x - mu) rstd   y = xh w + b
 //   g  = dy w      dx = rstd (g - mean(g) - xh mean(g xh))   dw = sum_rows dy xh  db = sum_rows dy
 //
-// A group of threads (a warp, four or eight) owns a row: it is read once into registers, the variance is
+// A group of threads (one warp or more) owns a row: it is read once into registers, the variance is
 // taken from the centred values (a second sum over the registers, so a large offset of the row costs no bits), and
 // the result is written from the registers.  All sums are fp32.  The groups stay resident and walk over the rows, so
 // the weights stay in shared memory and, in the backward pass, the sums of dw and db in registers; the next row is loaded
-// before the present one is reduced, and a row is kept as it lies in memory (half the registers for 16-bit types).  Each CTA leaves its dw and db sums in the workspace and a second kernel adds them up in
-// a fixed order: no atomics, the same bits every time.
+// before the present one is reduced, and a row is kept as it lies in memory (half the registers for 16-bit types).  Each CTA
+// leaves its dw and db sums in the workspace and a second kernel adds them up in a fixed order: no atomics, the same bits every time.
 //
-// Bound: HBM, 2 N E elements forward, 3 N E backward.
+// Bound: HBM, 2 N E elements forward, 3 N E backward.  65536 x 768 bf16: 37 and 56 us, 5.4 TB/s each (82 % of the copy rate);
+// rows of 384 values reach 68 %: fewer bytes are in flight for a row's sums.
 #include <algorithm>
 #include <type_traits>
 
@@ -19,7 +20,14 @@
 namespace swv {
 namespace {
 
-constexpr int kLnThreads = 256;
+constexpr int kLnThreads = 256;                              // forms of wide rows
+// Threads of a CTA with runs of `run` values a thread and groups of `tpr` threads, and resident CTAs per SM.  Backward: three runs
+// of 8 take 168 registers a thread, two take 128.
+constexpr int ln_block(int tpr, int run, bool bwd) { return bwd && run == 24 && tpr <= 64 ? 384 : 256 / tpr * tpr; }
+constexpr int ln_ctas(int tpr, int run, bool bwd, int es) {
+  if (bwd) return run > 16 ? 1 : 2;
+  return (run > 24 ? 2 : es == 4 ? 3 : 4) * 256 / ln_block(tpr, run, false);
+}
 
 struct LnParams {
   const void* x;
@@ -35,7 +43,7 @@ struct LnParams {
 };
 
 // Sums over the threads of a group: a warp, some warps of a CTA (named barrier 1 + the group) or the whole CTA.
-template <int TPR, int K>
+template <int TPR, int NT, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* smem, int& phase) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
@@ -46,13 +54,13 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* smem, int& phase
     constexpr int W = TPR / 32;
     const int grp = threadIdx.x / TPR, w = (threadIdx.x % TPR) >> 5;
     // two buffers in turn: a warp may be one reduction ahead of the others, never two
-    float* buf = smem + ((phase & 1) * (kLnThreads / TPR) + grp) * (2 * W);
+    float* buf = smem + ((phase & 1) * (NT / TPR) + grp) * (2 * W);
     ++phase;
     if ((threadIdx.x & 31) == 0) {
 #pragma unroll
       for (int k = 0; k < K; ++k) buf[k * W + w] = v[k];
     }
-    if constexpr (TPR == kLnThreads) __syncthreads();
+    if constexpr (TPR == NT) __syncthreads();
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(TPR) : "memory");   // (a group's warps do the same rows)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -65,21 +73,21 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* smem, int& phase
 
 // The weights lie in shared memory as fp32, [w | b]; the columns behind E are zero.  A run of 8 is read as two halves, and the
 // threads' first halves lie side by side, then their second ones: neighbours 32 bytes apart met in the same banks (forward,
-// 65536 x 768: 41 us against FWD_US).
+// 65536 x 768: 40.7 us against 37.2).
 template <int VEC, int TPR>
 __device__ __forceinline__ int weight_at(int c) {
   if constexpr (VEC == 1) return c;
   else return ((c / (8 * TPR) * 2 + (c >> 2 & 1)) * TPR + (c >> 3) % TPR) * 4 + (c & 3);
 }
-template <int VEC, int ITER, int TPR>
+template <int VEC, int ITER, int TPR, int NT>
 __device__ __forceinline__ void stage_row(const void* a, int dtype, int E, float otherwise, float* out) {
   constexpr int C = VEC * ITER * TPR;
   if (a != nullptr && dtype == SWV_F32 && (reinterpret_cast<uintptr_t>(a) & 15) == 0) {
-    constexpr int kRuns = (C + 4 * kLnThreads - 1) / (4 * kLnThreads);
+    constexpr int kRuns = (C + 4 * NT - 1) / (4 * NT);
     float4 v[kRuns];                                         // all loads in flight together
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
-      const int c = (i * kLnThreads + threadIdx.x) * 4;
+      const int c = (i * NT + threadIdx.x) * 4;
       v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       const float* f = static_cast<const float*>(a) + c;
       if (c + 3 < E) {
@@ -92,23 +100,23 @@ __device__ __forceinline__ void stage_row(const void* a, int dtype, int E, float
     }
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
-      const int c = (i * kLnThreads + threadIdx.x) * 4;
+      const int c = (i * NT + threadIdx.x) * 4;
       if (c < C) *reinterpret_cast<float4*>(out + weight_at<VEC, TPR>(c)) = v[i];
     }
     return;
   }
-  constexpr int kRuns = (C + kLnThreads - 1) / kLnThreads;
+  constexpr int kRuns = (C + NT - 1) / NT;
 #pragma unroll 8
   for (int i = 0; i < kRuns; ++i) {
-    const int c = i * kLnThreads + threadIdx.x;
+    const int c = i * NT + threadIdx.x;
     if (c < C) out[weight_at<VEC, TPR>(c)] = c >= E ? 0.f : a != nullptr ? load_as_f32(a, dtype, c) : otherwise;
   }
 }
-template <int VEC, int ITER, int TPR>
+template <int VEC, int ITER, int TPR, int NT>
 __device__ __forceinline__ void stage_weights(const LnParams& p, float* ws, bool bias) {
   constexpr int C = VEC * ITER * TPR;
-  stage_row<VEC, ITER, TPR>(p.w, p.w_dtype, p.E, 1.f, ws);
-  if (bias) stage_row<VEC, ITER, TPR>(p.b, p.b_dtype, p.E, 0.f, ws + C);
+  stage_row<VEC, ITER, TPR, NT>(p.w, p.w_dtype, p.E, 1.f, ws);
+  if (bias) stage_row<VEC, ITER, TPR, NT>(p.b, p.b_dtype, p.E, 0.f, ws + C);
   __syncthreads();
 }
 // those of a thread's run i
@@ -125,16 +133,18 @@ __device__ __forceinline__ void load_weights(const float* ws, int i, int t, floa
 }
 
 template <typename T, typename U, int VEC, int ITER, int TPR>
-__global__ void __launch_bounds__(kLnThreads, VEC * ITER > 24 ? 2 : sizeof(T) == 4 ? 3 : 4) layer_norm_fwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__((ln_block(TPR, VEC * ITER, false)), (ln_ctas(TPR, VEC * ITER, false, sizeof(T))))
+    layer_norm_fwd_kernel(const LnParams p) {
+  constexpr int NT = ln_block(TPR, VEC * ITER, false);
   grid_wait();
   grid_release();
-  __shared__ float red[4 * (kLnThreads / 32)];
+  __shared__ float red[4 * (NT / 32)];
   extern __shared__ float ws[];
   constexpr int C = VEC * ITER * TPR;
   int phase = 0;
   const int t = threadIdx.x % TPR;
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kLnThreads / TPR);
-  int64_t row = static_cast<int64_t>(blockIdx.x) * (kLnThreads / TPR) + threadIdx.x / TPR;
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (NT / TPR);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (NT / TPR) + threadIdx.x / TPR;
   const float inv_e = 1.f / p.E;
   Raw<T, VEC> next[ITER];
   auto fetch = [&](int64_t r) {
@@ -147,7 +157,7 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 24 ? 2 : sizeof(T) ==
     }
   };
   fetch(row);
-  stage_weights<VEC, ITER, TPR>(p, ws, true);
+  stage_weights<VEC, ITER, TPR, NT>(p, ws, true);
   for (; row < p.N; row += groups) {
     float v[ITER * VEC];
 #pragma unroll
@@ -156,7 +166,7 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 24 ? 2 : sizeof(T) ==
     float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < ITER * VEC; ++i) s[0] += v[i];
-    group_sum<TPR>(s, red, phase);
+    group_sum<TPR, NT>(s, red, phase);
     const float mu = s[0] * inv_e;
     s[0] = 0.f;
 #pragma unroll
@@ -169,7 +179,7 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 24 ? 2 : sizeof(T) ==
         s[0] = fmaf(d, d, s[0]);
       }
     }
-    group_sum<TPR>(s, red, phase);
+    group_sum<TPR, NT>(s, red, phase);
     const float rstd = 1.f / sqrtf(fmaf(s[0], inv_e, p.eps));
     U* yr = static_cast<U*>(p.y) + row * p.ys;
 #pragma unroll
@@ -190,16 +200,18 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 24 ? 2 : sizeof(T) ==
 }
 
 template <typename T, typename U, int VEC, int ITER, int TPR>
-__global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_norm_bwd_kernel(const LnParams p) {
+__global__ void __launch_bounds__((ln_block(TPR, VEC * ITER, true)), (ln_ctas(TPR, VEC * ITER, true, 0)))
+    layer_norm_bwd_kernel(const LnParams p) {
+  constexpr int NT = ln_block(TPR, VEC * ITER, true);
   grid_wait();
   grid_release();
-  __shared__ float red[4 * (kLnThreads / 32)];
+  __shared__ float red[4 * (NT / 32)];
   extern __shared__ float ws[];
   constexpr int R = ITER * VEC, C = R * TPR;
   int phase = 0;
   const int t = threadIdx.x % TPR;
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * (kLnThreads / TPR);
-  int64_t row = static_cast<int64_t>(blockIdx.x) * (kLnThreads / TPR) + threadIdx.x / TPR;
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * (NT / TPR);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (NT / TPR) + threadIdx.x / TPR;
   const float inv_e = 1.f / p.E;
   float dw[R], db[R];
   constexpr bool kAhead = sizeof(T) + sizeof(U) <= 4;        // 16-bit rows: the next one is loaded under the present one's sums
@@ -226,7 +238,7 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_nor
     }
   };
   if (kAhead) fetch(row);
-  stage_weights<VEC, ITER, TPR>(p, ws, false);
+  stage_weights<VEC, ITER, TPR, NT>(p, ws, false);
   for (; row < p.N; row += groups) {
     if (!kAhead) fetch(row);
     const float mu = mu_next, rstd = rstd_next;
@@ -255,7 +267,7 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_nor
         s[1] = fmaf(gw, xh, s[1]);
       }
     }
-    group_sum<TPR>(s, red, phase);
+    group_sum<TPR, NT>(s, red, phase);
     const float m0 = s[0] * inv_e, m1 = s[1] * inv_e;
     T* dxr = static_cast<T*>(p.y) + row * p.ys;
 #pragma unroll
@@ -272,7 +284,7 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_nor
   }
   if (p.part == nullptr) return;
   float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.E;
-  if constexpr (TPR == kLnThreads) {
+  if constexpr (TPR == NT) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int c = (i / VEC * TPR + t) * VEC + i % VEC;
@@ -292,11 +304,11 @@ __global__ void __launch_bounds__(kLnThreads, VEC * ITER > 16 ? 1 : 2) layer_nor
       mine[C + c] = db[i];
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < 2 * p.E; c += kLnThreads) {
+    for (int c = threadIdx.x; c < 2 * p.E; c += NT) {
       const float* col = ws + (c < p.E ? c : C + c - p.E);
       float a = 0.f;
 #pragma unroll
-      for (int k = 0; k < kLnThreads / TPR; ++k) a += col[k * 2 * C];
+      for (int k = 0; k < NT / TPR; ++k) a += col[k * 2 * C];
       out[c] = a;
     }
   }
@@ -314,14 +326,14 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_wide_fwd_kernel(const L
     const T* xr = static_cast<const T*>(p.x) + row * p.xs;
     float s[1] = {0.f};
     for (int c = threadIdx.x; c < p.E; c += kLnThreads) s[0] += to_f32(xr[c]);
-    group_sum<kLnThreads>(s, red, phase);
+    group_sum<kLnThreads, kLnThreads>(s, red, phase);
     const float mu = s[0] * inv_e;
     s[0] = 0.f;
     for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
       const float d = to_f32(xr[c]) - mu;
       s[0] = fmaf(d, d, s[0]);
     }
-    group_sum<kLnThreads>(s, red, phase);
+    group_sum<kLnThreads, kLnThreads>(s, red, phase);
     const float rstd = 1.f / sqrtf(fmaf(s[0], inv_e, p.eps));
     U* yr = static_cast<U*>(p.y) + row * p.ys;
     for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
@@ -362,7 +374,7 @@ __global__ void __launch_bounds__(kLnThreads) layer_norm_wide_bwd_kernel(const L
         part[p.E + c] = (first ? 0.f : part[p.E + c]) + d;
       }
     }
-    group_sum<kLnThreads>(s, red, phase);
+    group_sum<kLnThreads, kLnThreads>(s, red, phase);
     const float m0 = s[0] * inv_e, m1 = s[1] * inv_e;
     T* dxr = static_cast<T*>(p.y) + row * p.ys;
     for (int c = threadIdx.x; c < p.E; c += kLnThreads) {
@@ -400,43 +412,61 @@ __global__ void __launch_bounds__(1024) layer_norm_sum_kernel(const float* part,
 }
 
 // Which kernel serves a row: runs of 8 elements where every row starts on 16 bytes and E is a multiple of 8, single
-// elements otherwise.  Forward, 16-bit rows: a warp a row up to 1024 values (65536 x 768: 41 us, two warps 51 us); fp32
-// rows, twice the registers: one run a thread (4099 x 1280: 12.6 us, two runs 15.7 us).  Backward: as many threads as
-// leave two runs (x, dy, dw and db of 16 values) to each; a warp a row with three runs spilled at two CTAs per SM (76
-// against 105 us at 65536 x 768).  Beyond 8192 values the form that reads the row again.
+// elements otherwise.  Runs of 8: few threads with several runs each, as many as the registers hold, so that few warps meet at a
+// barrier and few lanes idle behind the row's end.  Forward, 16-bit rows: a warp up to 1280 values (32768 x 1280: 30 us, four
+// warps 38, five 40), then two runs a thread (16384 x 2048: 25.5 us, one run 33); fp32 rows, twice the registers: one run a
+// thread (4099 x 1280: 11.5 us, two runs 15.7).  Backward: two runs (x, dy, dw and db of 16 values) in 128 registers, or
+// three in 168 where they fit the row better (65536 x 768: 56 us, two warps with two runs 65; 32768 x 1280: 52 us, four warps 65);
+// four runs spill (32768 x 1024: 55 us, two warps with two runs 38.5).  Beyond 8192 values the form that reads the row again.
 struct LnForm {
   int vec, tpr, iter;       // iter = 0: the form for wide rows
 };
 LnForm ln_form(int E, bool vec8, bool bwd, bool wide) {
   LnForm f;
   f.vec = vec8 ? 8 : 1;
-  if (f.vec == 8 && !bwd && wide) f.tpr = E <= 256 ? 32 : E <= 512 ? 64 : E <= 1024 ? 128 : kLnThreads;
-  else if (f.vec == 8) f.tpr = E <= (bwd ? 512 : 1024) ? 32 : E <= 1024 ? 64 : E <= 2048 ? 128 : kLnThreads;
-  else f.tpr = E <= 1024 ? 32 : E <= 4096 ? 128 : kLnThreads;
+  if (f.vec == 1) f.tpr = E <= 1024 ? 32 : E <= 4096 ? 128 : 256;
+  else if (!bwd && wide) f.tpr = std::min((E + 255) / 256 * 32, 256);
+  else f.tpr = E <= (bwd ? 768 : 1280) ? 32 : bwd && E <= 1536 ? 64 : E <= 2048 ? 128 : 256;
   const int n = (E + f.vec * f.tpr - 1) / (f.vec * f.tpr);
-  if (f.vec == 8) f.iter = n <= 4 ? n : 0;
+  if (f.vec == 8) f.iter = n <= (f.tpr == 32 ? 5 : 4) ? n : 0;
   else f.iter = n <= 8 ? 8 : n <= 32 ? 32 : 0;
   return f;
 }
 
-int ln_grid(int64_t N, int tpr, int per_sm) {
-  const int64_t rows = kLnThreads / tpr;
-  return static_cast<int>(std::min<int64_t>((N + rows - 1) / rows, static_cast<int64_t>(sm_count()) * per_sm));
+constexpr int kLnBwdCtas = 2;                     // the most of any backward form, also of the wide one
+int ln_grid(const LnForm& f, int64_t N, bool bwd, int es) {
+  const int run = f.vec * f.iter;
+  int64_t rows = 1, per_sm = bwd ? kLnBwdCtas : 4;               // the form for wide rows
+  if (f.iter > 0) {
+    rows = ln_block(f.tpr, run, bwd) / f.tpr;
+    per_sm = ln_ctas(f.tpr, run, bwd, es);
+  }
+  return static_cast<int>(std::min<int64_t>((N + rows - 1) / rows, sm_count() * per_sm));
 }
-constexpr int kLnFwdCtas = 4, kLnBwdCtas = 2;     // resident CTAs per SM
+
+template <typename T, typename U, int VEC, int ITER, int TPR, bool BWD>
+auto ln_kernel() {
+  if constexpr (BWD) return layer_norm_bwd_kernel<T, U, VEC, ITER, TPR>;
+  else return layer_norm_fwd_kernel<T, U, VEC, ITER, TPR>;
+}
 
 template <typename T, typename U, bool BWD>
 int ln_launch(const LnParams& p, const LnForm& f, int grid, cudaStream_t st) {
-#define SWV_LN(V, I, R)                                                                                      \
+#define SWV_LN(V, I, R, USED)                                                                                \
   if (f.vec == V && f.iter == I && f.tpr == R) {                                                             \
-    constexpr int kSmem = 2 * V * I * (BWD ? kLnThreads : R) * 4;                                                               \
-    auto k = BWD ? layer_norm_bwd_kernel<T, U, V, I, R> : layer_norm_fwd_kernel<T, U, V, I, R>;              \
-    if (kSmem > 40 * 1024) SWV_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)); \
-    SWV_CUDA_OK(launch_after(k, grid, kLnThreads, kSmem, st, p));                                            \
+    if constexpr (USED) {                                                                                    \
+      constexpr int kBlock = ln_block(R, V * I, BWD), kSmem = 2 * V * I * (BWD ? kBlock : R) * 4;            \
+      auto k = ln_kernel<T, U, V, I, R, BWD>();                                                              \
+      if (kSmem > 40 * 1024) SWV_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)); \
+      SWV_CUDA_OK(launch_after(k, grid, kBlock, kSmem, st, p));                                              \
+    }                                                                                                        \
   } else
-  SWV_LN(8, 1, 32) SWV_LN(8, 2, 32) SWV_LN(8, 3, 32) SWV_LN(8, 4, 32) SWV_LN(8, 1, 64) SWV_LN(8, 1, 128) SWV_LN(8, 1, kLnThreads) SWV_LN(8, 2, 64) SWV_LN(8, 2, 128) SWV_LN(8, 2, kLnThreads) SWV_LN(8, 3, kLnThreads)
-  SWV_LN(8, 4, kLnThreads)
-  SWV_LN(1, 8, 32) SWV_LN(1, 32, 32) SWV_LN(1, 32, 128) SWV_LN(1, 32, kLnThreads) {
+  constexpr bool kOne = !BWD && sizeof(T) == 4;              // one run a thread at any width
+  SWV_LN(8, 1, 32, true) SWV_LN(8, 2, 32, !kOne) SWV_LN(8, 3, 32, !kOne) SWV_LN(8, 4, 32, !kOne && !BWD) SWV_LN(8, 5, 32, !kOne && !BWD)
+  SWV_LN(8, 1, 64, kOne) SWV_LN(8, 1, 96, kOne) SWV_LN(8, 1, 128, kOne) SWV_LN(8, 1, 160, kOne) SWV_LN(8, 1, 192, kOne)
+  SWV_LN(8, 1, 224, kOne) SWV_LN(8, 1, 256, kOne) SWV_LN(8, 2, 64, BWD) SWV_LN(8, 3, 64, BWD) SWV_LN(8, 2, 128, !kOne)
+  SWV_LN(8, 2, 256, true) SWV_LN(8, 3, 256, true) SWV_LN(8, 4, 256, true)
+  SWV_LN(1, 8, 32, true) SWV_LN(1, 32, 32, true) SWV_LN(1, 32, 128, true) SWV_LN(1, 32, 256, true) {
     auto k = BWD ? layer_norm_wide_bwd_kernel<T, U> : layer_norm_wide_fwd_kernel<T, U>;
     SWV_CUDA_OK(launch_after(k, grid, kLnThreads, 0, st, p));
   }
@@ -482,7 +512,7 @@ int layer_norm_fwd_impl(const void* x, int64_t xs, int x_dtype, const void* w, i
   LnParams p{};
   p.x = x; p.w = w; p.b = b; p.y = y; p.mean = mean; p.rstd = rstd;
   p.N = N; p.xs = xs; p.ys = ys; p.E = E; p.w_dtype = w_dtype; p.b_dtype = b_dtype; p.eps = eps;
-  return ln_dispatch<false>(p, x_dtype, y_dtype, f, ln_grid(N, f.iter == 0 ? kLnThreads : f.tpr, kLnFwdCtas), st);
+  return ln_dispatch<false>(p, x_dtype, y_dtype, f, ln_grid(f, N, false, dtype_bytes(x_dtype)), st);
 }
 
 // The backward pass takes no more CTAs than this, whichever form serves it: room for their sums.
@@ -506,7 +536,7 @@ int layer_norm_bwd_impl(const void* dy, int64_t dys, int y_dtype, const void* x,
   const bool vec = E % 8 == 0 && rows_vec8(x, xs, dtype_bytes(x_dtype)) && rows_vec8(dy, dys, dtype_bytes(y_dtype)) &&
                    rows_vec8(dx, dxs, dtype_bytes(x_dtype));
   const LnForm f = ln_form(E, vec, true, false);
-  const int grid = N == 0 ? 0 : ln_grid(N, f.iter == 0 ? kLnThreads : f.tpr, kLnBwdCtas);
+  const int grid = N == 0 ? 0 : ln_grid(f, N, true, 0);
   if (sums && N > 0) {
     size_t need = static_cast<size_t>(grid) * 2 * E * sizeof(float);
     if (!workspace) return SWV_ERR_NULL;

@@ -657,3 +657,11 @@ def test_attention_row_that_sees_no_key_is_zero_beside_nan_values(swv, D):
     o, lse = swv.packed_attention(q, k, bad, plan, return_lse=True)
     assert not bool(o[:10].any()) and bool((lse[:, :10] == -math.inf).all())
     assert bool(torch.isnan(o[10:40]).all()) and torch.equal(o[40:], clean[40:])
+
+
+@pytest.mark.parametrize("N,E,dt", [(2500, 1280, "bfloat16"), (700, 1288, "float16"), (300, 1536, "bfloat16"), (300, 1544, "float32"),
+                                    (40, 2048, "bfloat16"), (40, 2056, "float16"), (50, 1800, "float32"), (100, 600, "float32"),
+                                    (5000, 512, "bfloat16"), (3000, 520, "float16")])
+def test_layer_norm_widths(swv, N, E, dt):
+    """Rows on both sides of the widths at which another number of threads serves a row."""
+    test_layer_norm(swv, N, E, dt, 0.4)
