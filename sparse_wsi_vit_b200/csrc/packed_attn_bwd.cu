@@ -4,7 +4,8 @@
 //   dS_ij = P_ij (dO_i . v_j - delta_i)
 //   dV_j = sum_i P_ij dO_i      dK_j = scale sum_i dS_ij q_i      dQ_i = scale sum_j dS_ij k_j
 //
-// Three launches: delta (and lse in powers of two) per row; the keys' side (dK, dV); the queries' side (dQ).  Scores and
+// Three launches: delta (and lse in powers of two) per row; the keys' side (dK, dV); the queries' side (dQ), which starts under
+// the end of the keys' side (they share nothing but delta).  Scores and
 // probabilities are formed again in both: two sums that each stay in one CTA's TMEM, so every gradient is
 // written once, in its own type, and there are no atomics -- the same bits every time.  The rows of a tile are packed from
 // the group's heads as in the forward pass, which makes the sum over a group's heads part of the product.
@@ -519,40 +520,55 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (MODE == kDq && blockIdx.x == gridDim.x - 1) grid_wait();   // the grid's end stands for the keys' side's too
 }
 
-// -delta = -dO . O per row, and -lse in powers of two; half a warp a row.
+// -delta = -dO . O per row, and -lse in powers of two.  L lanes a row (8 channels each), four rows a thread in flight.  Bound: HBM.
+constexpr int kDeltaRows = 4;
+template <int L>
 __global__ void __launch_bounds__(256) packed_attn_delta_kernel(const __nv_bfloat16* o, int64_t os_t, int64_t os_h,
                                                                 const __nv_bfloat16* g, int64_t gs_t, int64_t gs_h,
-                                                                const float* lse, float2* stats, int64_t rows, int Tq,
-                                                                int tokens, int group, int d) {
+                                                                const float* lse, float2* stats, int Tq, int tokens,
+                                                                int group, int d) {
   grid_wait();
   grid_release();
-  const int sub = threadIdx.x & 15;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  if (r >= rows) return;                                       // (half warps leave together: the sums below stay inside one)
+  constexpr int kAtOnce = 256 / L;                             // rows a CTA has in flight in each step
+  const int sub = threadIdx.x % L, kvh = blockIdx.y, c = sub * 8;
   // rows in the order of the tiles: [kv head][token][head of the group]
-  const int hg = static_cast<int>(r % group);
-  const int64_t t = (r / group) % tokens;
-  const int kvh = static_cast<int>(r / group / tokens);
-  const int head = kvh * group + hg;
-  const int c = sub * 8;
-  float a = 0.f;
-  if (c < d) {
-    const uint4 x = *reinterpret_cast<const uint4*>(o + t * os_t + head * os_h + c);
-    const uint4 y = *reinterpret_cast<const uint4*>(g + t * gs_t + head * gs_h + c);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kAtOnce * kDeltaRows);
+  const int64_t t0 = first / group;
+  const int rest = static_cast<int>(first - t0 * group) + threadIdx.x / L;
+  uint4 x[kDeltaRows], y[kDeltaRows];
+  float l[kDeltaRows];
+  int64_t t[kDeltaRows];
+  int hg[kDeltaRows];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a = fmaf(__uint_as_float(xs[i] << 16), __uint_as_float(ys[i] << 16), a);
-      a = fmaf(__uint_as_float(xs[i] & 0xffff0000u), __uint_as_float(ys[i] & 0xffff0000u), a);
+  for (int i = 0; i < kDeltaRows; ++i) {
+    const int j = rest + i * kAtOnce;
+    t[i] = t0 + j / group;
+    hg[i] = j % group;
+    const int head = kvh * group + hg[i];
+    x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
+    l[i] = 0.f;
+    if (t[i] >= tokens) continue;
+    if (c < d) {
+      x[i] = *reinterpret_cast<const uint4*>(o + t[i] * os_t + head * os_h + c);
+      y[i] = *reinterpret_cast<const uint4*>(g + t[i] * gs_t + head * gs_h + c);
     }
+    if (sub == 0) l[i] = lse[static_cast<int64_t>(head) * Tq + t[i]];
   }
-  const uint32_t mask = 0xffffu << (threadIdx.x & 16);
 #pragma unroll
-  for (int off = 8; off > 0; off >>= 1) a += __shfl_xor_sync(mask, a, off);
-  if (sub == 0) {
-    const float l = lse[static_cast<int64_t>(head) * Tq + t];
+  for (int i = 0; i < kDeltaRows; ++i) {
+    const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+    float a = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a = fmaf(__uint_as_float(xs[k] << 16), __uint_as_float(ys[k] << 16), a);
+      a = fmaf(__uint_as_float(xs[k] & 0xffff0000u), __uint_as_float(ys[k] & 0xffff0000u), a);
+    }
+#pragma unroll
+    for (int off = L / 2; off > 0; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off);
     const float inf = __int_as_float(0x7f800000);
-    stats[(static_cast<int64_t>(kvh) * Tq + t) * group + hg] = make_float2(l == -inf ? -inf : l * -1.4426950408889634f, -a);
+    if (sub == 0 && t[i] < tokens)
+      stats[(static_cast<int64_t>(kvh) * Tq + t[i]) * group + hg[i]] =
+          make_float2(l[i] == -inf ? -inf : l[i] * -1.4426950408889634f, -a);
   }
 }
 
@@ -695,10 +711,13 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   float2* stats = static_cast<float2*>(workspace);
   p.stats = stats;
   if (h.Tq > 0) {
-    const int64_t rows = static_cast<int64_t>(h.H) * h.Tq;
-    SWV_CUDA_OK(launch_after(packed_attn_delta_kernel, static_cast<unsigned>((rows + 15) / 16), 256, 0, st,
-                             static_cast<const __nv_bfloat16*>(o), os[0], os[1], static_cast<const __nv_bfloat16*>(d_out),
-                             gs[0], gs[1], lse, stats, rows, static_cast<int>(Tq), h.Tq, p.group, D));
+    const int lanes = D <= 64 ? 8 : 16, per_cta = 256 / lanes * kDeltaRows;
+    const int64_t ctas = (static_cast<int64_t>(h.Tq) * p.group + per_cta - 1) / per_cta;
+    if (ctas > 0x7fffffff) return SWV_ERR_UNSUPPORTED;
+    SWV_CUDA_OK(launch_after(lanes == 8 ? packed_attn_delta_kernel<8> : packed_attn_delta_kernel<16>,
+                             dim3(static_cast<unsigned>(ctas), h.Hkv), 256, 0, st, static_cast<const __nv_bfloat16*>(o), os[0],
+                             os[1], static_cast<const __nv_bfloat16*>(d_out), gs[0], gs[1], lse, stats, static_cast<int>(Tq),
+                             h.Tq, p.group, D));
   }
   CUtensorMap tq, tg, tk, tv;
   if ((rc = packed_tmap(&tq, q, qs, Tq, h.Hkv, p.group, D, p.tok)) != SWV_OK) return rc;
