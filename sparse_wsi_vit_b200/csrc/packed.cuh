@@ -47,6 +47,18 @@ struct PackedJoin {                       // the slots [slot, slot + parts) are 
   int t0, n, slot, parts;
 };
 
+// Loads of what an earlier kernel of the stream may have written, behind grid_wait: from L2, and not moved ahead of the wait.
+__device__ __forceinline__ float2 load_written(const float2* p) {
+  float2 v;
+  asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ int4 load_written(const int4* p) {
+  int4 v;
+  asm volatile("ld.global.cg.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // Which unit and key head a CTA serves.  The units of `at_once` heads go together, the longest units of all of them
 // first: the launch ends with short ones, and what the CTAs in flight read stays in L2.
 __device__ __forceinline__ PackedUnit packed_unit(const PackedUnit* units, int n_units, int heads, int at_once, int& head) {
@@ -56,8 +68,8 @@ __device__ __forceinline__ PackedUnit packed_unit(const PackedUnit* units, int n
   head = g * at_once + r % here;
   union { int4 v[2]; PackedUnit u; } x;
   const int4* src = reinterpret_cast<const int4*>(units + r / here);
-  x.v[0] = __ldg(src);
-  x.v[1] = __ldg(src + 1);
+  x.v[0] = load_written(src);
+  x.v[1] = load_written(src + 1);
   return x.u;
 }
 // Heads whose two streamed tensors (`rows` rows of the longest sequence) fill half of the L2.

@@ -116,6 +116,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tma_prefetch_desc(&tm_a);
     tma_prefetch_desc(&tm_b);
   }
+  if (MODE == kDkv || p.wait_first) grid_wait();
+  int kvh;
+  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
   if (threadIdx.x == 0) {
     mbar_init(&ctl->lane_full, 1);
     for (int s = 0; s < 4; ++s) {
@@ -144,9 +147,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
   }
-  if (MODE == kDkv || p.wait_first) grid_wait();
-  int kvh;
-  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
   const int n = u.b1 - u.b0;
   const int per = MODE == kDkv ? p.tok * p.group : kTile;      // streamed rows a tile
   const int step = MODE == kDkv ? p.tok : kTile;               // streamed tokens a tile
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = i * 32 + lane;
-          f[i] = r < rows ? __ldg(src + r) : make_float2(0.f, 0.f);
+          f[i] = r < rows ? load_written(src + r) : make_float2(0.f, 0.f);
         }
         bool ok = j < 2 || wait(&ctl->stat_empty[j & 1], ((j >> 1) & 1) ^ 1, kDevWaitAccEmpty);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const bool row_ok = row < rows;
     const int tk = MODE == kDkv ? row : row_token(row, p.group_inv);         // token of the lane side
     if (MODE == kDq && row_ok) {
-      const float2 f = __ldcg(p.stats + (static_cast<int64_t>(kvh) * p.Tq + u.t0) * p.group + row);
+      const float2 f = load_written(p.stats + (static_cast<int64_t>(kvh) * p.Tq + u.t0) * p.group + row);
       neg_lse = f.x;
       neg_delta = f.y;
       limit = min(u.len, u.off + tk + 1) - u.b0 * kTile;
