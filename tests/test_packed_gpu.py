@@ -665,3 +665,44 @@ def test_attention_row_that_sees_no_key_is_zero_beside_nan_values(swv, D):
 def test_layer_norm_widths(swv, N, E, dt):
     """Rows on both sides of the widths at which another number of threads serves a row."""
     test_layer_norm(swv, N, E, dt, 0.4)
+
+
+def test_calls_that_follow_one_another(swv):
+    """Thirty training passes without a wait between them, each on inputs that the one before has just read, written into
+    the same memory: the launches start early, their reads and writes do not.  The bits are those of passes run alone."""
+    ql, kl, H, Hk, D, E = [40, 300, 7], [900, 20, 64], 4, 2, 64, 256
+    plan, rope = swv.PackedPlan(ql, kl, heads=H, kv_heads=Hk), swv.RopeAxes(D, (16, 16))
+    g = torch.Generator(device="cuda").manual_seed(40)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+    rounds = [(r(sum(ql), E), r(sum(kl), Hk, D), r(sum(kl), Hk, D), r(sum(ql), H, D)) for _ in range(30)]
+    buf = [torch.zeros_like(t) for t in rounds[0]]
+    pos = torch.randint(0, 500, (sum(ql), 2), device="cuda")
+    w, b = torch.randn(E, device="cuda", generator=g), torch.randn(E, device="cuda", generator=g)
+
+    def run(data):
+        for t, new in zip(buf, data):
+            t.copy_(new)
+        x, k, v = (t.detach().requires_grad_() for t in buf[:3])
+        wl, bl = w.requires_grad_(), b.requires_grad_()
+        q = swv.rope_axes(swv.layer_norm(x, wl, bl).view(-1, H, D), pos, rope)
+        o = swv.packed_attention(q, k, v, plan)
+        grads = torch.autograd.grad(o, (x, k, v, wl, bl), buf[3])
+        with torch.no_grad():
+            swv.rope_axes(buf[3], pos, rope, out=buf[3])
+        return (o.detach(), buf[3].clone()) + grads
+
+    alone = []
+    for data in rounds:
+        alone.append(run(data))
+        torch.cuda.synchronize()
+    for _ in range(3):
+        chained = [run(data) for data in rounds]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for x, y in zip(alone, chained) for a, c in zip(x, y))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [run(data) for data in rounds[:6]]
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for x, y in zip(alone, captured) for a, c in zip(x, y))
