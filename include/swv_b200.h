@@ -443,6 +443,7 @@ int swv_rope_axes_apply(const void* x, const int64_t x_strides[3], void* y, cons
  *   D a multiple of 8 up to 128; Tq, Tk at least the plan's tokens: rows behind them are neither read nor written;
  *   lse (H,Tq) f32, natural logarithm of each row's sum of exponentials, NULL if not wanted (the backward pass
  *   takes it); scale in [2^-60, 2^60]; `workspace` of swv_packed_attn_bytes() / swv_packed_attn_bwd_bytes(), 16-byte aligned.
+ * Outputs share no memory with inputs (the two sides of the backward pass run side by side).
  * Inside one sequence a NaN or an infinity in a value row can reach earlier (causally masked) queries whose key tiles
  * hold that row; other sequences it never reaches. */
 int swv_packed_plan(int n_seq, const int64_t* q_lens_host, const int64_t* k_lens_host, int H, int Hkv, int causal,
