@@ -59,11 +59,12 @@ __device__ __forceinline__ int4 load_written(const int4* p) {
   return v;
 }
 
-// Which unit and key head a CTA serves.  The units of `at_once` heads go together, the longest units of all of them
+// Which unit and key head CTA `block` serves.  The units of `at_once` heads go together, the longest units of all of them
 // first: the launch ends with short ones, and what the CTAs in flight read stays in L2.
-__device__ __forceinline__ PackedUnit packed_unit(const PackedUnit* units, int n_units, int heads, int at_once, int& head) {
-  const int g = blockIdx.x / (n_units * at_once);
-  const int r = blockIdx.x - g * n_units * at_once;
+__device__ __forceinline__ PackedUnit packed_unit(const PackedUnit* units, int n_units, int heads, int at_once, int block,
+                                                   int& head) {
+  const int g = block / (n_units * at_once);
+  const int r = block - g * n_units * at_once;
   const int here = min(at_once, heads - g * at_once);
   head = g * at_once + r % here;
   union { int4 v[2]; PackedUnit u; } x;

@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   }
   grid_wait();
   int kvh;
-  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
+  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, blockIdx.x, kvh);
   const int n = u.b1 - u.b0;
   // tokens and key blocks of tile t (its last token sees the most keys)
   auto tokens = [&](int t) { return min(p.tok, u.n - t * p.tok); };

@@ -4,13 +4,14 @@
 //   dS_ij = P_ij (dO_i . v_j - delta_i)
 //   dV_j = sum_i P_ij dO_i      dK_j = scale sum_i dS_ij q_i      dQ_i = scale sum_j dS_ij k_j
 //
-// Three launches: delta (and lse in powers of two) per row; the keys' side (dK, dV); the queries' side (dQ), which starts under
-// the end of the keys' side (they share nothing but delta).  Scores and
+// Two launches: delta (and lse in powers of two) per row; then one grid whose first CTAs are the keys' side (dK, dV) and whose
+// others are the queries' side (dQ): they read the same inputs, write nothing in common, and the queries' side fills the SMs
+// that the keys' side leaves free.  Scores and
 // probabilities are formed again in both: two sums that each stay in one CTA's TMEM, so every gradient is
 // written once, in its own type, and there are no atomics -- the same bits every time.  The rows of a tile are packed from
 // the group's heads as in the forward pass, which makes the sum over a group's heads part of the product.
 //
-// One kernel for both sides.  The lane side (128 rows) stays in shared memory, the streamed side passes through two rings:
+// One scheme for both sides.  The lane side (128 rows) stays in shared memory, the streamed side passes through two rings:
 //   kDkv : lanes = keys;    streamed: Q (ring A), dO (ring B)     S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
 //   kDq  : lanes = queries; streamed: K (ring A), V (ring B)      S = Q K^T,   dP = dO V^T,   dQ += dS K
 // warp 0: TMA producer; warp 1: issues S and dP; warp 2: lse and delta of the streamed rows (kDkv); warp 3: issues the
@@ -53,7 +54,6 @@ struct PackedBwdParams {
   float scale, scale_log2;
   float* part;                  // [slot][Hkv][128][D (kDq) or 2 D (kDkv: dV, dK)] sums of divided units, before the scale
   int* status;
-  int wait_first;               // kDq: not launched behind the keys' side
 };
 
 template <int D, int MODE>
@@ -98,11 +98,10 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int first, int thread, 
     for (int i = first * 8 + thread; i < kTile * 8; i += threads) sts128(tile + c * (kTile * 128) + i * 16, 0u, 0u, 0u, 0u);
 }
 
+// What CTA `block` of a side does; everything that earlier kernels wrote is there.
 template <int D, int MODE>
-__global__ void __launch_bounds__(kBwdThreads, 1)
-    packed_attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_l1, const __grid_constant__ CUtensorMap tm_l2,
-                           const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                           const PackedBwdParams p) {
+__device__ __forceinline__ void bwd_side(const CUtensorMap& tm_l1, const CUtensorMap& tm_l2, const CUtensorMap& tm_a,
+                                         const CUtensorMap& tm_b, const PackedBwdParams& p, int block) {
   using Cfg = BwdCfg<D, MODE>;
   constexpr int NA = Cfg::kA, NB = Cfg::kB, TB = Cfg::kTileBytes;
   constexpr uint32_t kIdescS = make_idesc(/*bf16*/ 1, kTile, kTile, 0, 0);
@@ -114,15 +113,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   BwdCtl* ctl = reinterpret_cast<BwdCtl*>(smem + Cfg::kOffCtl);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {                            // (fetched while the barriers are made)
-    tma_prefetch_desc(&tm_l1);
-    tma_prefetch_desc(&tm_l2);
-    tma_prefetch_desc(&tm_a);
-    tma_prefetch_desc(&tm_b);
-  }
-  if (MODE == kDkv || p.wait_first) grid_wait();
   int kvh;
-  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, kvh);
+  const PackedUnit u = packed_unit(p.units, p.n_units, p.Hkv, p.heads_at_once, block, kvh);
   if (threadIdx.x == 0) {
     mbar_init(&ctl->lane_full, 1);
     for (int s = 0; s < 4; ++s) {
@@ -521,7 +513,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     __syncwarp();
     tmem_dealloc(tmem_base, 512);
   }
-  if (MODE == kDq && blockIdx.x == gridDim.x - 1) grid_wait();   // the grid's end stands for the keys' side's too
+}
+
+template <int D>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    packed_attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_g,
+                           const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                           const PackedBwdParams keys, const PackedBwdParams queries) {
+  if (threadIdx.x == 0) {                            // (fetched during the wait)
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_g);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  grid_wait();                                       // of every CTA: both sides read delta, q, k, v and dO
+  const int first = keys.n_units * keys.Hkv;
+  if (static_cast<int>(blockIdx.x) < first) bwd_side<D, kDkv>(tm_k, tm_v, tm_q, tm_g, keys, blockIdx.x);
+  else bwd_side<D, kDq>(tm_q, tm_g, tm_k, tm_v, queries, blockIdx.x - first);
 }
 
 // -delta = -dO . O per row, and -lse in powers of two.  L lanes a row (8 channels each), four rows a thread in flight.  Bound: HBM.
@@ -620,17 +628,6 @@ __global__ void __launch_bounds__(256) packed_attn_bwd_join_kernel(const PackedJ
 }
 
 template <int D, int MODE>
-int launch_bwd(const CUtensorMap& l1, const CUtensorMap& l2, const CUtensorMap& a, const CUtensorMap& b,
-               const PackedBwdParams& p, cudaStream_t st) {
-  if (p.n_units == 0) return SWV_OK;
-  static std::atomic<uint64_t> prepared{0};
-  const int rc = prepare_kernel(packed_attn_bwd_kernel<D, MODE>, prepared, kBwdThreads, kBwdRegs, bwd_smem<D, MODE>());
-  if (rc != SWV_OK) return rc;
-  SWV_CUDA_OK(launch_after(packed_attn_bwd_kernel<D, MODE>, static_cast<unsigned>(p.n_units) * p.Hkv, kBwdThreads,
-                           bwd_smem<D, MODE>(), st, l1, l2, a, b, p));
-  return SWV_OK;
-}
-template <int D, int MODE>
 int launch_join(const PackedBwdParams& p, const int32_t* joins, int n_join, cudaStream_t st) {
   if (n_join > 0)
     SWV_CUDA_OK(launch_after(packed_attn_bwd_join_kernel<D, MODE>, dim3(n_join, p.Hkv, 16), 256, 0, st,
@@ -641,9 +638,13 @@ template <int D>
 int launch_sides(const CUtensorMap& tq, const CUtensorMap& tg, const CUtensorMap& tk, const CUtensorMap& tv,
                  const PackedBwdParams& keys, const PackedBwdParams& queries, const PackedHeader& h, const int32_t* plan,
                  cudaStream_t st) {
-  int rc = launch_bwd<D, kDkv>(tk, tv, tq, tg, keys, st);
-  if (rc == SWV_OK) rc = launch_bwd<D, kDq>(tq, tg, tk, tv, queries, st);
-  if (rc == SWV_OK) rc = launch_join<D, kDkv>(keys, plan + h.dkv_join_off, h.n_dkv_join, st);
+  static std::atomic<uint64_t> prepared{0};
+  constexpr size_t kSmem = std::max(bwd_smem<D, kDkv>(), bwd_smem<D, kDq>());
+  int rc = prepare_kernel(packed_attn_bwd_kernel<D>, prepared, kBwdThreads, kBwdRegs, kSmem);
+  if (rc != SWV_OK) return rc;
+  SWV_CUDA_OK(launch_after(packed_attn_bwd_kernel<D>, static_cast<unsigned>(h.n_dkv + h.n_dq) * h.Hkv, kBwdThreads, kSmem, st, tq,
+                           tg, tk, tv, keys, queries));
+  rc = launch_join<D, kDkv>(keys, plan + h.dkv_join_off, h.n_dkv_join, st);
   if (rc == SWV_OK) rc = launch_join<D, kDq>(queries, plan + h.dq_join_off, h.n_dq_join, st);
   return rc;
 }
@@ -699,7 +700,7 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   if ((h.Tq > 0 && !packed_aligned(dq, dqs, 2)) ||
       (h.Tk > 0 && (!packed_aligned(dk, dks, 2) || !packed_aligned(dv, dvs, 2))))
     return SWV_ERR_ALIGN;
-  if (static_cast<int64_t>(std::max(h.n_dq, h.n_dkv)) * h.Hkv > 0x7fffffff || h.Hkv > 65535) return SWV_ERR_UNSUPPORTED;
+  if ((static_cast<int64_t>(h.n_dq) + h.n_dkv) * h.Hkv > 0x7fffffff || h.Hkv > 65535) return SWV_ERR_UNSUPPORTED;
   const BwdSizes sz = bwd_sizes(h, h.Tq == 0 ? 0 : Tq, D);
   if (!workspace && sz.stats + sz.dq + sz.dkv > 0) return SWV_ERR_NULL;
   if (workspace_bytes < sz.stats + sz.dq + sz.dkv) return SWV_ERR_WORKSPACE;
@@ -743,7 +744,6 @@ int packed_attn_bwd_impl(const void* d_out, const int64_t* gs, const void* q, co
   b.heads_at_once = packed_heads_at_once(h.Hkv, h.longest_k, D);
   b.g1 = dq; b.g1_t = dqs[0]; b.g1_h = dqs[1];
   b.part = reinterpret_cast<float*>(w);
-  b.wait_first = a.n_units == 0;
   return D <= 64 ? launch_sides<64>(tq, tg, tk, tv, a, b, h, plan, st) : launch_sides<128>(tq, tg, tk, tv, a, b, h, plan, st);
 }
 

@@ -53,8 +53,8 @@ int64_t total(const Work& w, int heads) {
   return sum * heads;
 }
 
-// divides the units (all of `heads` heads each) and sorts them; `behind`: the work of the next launch, which fills the SMs that they
-// leave free, so that they need not end together (keys' side of 8192 causal tokens, 16 heads of 128 sharing two key heads:
+// divides the units (all of `heads` heads each) and sorts them; `behind`: the work of the CTAs behind them in the grid, which fill the SMs
+// that they leave free, so that they need not end together (keys' side of 8192 causal tokens, 16 heads of 128 sharing two key heads:
 // 128 instead of 430 partial sums, training pass 1035 -> 1005 us)
 void divide(Work& w, int heads, int sms, int64_t behind = 0) {
   int longest = 0;
@@ -156,7 +156,7 @@ void build(int n_seq, const int64_t* ql, const int64_t* kl, int H, int Hkv, int 
   }
   divide(fwd, Hkv, sms);
   divide(dq, Hkv, sms);
-  divide(dkv, Hkv, sms, total(dq, Hkv));                      // (the queries' side is launched behind it)
+  divide(dkv, Hkv, sms, total(dq, Hkv));                      // (the queries' side follows in the same grid)
   PackedHeader h{};
   h.magic = kPlanMagic;
   h.n_seq = n_seq; h.H = H; h.Hkv = Hkv; h.causal = causal; h.Tq = q0; h.Tk = k0;
