@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const uint32_t p_col = tmem_base + lane_off + Cfg::kColP + t * 64;
     const uint32_t o_col = tmem_base + lane_off + Cfg::kColO + t * D;
     const float sc = p.scale_log2;
-    const float ninf = -__int_as_float(0x7f800000);
+    const float ninf = -__int_as_float(0x7f800000), nan = __int_as_float(0x7fc00000);
     float m_used = ninf;
     float l = 0.f;
     bool ok = true;
@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             }
           }
         }
-        // A row that sees no key has probabilities of zero; one whose scores are all -inf comes out NaN (-inf + inf).
-        const float neg_m = limit > 0 ? -m_used : 0.f;
+        // Scores of -inf have probability zero, also where the row has met nothing else yet (-inf + inf would be NaN).
+        const float neg_m = m_used == ninf ? 0.f : -m_used;
         float l0 = 0.f, l1 = 0.f;
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
@@ -407,9 +407,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             *reinterpret_cast<uint4*>(p.part_o + r * D + c * 16 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       } else {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        // A row that sees no key is zero (lse -inf), one whose scores are all -inf is NaN, as 0 / 0 (an undivided unit
+        // starts at its sequence's first key, so `limit` counts all that the row sees).
+        const bool none = limit <= 0;
+        const float inv = none ? 0.f : l == 0.f ? nan : 1.f / l;
         if (row_ok && p.lse != nullptr)
-          p.lse[static_cast<int64_t>(head) * p.Tq + token] = l == 0.f ? ninf : (m_used + log2f(l)) * 0.6931471805599453f;
+          p.lse[static_cast<int64_t>(head) * p.Tq + token] =
+              none ? ninf : l == 0.f ? nan : (m_used + log2f(l)) * 0.6931471805599453f;
         // (the tile's Q is no longer needed: its last scores are done)
         const uint32_t stage = smem_u32(smem + t * Cfg::kTileBytes);
 #pragma unroll 1
@@ -422,10 +426,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0u;
           }
-          if (__any_sync(0xffffffffu, l == 0.f)) {             // a row that sees no key is zero, also where 0 x v is NaN
+          if (__any_sync(0xffffffffu, none)) {                 // (also where 0 x v is NaN)
             KEEP_BRANCH();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0u : o[i];
+            for (int i = 0; i < 32; ++i) o[i] = none ? 0u : o[i];
           }
           stage_columns<D, 32>(stage, row, c, o, inv);
         }
@@ -452,6 +456,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 
 // Joins the sums of divided units, one warp per row: o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.  The parts'
 // (m, l) lie in the lanes, 32 parts at a time, their rows are added up in the parts' order with eight loads in flight.
+// Every row of a divided unit sees a key (the unit has more than two blocks, its 256 tokens at most follow each other), so one without
+// any weight has scores of -inf alone: NaN.
 template <int D>
 __global__ void __launch_bounds__(256) packed_attn_join_kernel(const PackedJoin* joins, const PackedFwdParams p) {
   constexpr int V = D / 32;                                    // channels a lane
@@ -494,9 +500,9 @@ __global__ void __launch_bounds__(256) packed_attn_join_kernel(const PackedJoin*
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     const int head = kvh * p.group + i % p.group;
     const int64_t token = jn.t0 + i / p.group;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? __int_as_float(0x7fc00000) : 1.f / l;
     if (lane == 0 && p.lse != nullptr)
-      p.lse[static_cast<int64_t>(head) * p.Tq + token] = l == 0.f ? ninf : (m + log2f(l)) * 0.6931471805599453f;
+      p.lse[static_cast<int64_t>(head) * p.Tq + token] = l == 0.f ? inv : (m + log2f(l)) * 0.6931471805599453f;
     if (lane * V >= p.d) continue;                             // (d is a multiple of 8)
     uint32_t w[V / 2];
 #pragma unroll

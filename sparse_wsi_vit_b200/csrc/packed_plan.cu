@@ -5,7 +5,8 @@
 // sorted by their work, the longest first, so that the last CTAs of a launch are the short ones.
 //
 // Where the units are few, long ones are divided: how often is found by laying candidates out over the SMs the way
-// the hardware does (the next unit to the SM that is free first) and taking the one that ends first.  A unit costs its
+// the hardware does (the next unit to the SM that is free first) and taking the one that ends first.  (Only units of three blocks
+// and more are divided: the forward join relies on it.)  A unit costs its
 // blocks and two more for its start and end, a divided one a further block to leave its sums and read them back; the
 // join launch costs three.
 #include <algorithm>

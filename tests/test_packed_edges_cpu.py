@@ -44,3 +44,14 @@ def test_every_kernel_that_starts_early_waits_in_every_thread():
             assert waits[0] < body.find("grid_release()") or "grid_release()" not in body, f"{f}: {name}"
             seen += 1
     assert seen >= 10
+
+
+@pytest.mark.parametrize("ql,kl,H,Hkv", [([300], [260], 1, 1), ([700, 3], [650, 900], 2, 1), ([2, 256], [4000, 400], 16, 2),
+                                         ([1000], [3000], 8, 1), ([256], [384], 4, 4), ([2048], [1800], 1, 1)])
+def test_every_row_of_a_divided_unit_sees_a_key(swv, ql, kl, H, Hkv):
+    """The join of a divided unit takes a row without any weight for one whose scores are all -inf."""
+    plan = swv.PackedPlan(ql, kl, heads=H, kv_heads=Hkv, causal=True, device="cpu")
+    w = plan._host
+    units = w[w[8]:w[8] + 8 * w[9]].reshape(-1, 8)
+    for t0, n, s0, ln, off, b0, b1, slot in units.tolist():
+        assert slot < 0 or min(ln, off + 1) > 0

@@ -1,0 +1,72 @@
+"""Packed operators on a B200 at the edges of what they take: scores of -inf, copies of handles, buffers inside an arena, derivatives
+that the kernels do not have.  Bounds and references are those of the operators' other tests."""
+import math
+
+import pytest
+import torch
+
+from .test_packed_gpu import _close, reference
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def swv():
+    import sparse_wsi_vit_b200 as m
+    yield m
+    m.check_status(torch.device("cuda:0"))
+
+
+def _inputs(lq, lk, H, Hk, D, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+    return r(lq, H, D), r(lk, Hk, D), r(lk, Hk, D), r(lq, H, D)
+
+
+@pytest.mark.parametrize("low", [-math.inf, -3e38])
+@pytest.mark.parametrize("lq,lk,lead,D", [(40, 500, 128, 64), (300, 1000, 300, 128), (2, 6007, 128, 64), (2, 6007, 300, 128),
+                                          (1, 9000, 4111, 64), (3, 300, 299, 64)])
+def test_attention_leading_keys_of_probability_zero(swv, low, lq, lk, lead, D):
+    """Whole key blocks, and whole parts of divided units, whose scores are all -inf ahead of finite ones: the result is that of
+    the finite keys alone.  Channel 0 of the queries is 8, of the leading keys -inf or so low that the product passes the
+    range (then every gradient exists: zero for those keys)."""
+    q, k, v, do = _inputs(lq, lk, 4, 2, D, lead)
+    q[:, :, 0], k[:, :, 0] = 8, 0
+    k[:lead, :, 0] = low
+    plan = swv.PackedPlan([lq], [lk], heads=4, kv_heads=2)
+    ref = reference(q, k[lead:], v[lead:], do, [lq], [lk - lead], False)
+    o, lse = swv.packed_attention(q, k, v, plan, return_lse=True)
+    _close(o, *ref["o"], "o")
+    _close(lse, *ref["lse"], "lse")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(swv.packed_attention(*leaves, plan), leaves, do)
+    for name, got in (("dk", dk), ("dv", dv)):
+        assert not bool(got[:lead].any())
+        _close(got[lead:], *ref[name], name)
+    if low == -math.inf:
+        assert bool(torch.isnan(dq[:, :, 0]).all())               # 0 x inf, as the formula has it
+    else:
+        _close(dq, *ref["dq"], "dq")
+
+
+def test_attention_causal_leading_keys_of_probability_zero(swv):
+    """Causal rows that see the leading keys alone are NaN, the ones behind them those of the finite keys."""
+    n, lead = 700, 300
+    q, k, v, do = _inputs(n, n, 2, 2, 64, 5)
+    q[:, :, 0], k[:, :, 0] = 8, 0
+    k[:lead, :, 0] = -math.inf
+    o, lse = swv.packed_attention(q, k, v, swv.PackedPlan([n], heads=2, causal=True), return_lse=True)
+    ref = reference(q[lead:], k[lead:], v[lead:], do[lead:], [n - lead], [n - lead], True)
+    assert bool(torch.isnan(o[:lead]).all()) and bool(torch.isnan(lse[:, :lead]).all())
+    _close(o[lead:], *ref["o"], "o")
+    _close(lse[:, lead:], *ref["lse"], "lse")
+
+
+@pytest.mark.parametrize("lq,lk", [(2, 6007), (300, 400)])
+def test_attention_rows_of_infinite_scores_alone_are_nan(swv, lq, lk):
+    """Divided and undivided: all scores -inf is 0 / 0, also where the values are finite."""
+    q, k, v, _ = _inputs(lq, lk, 2, 1, 64, 6)
+    q[:, :, 0] = 1
+    k[:, :, 0] = -math.inf
+    o, lse = swv.packed_attention(q, k, v, swv.PackedPlan([lq], [lk], heads=2, kv_heads=1), return_lse=True)
+    assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
