@@ -207,7 +207,18 @@ class RopeAxes:
         power = [(sum(sections[:a]) + i) / R if ladder == "head" else i / n for a, n in enumerate(sections) for i in range(n)]
         self._axis = np.repeat(np.arange(len(sections)), sections).astype(np.uint8)
         self._freq = np.asarray(scales)[self._axis] * np.float64(theta) ** -np.asarray(power, dtype=np.float64)
-        self._call = (self._freq.ctypes.data, self._axis.ctypes.data, R, len(sections), int(self.halves))
+        self._bind()
+
+    def _bind(self):
+        """The library's arguments: addresses of this object's own arrays."""
+        self._call = (self._freq.ctypes.data, self._axis.ctypes.data, self.pairs, len(self.sections), int(self.halves))
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_call"}
+
+    def __setstate__(self, state):                        # (a copied or unpickled object has arrays of its own)
+        self.__dict__.update(state)
+        self._bind()
 
 
 def _rope_apply(x, positions, rope, inverse, out=None):
@@ -291,8 +302,7 @@ class PackedPlan:
             raise SwvError(f"{len(ql)} query lengths and {len(kl)} key lengths")
         self.heads, self.kv_heads, self.causal = int(heads), int(heads if kv_heads is None else kv_heads), bool(causal)
         device = torch.device(device)
-        if device.type == "cuda" and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            raise SwvError("make the plan before the capture: its tables are copied from the host")
+        self._not_captured(device)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
         self.q_tokens, self.k_tokens = int(ql.sum()), int(kl.sum())
         size = ctypes.c_size_t()
@@ -305,10 +315,26 @@ class PackedPlan:
             words = np.empty(size.value // 4, dtype=np.int32)
         check(rc, "swv_packed_plan")
         self._host = words[: size.value // 4].copy()
+        self._upload()
+
+    @staticmethod
+    def _not_captured(device):
+        if device.type == "cuda" and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise SwvError("make the plan before the capture: its tables are copied from the host")
+
+    def _upload(self):
         self._table = torch.from_numpy(self._host).to(self.device)      # (waits for the copy: any stream may use it)
         self._call = (self._host.ctypes.data, self._table.data_ptr())
         self._stream = _raw_stream(self.device.index) if self.device.type == "cuda" else 0
         self._bytes = {}
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_table", "_call", "_stream", "_bytes")}
+
+    def __setstate__(self, state):                        # (a copied or unpickled plan has tables of its own)
+        self.__dict__.update(state)
+        self._not_captured(self.device)
+        self._upload()
 
     def _used(self):
         """The tables are read on the current stream: their memory is not given to others before that is through."""

@@ -1,6 +1,8 @@
 """Host side of the packed operators, without a GPU: what the kernels' launches rely on, and calls at the edges of what is
 taken."""
+import copy
 import os
+import pickle
 import re
 
 import pytest
@@ -55,3 +57,24 @@ def test_every_row_of_a_divided_unit_sees_a_key(swv, ql, kl, H, Hkv):
     units = w[w[8]:w[8] + 8 * w[9]].reshape(-1, 8)
     for t0, n, s0, ln, off, b0, b1, slot in units.tolist():
         assert slot < 0 or min(ln, off + 1) > 0
+
+
+COPIES = [copy.copy, copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))]
+
+
+@pytest.mark.parametrize("make", COPIES)
+def test_copied_handles_hold_addresses_of_their_own(swv, make):
+    """Copies of a rotary handle, of a plan and of a module that holds one pass addresses of what they own themselves, with the
+    same contents: they outlive the original."""
+    rope = swv.RopeAxes(64, (8, 12, 12), scales=(1.0, 0.5, 0.25), pairing="halves")
+    plan = swv.PackedPlan([5, 600], [70, 900], heads=4, kv_heads=2, causal=True, device="cpu")
+    net = swv.PackedViTSlideEncoder(in_features=8, embed_dim=64, num_heads=2, num_layers=1, rope_sections=(4, 4))
+    r, p, n = make(rope), make(plan), make(net)
+    for a, b in ((r, rope), (n.rope, net.rope)):
+        assert a._call[:2] == (a._freq.ctypes.data, a._axis.ctypes.data) and a._call[2:] == b._call[2:]
+        assert (a._freq == b._freq).all() and (a._axis == b._axis).all() and a._axis.dtype == b._axis.dtype
+    assert p._call == (p._host.ctypes.data, p._table.data_ptr()) and torch.equal(p._table, plan._table)
+    assert (p.q_tokens, p.k_tokens, p.heads, p.kv_heads, p.causal, p.device) == (605, 970, 4, 2, True, plan.device)
+    assert p._workspace_bytes(64) == plan._workspace_bytes(64)
+    for a, b in ((r, rope), (p, plan)):                           # no address of the original, unless its memory is shared
+        assert make is copy.copy or a._call[0] != b._call[0]

@@ -1,7 +1,11 @@
 """Packed operators on a B200 at the edges of what they take: scores of -inf, copies of handles, buffers inside an arena, derivatives
 that the kernels do not have.  Bounds and references are those of the operators' other tests."""
+import copy
+import gc
 import math
+import pickle
 
+import numpy as np
 import pytest
 import torch
 
@@ -70,3 +74,16 @@ def test_attention_rows_of_infinite_scores_alone_are_nan(swv, lq, lk):
     k[:, :, 0] = -math.inf
     o, lse = swv.packed_attention(q, k, v, swv.PackedPlan([lq], [lk], heads=2, kv_heads=1), return_lse=True)
     assert bool(torch.isnan(o).all()) and bool(torch.isnan(lse).all())
+
+
+@pytest.mark.parametrize("make", [copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))])
+def test_copied_handles_outlive_the_original(swv, make):
+    q, k, v, _ = _inputs(300, 300, 4, 2, 64, 7)
+    pos = torch.randint(0, 900, (300, 3), device="cuda")
+    rope, plan = swv.RopeAxes(64, (8, 12, 12)), swv.PackedPlan([100, 200], heads=4, kv_heads=2)
+    want = swv.packed_attention(swv.rope_axes(q, pos, rope), k, v, plan)
+    r, p = make(rope), make(plan)
+    del rope, plan
+    gc.collect()
+    junk = [np.full(n, 7.0) for n in (4, 8, 32, 64, 1024) for _ in range(50)]
+    assert torch.equal(swv.packed_attention(swv.rope_axes(q, pos, r), k, v, p), want) and len(junk) == 250
