@@ -6,8 +6,8 @@ behind the other in token-major tensors, without padding.
   rope_axes        : rotary positions with up to eight axes (for example level, row and column of a patch)
   layer_norm       : layer norm over the last dimension
 
-All of them are differentiable once, run on the current CUDA stream of the inputs' device and raise ``SwvError`` for
-calls that the kernels do not serve.  The reference's dense ViT-5 has the same pieces for one slide at a time
+All of them are differentiable once (in reverse mode; dual tensors of ``torch.autograd.forward_ad`` are refused), run on the
+current CUDA stream of the inputs' device and raise ``SwvError`` for calls that the kernels do not serve.  The reference's dense ViT-5 has the same pieces for one slide at a time
 (src/sparse_wsi_vit/models/vit_5/models_vit5.py:72-115, rope.py:72-97).
 """
 from __future__ import annotations
@@ -17,6 +17,7 @@ import functools
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import SwvError, check, lib
 from .ops import _CHECK, _require_cuda, check_status, status_word
@@ -47,6 +48,12 @@ def _same_device(first, *ts):
     for t in ts:
         if t is not None and t.device != dev:
             raise SwvError("all tensors of a call must be on one device")
+
+
+def _no_tangent(*ts):
+    """A dual tensor asks for a derivative without ``requires_grad``: the result would silently have none."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise SwvError("forward-mode differentiation is not supported: the operators have reverse-mode gradients only")
 
 
 def _check_out(out, like, inputs, same=None):
@@ -124,6 +131,7 @@ class LayerNormFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _no_tangent(dy)
         x, weight, stats = ctx.saved_tensors
         E, dev = x.shape[-1], x.device
         x2, dy2 = _rows2d(x), _rows2d(dy)
@@ -158,6 +166,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     sums are fp32.  ``out_dtype``: x's type (the default) or fp32, for an fp32 ``x`` any of the three.  Rows may be evenly
     spaced views; other layouts are copied."""
     _same_device(x, weight, bias)
+    _no_tangent(x, weight, bias)
     dt = x.dtype
     out_dtype = out_dtype or dt
     if dt not in _DTYPES or out_dtype not in _DTYPES:
@@ -244,6 +253,7 @@ class RopeAxesFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _no_tangent(g)
         return _rope_apply(g, ctx.saved_tensors[0], ctx.rope, True), None, None
 
 
@@ -252,6 +262,7 @@ def rope_axes(x, positions, rope, out=None):
     ``rope`` (a ``RopeAxes``) says.  The queries and keys of a fused projection turn in one call as its leading heads.
     ``out``: where to write, exactly ``x`` or memory of its own (inference only)."""
     _same_device(x, positions)
+    _no_tangent(x, positions, out)
     if x.dim() != 3 or x.shape[2] != rope.head_dim:
         raise SwvError(f"x has shape {tuple(x.shape)}, expected (tokens, heads, {rope.head_dim})")
     if x.shape[1] < 1:
@@ -422,6 +433,7 @@ class PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, _):
+        _no_tangent(d_out)
         q, k, v, o, lse = ctx.saved_tensors
         plan, dev, D = ctx.plan, q.device, q.shape[2]
         q, k, v, d_out = _aligned(q), _aligned(k), _aligned(v), _aligned(d_out)
@@ -453,6 +465,7 @@ def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
     inside a causal one it can reach rows that do not see it (a masked pair is multiplied with zero): from a value row
     the results, from any input the gradients."""
     _attn_check(q, k, v, plan)
+    _no_tangent(q, k, v, out)
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     if not 2.0 ** -60 <= scale <= 2.0 ** 60:
         raise SwvError("scale must be positive, between 2^-60 and 2^60")

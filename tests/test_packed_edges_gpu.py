@@ -8,6 +8,7 @@ import pickle
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from .test_packed_gpu import _close, reference
 
@@ -87,3 +88,31 @@ def test_copied_handles_outlive_the_original(swv, make):
     gc.collect()
     junk = [np.full(n, 7.0) for n in (4, 8, 32, 64, 1024) for _ in range(50)]
     assert torch.equal(swv.packed_attention(swv.rope_axes(q, pos, r), k, v, p), want) and len(junk) == 250
+
+
+def test_dual_tensors_are_refused(swv):
+    """Forward-mode derivatives do not exist: a dual input, parameter, buffer or upstream gradient is refused instead of losing its
+    tangent; plain tensors are served inside a dual level as outside."""
+    E = swv._lib.SwvError
+    q, k, v, do = _inputs(20, 20, 4, 2, 64, 8)
+    plan, rope, pos = swv.PackedPlan([20], heads=4, kv_heads=2), swv.RopeAxes(64, (16, 16)), torch.rand(20, 2, device="cuda")
+    w, b = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+    ops = [(swv.layer_norm, (q, w, b)), (lambda x, p: swv.rope_axes(x, p, rope), (q, pos)),
+           (lambda *a: swv.packed_attention(*a, plan), (q, k, v))]
+    want = [f(*a) for f, a in ops]
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for (f, a), y in zip(ops, want):
+            assert torch.equal(f(*a), y)
+            for i in range(len(a)):
+                for grad in (False, True):
+                    t = a[i].detach().requires_grad_(grad and a[i] is not pos)
+                    with pytest.raises(E, match="forward-mode"):
+                        f(*a[:i], dual(t), *a[i + 1:])
+            x = a[0].detach().requires_grad_()
+            with pytest.raises(E, match="forward-mode"):
+                torch.autograd.grad(f(x, *a[1:]), x, dual(do))
+        for call in (lambda o: swv.rope_axes(q, pos, rope, out=o), lambda o: swv.packed_attention(q, k, v, plan, out=o)):
+            with pytest.raises(E, match="forward-mode"):
+                call(dual(torch.empty_like(q)))
+    assert all(torch.equal(f(*a), y) for (f, a), y in zip(ops, want))
