@@ -56,9 +56,28 @@ def _no_tangent(*ts):
         raise SwvError("forward-mode differentiation is not supported: the operators have reverse-mode gradients only")
 
 
+def _reach(shape, strides):
+    """Elements from the first to behind the last one."""
+    return 1 + sum((n - 1) * s for n, s in zip(shape, strides)) if all(shape) else 0
+
+
+def _apart(a, b):
+    """No byte of the two is shared: one ends before the other begins, or their rows (first dimension) are equally far apart and
+    they lie in different columns, as the heads of one projection do."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    if a0 + _reach(a.shape, a.stride()) * a.itemsize <= b0 or b0 + _reach(b.shape, b.stride()) * b.itemsize <= a0:
+        return True
+    row = a.stride(0) * a.itemsize
+    if row == 0 or row != b.stride(0) * b.itemsize:
+        return False
+    between = (b0 - a0) % row
+    return (_reach(a.shape[1:], a.stride()[1:]) * a.itemsize <= between and
+            between + _reach(b.shape[1:], b.stride()[1:]) * b.itemsize <= row)
+
+
 def _check_out(out, like, inputs, same=None):
-    """An output buffer of the caller: no part of an autograd graph, and no memory of the inputs (``same``: or exactly
-    that one).  Its version is raised, so that a graph that has saved it notices."""
+    """An output buffer of the caller: no part of an autograd graph, no element twice, and no memory of the inputs (``same``: or
+    exactly that one)."""
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise SwvError("out must have the result's shape, type and device")
     if out.requires_grad:
@@ -69,11 +88,9 @@ def _check_out(out, like, inputs, same=None):
             if n > 1 and s < reach:
                 raise SwvError("out must not hold an element twice")
             reach += (n - 1) * s
-    if same is None or out.data_ptr() != same.data_ptr() or out.stride() != same.stride():
-        mine = out.untyped_storage().data_ptr()
-        if any(t.untyped_storage().data_ptr() == mine for t in inputs):
+    for t in inputs:
+        if not (t is same and out.data_ptr() == t.data_ptr() and out.stride() == t.stride()) and not _apart(out, t):
             raise SwvError("out must not share memory with the inputs")
-    torch.autograd.graph.increment_version(out)
 
 
 # --------------------------------------------------------------------------- #
@@ -260,7 +277,8 @@ class RopeAxesFunction(torch.autograd.Function):
 def rope_axes(x, positions, rope, out=None):
     """Turns the heads ``x (T, H, head_dim)`` (fp32, bf16 or fp16) by ``positions (T, axes)`` (fp32, int32 or int64) as
     ``rope`` (a ``RopeAxes``) says.  The queries and keys of a fused projection turn in one call as its leading heads.
-    ``out``: where to write, exactly ``x`` or memory of its own (inference only)."""
+    ``out``: where to write (inference only), exactly ``x`` or elements that no input holds; those of a row may lie beside the inputs'
+    in one buffer."""
     _same_device(x, positions)
     _no_tangent(x, positions, out)
     if x.dim() != 3 or x.shape[2] != rope.head_dim:
@@ -281,9 +299,10 @@ def rope_axes(x, positions, rope, out=None):
     if out is not None:
         if grad:
             raise SwvError("rope_axes writes into `out` only where no gradient is asked for")
+        _check_out(out, x, (x, positions), same=x)
         if out.stride(2) != 1:
             raise SwvError("out must have unit inner stride")
-        _check_out(out, x, (x, positions), same=x)
+        torch.autograd.graph.increment_version(out)       # (a graph that has saved it notices)
     return RopeAxesFunction.apply(x, positions, rope) if grad else _rope_apply(x, positions, rope, False, out)
 
 
@@ -461,7 +480,8 @@ def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
     projection are read as they are if their rows lie on 16 bytes); ``plan``: the batch's ``PackedPlan``; ``scale``
     defaults to 1 / sqrt(D).  Returns ``(Tq, heads, D)`` bf16, with ``return_lse`` also the rows' log-sum-exp (heads, Tq)
     fp32, which has no gradient.  A row that sees no key is zero (lse -inf), and so are rows behind the last
-    sequence; with ``out`` (inference only) those are left as they were.  A NaN or an infinity never leaves its sequence;
+    sequence; with ``out`` (inference only; elements that no input holds, for example other heads of one buffer) those are left as
+    they were.  A NaN or an infinity never leaves its sequence;
     inside a causal one it can reach rows that do not see it (a masked pair is multiplied with zero): from a value row
     the results, from any input the gradients."""
     _attn_check(q, k, v, plan)
@@ -476,5 +496,6 @@ def packed_attention(q, k, v, plan, scale=None, return_lse=False, out=None):
         _check_out(out, q, (q, k, v))
         if not _rows_ok(out):
             raise SwvError("out must have rows on 16 bytes")
+        torch.autograd.graph.increment_version(out)
     o, lse = PackedAttentionFunction.apply(q, k, v, plan, scale) if grad else _attn_fwd(q, k, v, plan, scale, return_lse, out)
     return (o, lse) if return_lse else o

@@ -78,3 +78,41 @@ def test_copied_handles_hold_addresses_of_their_own(swv, make):
     assert p._workspace_bytes(64) == plan._workspace_bytes(64)
     for a, b in ((r, rope), (p, plan)):                           # no address of the original, unless its memory is shared
         assert make is copy.copy or a._call[0] != b._call[0]
+
+
+def test_output_buffers_beside_the_inputs(swv):
+    """A part of the inputs' buffer that holds none of their elements is taken; any shared element is refused, and so is a buffer
+    of another number of dimensions."""
+    from sparse_wsi_vit_b200.packed import _check_out
+    E = swv._lib.SwvError
+    arena = torch.zeros(4000)
+    x = arena[:640].view(10, 4, 16)
+    _check_out(arena[640:1280].view(10, 4, 16), x, (x,))
+    _check_out(x, x, (x,), same=x)
+    for bad in (arena[639:1279].view(10, 4, 16), arena[16:656].view(10, 4, 16), torch.zeros(640), torch.zeros(10, 64),
+                arena[:1280].view(20, 4, 16)[::2]):
+        with pytest.raises(E):
+            _check_out(bad, x, (x,))
+    with pytest.raises(E):
+        _check_out(x, x, (x,))
+    qkv = torch.zeros(10, 12, 16)
+    q, k, v = qkv[:, :4], qkv[:, 4:8], qkv[:, 8:]
+    for out, ins in ((q, (k, v)), (k, (q, v)), (v, (q, k))):
+        _check_out(out, out, ins)
+        with pytest.raises(E):
+            _check_out(out, out, ins + (out,))
+    with pytest.raises(E):
+        _check_out(qkv[:, 2:6], q, (q,))
+    with pytest.raises(E):
+        _check_out(q, q, (x, qkv[:, 3:5, 5]))
+    odd = torch.zeros(200 * 9 + 64).as_strided((9, 4, 16), (200, 16, 1))          # another row distance in the same memory
+    with pytest.raises(E):
+        _check_out(odd, odd, (odd.as_strided((9, 4, 16), (192, 16, 1), 64),))
+    pos = x[:, 0, :2]                                             # in place, but over the positions
+    with pytest.raises(E):
+        _check_out(x, x, (x, pos), same=x)
+    _check_out(torch.zeros(0, 4, 16), torch.zeros(0, 4, 16), (x,))
+    version = x._version
+    with pytest.raises(E):
+        _check_out(x, x, (x,))
+    assert x._version == version

@@ -116,3 +116,27 @@ def test_dual_tensors_are_refused(swv):
             with pytest.raises(E, match="forward-mode"):
                 call(dual(torch.empty_like(q)))
     assert all(torch.equal(f(*a), y) for (f, a), y in zip(ops, want))
+
+
+def test_results_written_beside_the_inputs(swv):
+    """Results in a buffer that holds the inputs too: behind them in an arena, and between the heads of a fused projection."""
+    q, k, v, _ = _inputs(300, 300, 4, 4, 64, 9)
+    plan, rope = swv.PackedPlan([100, 200], heads=4), swv.RopeAxes(64, (16, 16))
+    pos = torch.randint(0, 900, (300, 2), device="cuda")
+    want, turned = swv.packed_attention(q, k, v, plan), swv.rope_axes(k, pos, rope)
+    qkv = torch.cat([q, k, v, torch.zeros_like(q)], 1)            # four heads each
+    part = lambda i: qkv[:, 4 * i:4 * i + 4]
+    swv.packed_attention(part(0), part(1), part(2), plan, out=part(3))
+    assert torch.equal(part(3), want)
+    swv.rope_axes(part(1), pos, rope, out=part(0))
+    assert torch.equal(part(0), turned) and torch.equal(part(1), k) and torch.equal(part(2), v) and torch.equal(part(3), want)
+    arena = torch.cat([t.flatten() for t in (q, k, v, torch.zeros_like(q))]).view(4, 300, 4, 64)
+    swv.packed_attention(arena[0], arena[1], arena[2], plan, out=arena[3])
+    assert torch.equal(arena[3], want) and torch.equal(arena[2], v)
+    E = swv._lib.SwvError
+    for bad in (arena[0], qkv[:, 2:6], q.flatten(), q[0]):
+        with pytest.raises(E):
+            swv.packed_attention(part(0), arena[0], arena[2], plan, out=bad)
+    for x, bad in ((part(0), qkv[:, 1:5]), (part(0), qkv[:, 2:6]), (q, q.flatten()), (q, q[0])):
+        with pytest.raises(E):
+            swv.rope_axes(x, pos, rope, out=bad)
