@@ -421,8 +421,8 @@ __global__ void __launch_bounds__(1024) layer_norm_sum_kernel(const float* part,
 struct LnForm {
   int vec, tpr, iter;       // iter = 0: the form for wide rows
 };
-LnForm ln_form(int E, bool vec8, bool bwd, bool wide) {
-  LnForm f;
+constexpr LnForm ln_form(int E, bool vec8, bool bwd, bool wide) {
+  LnForm f{};
   f.vec = vec8 ? 8 : 1;
   if (f.vec == 1) f.tpr = E <= 1024 ? 32 : E <= 4096 ? 128 : 256;
   else if (!bwd && wide) f.tpr = std::min((E + 255) / 256 * 32, 256);
@@ -450,8 +450,33 @@ auto ln_kernel() {
   else return layer_norm_fwd_kernel<T, U, VEC, ITER, TPR>;
 }
 
+// The forms that are compiled: (values a run, runs, threads a row, where: `bwd` or `one`, one run a thread at any width).
+#define SWV_LN_FORMS(X, bwd, one)                                                                                         \
+  X(8, 1, 32, true) X(8, 2, 32, !one) X(8, 3, 32, !one) X(8, 4, 32, !one && !bwd) X(8, 5, 32, !one && !bwd)                \
+  X(8, 1, 64, one) X(8, 1, 96, one) X(8, 1, 128, one) X(8, 1, 160, one) X(8, 1, 192, one) X(8, 1, 224, one)                \
+  X(8, 1, 256, one) X(8, 2, 64, bwd) X(8, 3, 64, bwd) X(8, 2, 128, !one) X(8, 2, 256, true) X(8, 3, 256, true)             \
+  X(8, 4, 256, true) X(1, 8, 32, true) X(1, 32, 32, true) X(1, 32, 128, true) X(1, 32, 256, true)
+
+// Every row that has a form finds it among them.
+constexpr bool ln_compiled(const LnForm& f, bool bwd, bool one) {
+#define SWV_LN(V, I, R, USED) \
+  if (f.vec == V && f.iter == I && f.tpr == R) return USED;
+  SWV_LN_FORMS(SWV_LN, bwd, one)
+#undef SWV_LN
+  return f.iter == 0;
+}
+constexpr bool ln_all_compiled(bool vec8, bool bwd, bool one) {
+  for (int E = vec8 ? 8 : 1; E <= 9216; E += vec8 ? 8 : 1)
+    if (!ln_compiled(ln_form(E, vec8, bwd, one), bwd, one)) return false;
+  return true;
+}
+static_assert(ln_all_compiled(true, false, false) && ln_all_compiled(false, false, false), "a forward form is missing");
+static_assert(ln_all_compiled(true, false, true) && ln_all_compiled(false, false, true), "a forward form of fp32 rows is missing");
+static_assert(ln_all_compiled(true, true, false) && ln_all_compiled(false, true, false), "a backward form is missing");
+
 template <typename T, typename U, bool BWD>
 int ln_launch(const LnParams& p, const LnForm& f, int grid, cudaStream_t st) {
+  constexpr bool kOne = !BWD && sizeof(T) == 4;
 #define SWV_LN(V, I, R, USED)                                                                                \
   if (f.vec == V && f.iter == I && f.tpr == R) {                                                             \
     if constexpr (USED) {                                                                                    \
@@ -459,18 +484,15 @@ int ln_launch(const LnParams& p, const LnForm& f, int grid, cudaStream_t st) {
       auto k = ln_kernel<T, U, V, I, R, BWD>();                                                              \
       if (kSmem > 40 * 1024) SWV_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)); \
       SWV_CUDA_OK(launch_after(k, grid, kBlock, kSmem, st, p));                                              \
+      return SWV_OK;                                                                                         \
     }                                                                                                        \
-  } else
-  constexpr bool kOne = !BWD && sizeof(T) == 4;              // one run a thread at any width
-  SWV_LN(8, 1, 32, true) SWV_LN(8, 2, 32, !kOne) SWV_LN(8, 3, 32, !kOne) SWV_LN(8, 4, 32, !kOne && !BWD) SWV_LN(8, 5, 32, !kOne && !BWD)
-  SWV_LN(8, 1, 64, kOne) SWV_LN(8, 1, 96, kOne) SWV_LN(8, 1, 128, kOne) SWV_LN(8, 1, 160, kOne) SWV_LN(8, 1, 192, kOne)
-  SWV_LN(8, 1, 224, kOne) SWV_LN(8, 1, 256, kOne) SWV_LN(8, 2, 64, BWD) SWV_LN(8, 3, 64, BWD) SWV_LN(8, 2, 128, !kOne)
-  SWV_LN(8, 2, 256, true) SWV_LN(8, 3, 256, true) SWV_LN(8, 4, 256, true)
-  SWV_LN(1, 8, 32, true) SWV_LN(1, 32, 32, true) SWV_LN(1, 32, 128, true) SWV_LN(1, 32, 256, true) {
-    auto k = BWD ? layer_norm_wide_bwd_kernel<T, U> : layer_norm_wide_fwd_kernel<T, U>;
-    SWV_CUDA_OK(launch_after(k, grid, kLnThreads, 0, st, p));
+    return SWV_ERR_UNSUPPORTED;                                                                              \
   }
+  SWV_LN_FORMS(SWV_LN, BWD, kOne)
 #undef SWV_LN
+  if (f.iter != 0) return SWV_ERR_UNSUPPORTED;
+  auto k = BWD ? layer_norm_wide_bwd_kernel<T, U> : layer_norm_wide_fwd_kernel<T, U>;
+  SWV_CUDA_OK(launch_after(k, grid, kLnThreads, 0, st, p));
   return SWV_OK;
 }
 
