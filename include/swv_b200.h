@@ -405,6 +405,7 @@ int swv_rope2d_apply(const void* x, const int64_t x_strides[3], void* y, const i
  * backward pass needs them); w and b (E) may be NULL (1 and 0).  Rows x_stride / y_stride / ... elements apart, unit
  * inner stride.  x of any dtype; y (and dy) of x's dtype or SWV_F32, and of any dtype where x is SWV_F32; dx of
  * x's dtype; w, b, dw, db each of any dtype.
+ * E up to 2^29.
  * Backward: dx (N,E), dw and db (E), either may be NULL.  `workspace`: swv_layer_norm_bwd_bytes(), only for dw, db. */
 int swv_layer_norm_fwd(const void* x, int64_t x_stride, int x_dtype, const void* w, int w_dtype, const void* b,
                        int b_dtype, void* y, int64_t y_stride, int y_dtype, float* mean, float* rstd, int64_t N, int E,
@@ -419,7 +420,7 @@ int swv_layer_norm_bwd(const void* dy, int64_t dy_stride, int y_dtype, const voi
  * of the `pairs` rotated pairs of every head turns by  position[t][axis[i]] * freq[i]  (`inverse`: by minus that, the
  * gradient); the pairs are channels (2i, 2i+1), or with `halves` (i, pairs + i); the channels from 2*pairs on are
  * copied.  The angle is formed in 64 bits.  freq_host (pairs) f64 and axis_host (pairs) u8 are HOST arrays, read during
- * the call; pairs <= 128.
+ * the call; pairs <= 128, H and head_dim up to 2^29.
  *   x, y (T,H,head_dim): strides (t,h,d) with unit inner stride, y may be x;  positions (T,axes) of pos_dtype, rows
  *   pos_stride elements apart. */
 #define SWV_POS_F32 0
@@ -432,7 +433,7 @@ int swv_rope_axes_apply(const void* x, const int64_t x_strides[3], void* y, cons
 
 /* Attention over packed sequences (dense softmax attention inside each of n_seq sequences that lie one behind the
  * other; for one sequence F.scaled_dot_product_attention of the reference's dense ViT-5, models_vit5.py:101).
- * Query head h reads key head h / (H / Hkv), H / Hkv <= 128.  Causal: query i of a sequence of lq queries and lk keys
+ * Query head h reads key head h / (H / Hkv), H / Hkv <= 128, Hkv <= 65535.  Causal: query i of a sequence of lq queries and lk keys
  * sees the keys j <= i + lk - lq.  A row that sees no key gives zeros and lse = -inf.
  *
  * swv_packed_plan turns the lengths (HOST arrays) into the kernels' work tables: one int32 HOST array that the caller

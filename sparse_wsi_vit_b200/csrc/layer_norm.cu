@@ -21,6 +21,7 @@ namespace swv {
 namespace {
 
 constexpr int kLnThreads = 256;                              // forms of wide rows
+constexpr int kLnMaxE = 1 << 29;                             // columns and their loops stay within 32 bits
 // Threads of a CTA with runs of `run` values a thread and groups of `tpr` threads, and resident CTAs per SM.  Backward: three runs
 // of 8 take 168 registers a thread, two take 128.
 constexpr int ln_block(int tpr, int run, bool bwd) { return bwd && run == 24 && tpr <= 64 ? 384 : 256 / tpr * tpr; }
@@ -514,6 +515,7 @@ int ln_dispatch(const LnParams& p, int x_dtype, int y_dtype, const LnForm& f, in
 
 int ln_check(int64_t N, int E, int x_dtype, int y_dtype, const void* w, int w_dtype, const void* b, int b_dtype) {
   if (N < 0 || E < 1) return SWV_ERR_SHAPE;
+  if (E > kLnMaxE) return SWV_ERR_UNSUPPORTED;
   if (!dtype_known(x_dtype) || !dtype_known(y_dtype)) return SWV_ERR_DTYPE;
   if (x_dtype != SWV_F32 && y_dtype != x_dtype && y_dtype != SWV_F32) return SWV_ERR_DTYPE;
   if ((w != nullptr && !dtype_known(w_dtype)) || (b != nullptr && !dtype_known(b_dtype))) return SWV_ERR_DTYPE;
@@ -541,6 +543,7 @@ int layer_norm_fwd_impl(const void* x, int64_t xs, int x_dtype, const void* w, i
 int layer_norm_bwd_bytes_impl(int64_t N, int E, size_t* bytes) {
   if (!bytes) return SWV_ERR_NULL;
   if (N < 0 || E < 1) return SWV_ERR_SHAPE;
+  if (E > kLnMaxE) return SWV_ERR_UNSUPPORTED;
   *bytes = static_cast<size_t>(std::min<int64_t>(std::max<int64_t>(N, 1), static_cast<int64_t>(sm_count()) * kLnBwdCtas)) * 2 * E *
            sizeof(float);
   return SWV_OK;

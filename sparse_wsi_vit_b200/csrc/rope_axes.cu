@@ -147,7 +147,8 @@ int rope_axes_impl(const void* x, const int64_t* xs, void* y, const int64_t* ys,
                    int axes, int halves, int inverse, int64_t T, int H, int hd, cudaStream_t st) {
   if (!xs || !ys || !freq_host || !axis_host) return SWV_ERR_NULL;
   if (T < 0 || H < 1 || hd < 2 || pairs < 1 || 2 * pairs > hd || axes < 1) return SWV_ERR_SHAPE;
-  if (pairs > kMaxPairs || axes > kMaxAxes) return SWV_ERR_UNSUPPORTED;
+  // (heads, channels and the loops over them stay within 32 bits)
+  if (pairs > kMaxPairs || axes > kMaxAxes || H > (1 << 29) || hd > (1 << 29)) return SWV_ERR_UNSUPPORTED;
   if (!dtype_known(dtype) || pos_dtype < SWV_POS_F32 || pos_dtype > SWV_POS_I64) return SWV_ERR_DTYPE;
   if (T == 0) return SWV_OK;
   if (!x || !y || !pos) return SWV_ERR_NULL;

@@ -24,6 +24,7 @@ from .ops import _CHECK, _require_cuda, check_status, status_word
 
 _POS_CODES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MAX_DIM = 1 << 29                                       # of the dimensions that the library takes as 32-bit numbers
 _I3 = ctypes.c_int64 * 3
 _raw_stream = torch._C._cuda_getCurrentRawStream        # (torch.cuda.current_stream builds an object: 2 us a call)
 
@@ -190,6 +191,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
         raise SwvError(f"layer_norm takes float32, bfloat16 and float16, not {dt} -> {out_dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise SwvError("layer_norm needs a last dimension of one value or more")
+    if x.shape[-1] > _MAX_DIM:
+        raise SwvError(f"layer_norm takes rows of up to {_MAX_DIM} values, not {x.shape[-1]}")
     if out_dtype != dt and dt != torch.float32 and out_dtype != torch.float32:
         raise SwvError(f"layer_norm of {dt} gives {dt} or float32, not {out_dtype}")
     grad = x.requires_grad
@@ -283,8 +286,8 @@ def rope_axes(x, positions, rope, out=None):
     _no_tangent(x, positions, out)
     if x.dim() != 3 or x.shape[2] != rope.head_dim:
         raise SwvError(f"x has shape {tuple(x.shape)}, expected (tokens, heads, {rope.head_dim})")
-    if x.shape[1] < 1:
-        raise SwvError("rope_axes needs one head or more")
+    if not 1 <= x.shape[1] <= _MAX_DIM or x.shape[2] > _MAX_DIM:
+        raise SwvError(f"rope_axes takes one to {_MAX_DIM} heads and channels, not {tuple(x.shape[1:])}")
     if x.dtype not in _DTYPES:
         raise SwvError(f"rope_axes takes float32, bfloat16 and float16, not {x.dtype}")
     if positions.dtype not in _POS_CODES:
@@ -331,6 +334,8 @@ class PackedPlan:
         if len(ql) != len(kl):
             raise SwvError(f"{len(ql)} query lengths and {len(kl)} key lengths")
         self.heads, self.kv_heads, self.causal = int(heads), int(heads if kv_heads is None else kv_heads), bool(causal)
+        if self.heads > _MAX_DIM or self.kv_heads > 65535:
+            raise SwvError(f"up to 65535 key / value heads of up to 128 query heads each, not {self.heads} and {self.kv_heads}")
         device = torch.device(device)
         self._not_captured(device)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device

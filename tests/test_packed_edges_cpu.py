@@ -1,10 +1,12 @@
 """Host side of the packed operators, without a GPU: what the kernels' launches rely on, and calls at the edges of what is
 taken."""
 import copy
+import ctypes
 import os
 import pickle
 import re
 
+import numpy as np
 import pytest
 import torch
 
@@ -33,8 +35,7 @@ def _kernels(text):
 def test_every_kernel_that_starts_early_waits_in_every_thread():
     """A kernel launched close behind another one may read what earlier kernels of the stream wrote only behind a wait of its
     own: each has the wait as a statement of its outermost block, ahead of any release of the kernel behind it."""
-    import sparse_wsi_vit_b200 as m
-    csrc = os.path.join(os.path.dirname(m.__file__), "csrc")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sparse_wsi_vit_b200", "csrc")
     seen = 0
     for f in sorted(os.listdir(csrc)):
         text = open(os.path.join(csrc, f)).read() if f.endswith(".cu") else ""
@@ -116,3 +117,20 @@ def test_output_buffers_beside_the_inputs(swv):
     with pytest.raises(E):
         _check_out(x, x, (x,))
     assert x._version == version
+
+
+def test_sizes_beyond_32_bits_are_refused(swv):
+    """The library takes widths, heads and channels as 32-bit numbers and steps beyond them in loops."""
+    L, fake, n = swv._lib.lib, ctypes.c_void_p(0x1000), ctypes.c_size_t()
+    big = (1 << 29) + 1
+    for E in (big, (1 << 31) - 1):
+        assert L.swv_layer_norm_fwd(fake, E, 0, None, 0, None, 0, fake, E, 0, None, None, 1, E, 1e-5, None) == -8
+        assert L.swv_layer_norm_bwd_bytes(1, E, ctypes.byref(n)) == -8
+        assert L.swv_layer_norm_bwd(fake, E, 0, fake, E, 0, None, 0, fake, fake, fake, E, None, 0, None, 0, 1, E, None, 0, None) == -8
+    f, a, s3 = np.ones(4), np.zeros(4, dtype=np.uint8), (ctypes.c_int64 * 3)(16, 8, 1)
+    for H, hd in ((big, 8), (2, big), ((1 << 31) - 1, 8)):
+        assert L.swv_rope_axes_apply(fake, s3, fake, s3, 0, fake, 0, 1, f.ctypes.data, a.ctypes.data, 4, 1, 0, 0, 1, H, hd, None) == -8
+    for heads, kv in (((1 << 32) + 4, 4), ((1 << 32) + 4, (1 << 32) + 4), (65536, 65536)):
+        with pytest.raises(swv._lib.SwvError):
+            swv.PackedPlan([4], heads=heads, kv_heads=kv, device="cpu")
+    assert swv.PackedPlan([4], heads=65535, device="cpu").heads == 65535

@@ -140,3 +140,13 @@ def test_results_written_beside_the_inputs(swv):
     for x, bad in ((part(0), qkv[:, 1:5]), (part(0), qkv[:, 2:6]), (q, q.flatten()), (q, q[0])):
         with pytest.raises(E):
             swv.rope_axes(x, pos, rope, out=bad)
+
+
+@pytest.mark.parametrize("n", [(1 << 29) + 8, (1 << 32) + 8])
+def test_sizes_beyond_32_bits_are_refused(swv, n):
+    """Ahead of any copy or launch: a width or a number of heads that the library would take modulo 2^32."""
+    one = torch.zeros(1, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(swv._lib.SwvError):
+        swv.layer_norm(one.expand(1, n))
+    with pytest.raises(swv._lib.SwvError):
+        swv.rope_axes(one.expand(1, n, 8), torch.zeros(1, 1, device="cuda"), swv.RopeAxes(8, (4,)))
