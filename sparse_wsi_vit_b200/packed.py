@@ -452,11 +452,14 @@ class PackedAttentionFunction(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, o, lse)
         ctx.plan, ctx.scale = plan, scale
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)                  # (no (heads, Tq) zeros for lse in every backward pass)
         return o, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, _):
+        if d_out is None:
+            return None, None, None, None, None
         _no_tangent(d_out)
         q, k, v, o, lse = ctx.saved_tensors
         plan, dev, D = ctx.plan, q.device, q.shape[2]

@@ -150,3 +150,19 @@ def test_sizes_beyond_32_bits_are_refused(swv, n):
         swv.layer_norm(one.expand(1, n))
     with pytest.raises(swv._lib.SwvError):
         swv.rope_axes(one.expand(1, n, 8), torch.zeros(1, 1, device="cuda"), swv.RopeAxes(8, (4,)))
+
+
+def test_attention_backward_gets_no_gradient_of_lse(swv, monkeypatch):
+    """lse has no gradient: none is made up for it (a tensor of zeros and a launch in every backward pass)."""
+    from sparse_wsi_vit_b200.packed import PackedAttentionFunction as F
+    seen, real = [], F.backward
+    monkeypatch.setattr(F, "backward", staticmethod(lambda ctx, *g: seen.append(g) or real(ctx, *g)))
+    q, k, v, do = _inputs(40, 40, 4, 2, 64, 10)
+    plan = swv.PackedPlan([40], heads=4, kv_heads=2)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    for lse in (False, True):
+        o = swv.packed_attention(*leaves, plan, return_lse=lse)
+        grads = torch.autograd.grad(o[0] if lse else o, leaves, do)
+        assert all(g is not None for g in grads)
+    assert len(seen) == 2 and all(g[0] is not None and g[1] is None for g in seen)
+    assert real(None, None, None) == (None,) * 5
