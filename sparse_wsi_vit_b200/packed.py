@@ -362,6 +362,8 @@ class PackedPlan:
         self._call = (self._host.ctypes.data, self._table.data_ptr())
         self._stream = _raw_stream(self.device.index) if self.device.type == "cuda" else 0
         self._bytes = {}
+        if self.device.type == "cuda":
+            status_word(self.device)                      # (made in a capture, it would be the graph's: zeroed by every replay)
 
     def __getstate__(self):
         return {k: v for k, v in self.__dict__.items() if k not in ("_table", "_call", "_stream", "_bytes")}

@@ -166,3 +166,21 @@ def test_attention_backward_gets_no_gradient_of_lse(swv, monkeypatch):
         assert all(g is not None for g in grads)
     assert len(seen) == 2 and all(g[0] is not None and g[1] is None for g in seen)
     assert real(None, None, None) == (None,) * 5
+
+
+def test_first_attention_call_inside_a_capture(swv, monkeypatch):
+    """The status word exists before the capture (the plan makes it): it is zero ahead of the first replay, and a replay does not
+    clear what another launch has recorded."""
+    from sparse_wsi_vit_b200 import ops
+    monkeypatch.setattr(ops, "_status", {})
+    q, k, v, _ = _inputs(40, 40, 4, 2, 64, 11)
+    plan = swv.PackedPlan([40], heads=4, kv_heads=2)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = swv.packed_attention(q, k, v, plan)
+    word = ops.status_word(q.device)
+    assert int(word) == 0
+    word.fill_(101)
+    g.replay()
+    assert int(word) == 101 and torch.equal(o, swv.packed_attention(q, k, v, plan))
+    word.zero_()
