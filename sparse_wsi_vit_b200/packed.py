@@ -235,7 +235,10 @@ class RopeAxes:
         self.head_dim, self.sections, self.pairs, self.halves = int(head_dim), tuple(sections), R, pairing == "halves"
         power = [(sum(sections[:a]) + i) / R if ladder == "head" else i / n for a, n in enumerate(sections) for i in range(n)]
         self._axis = np.repeat(np.arange(len(sections)), sections).astype(np.uint8)
-        self._freq = np.asarray(scales)[self._axis] * np.float64(theta) ** -np.asarray(power, dtype=np.float64)
+        with np.errstate(over="ignore"):
+            self._freq = np.asarray(scales)[self._axis] * np.float64(theta) ** -np.asarray(power, dtype=np.float64)
+        if not np.isfinite(self._freq).all():
+            raise SwvError(f"the frequencies pass the range of 64 bits: theta {theta}, scales {scales}")
         self._bind()
 
     def _bind(self):

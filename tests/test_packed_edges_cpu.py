@@ -134,3 +134,9 @@ def test_sizes_beyond_32_bits_are_refused(swv):
         with pytest.raises(swv._lib.SwvError):
             swv.PackedPlan([4], heads=heads, kv_heads=kv, device="cpu")
     assert swv.PackedPlan([4], heads=65535, device="cpu").heads == 65535
+
+
+def test_rotary_frequencies_are_finite(swv):
+    with pytest.raises(swv._lib.SwvError):
+        swv.RopeAxes(64, (32,), theta=1e-300, scales=(1e300,))
+    assert swv.RopeAxes(64, (32,), theta=1e-300)._freq[-1] > 1e280
