@@ -81,12 +81,10 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     if (_e != cudaSuccess) return SWV_ERR_CUDA;             \
   } while (0)
 
-// Number of SMs of the current device (cached), used to decide when a small grid should divide
-// the key range; 148 (B200) when no device can be asked, e.g. a size query on a machine without one.
-// Launches that follow one another closely: the next kernel of a stream may start (set up its barriers, its TMEM, its
-// weights) while the last CTAs of the one before it run.  grid_wait: everything that the stream's earlier kernels wrote is
-// there.  A kernel launched with launch_after executes it before it touches memory that an earlier kernel may still read or
-// write, and in any case before it ends, so that its end stands for theirs.  grid_release: the CTA has no objection to the next one's start.
+// Launches that follow one another closely: the next kernel of a stream may be launched (and set up what needs no memory) while
+// the last CTAs of the one before it run.  grid_wait: everything that the stream's earlier kernels wrote is there.  Every
+// thread of a kernel launched with launch_after executes it, before it touches memory that an earlier kernel may still read or
+// write (weights too), so that the kernel's end stands for theirs.  grid_release: the CTA has no objection to the next one's start.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -105,6 +103,8 @@ cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t sme
   return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
 }
 
+// Number of SMs of the current device (cached), used to decide when a small grid should divide
+// the key range; 148 (B200) when no device can be asked, e.g. a size query on a machine without one.
 inline int sm_count() {
   static int cached = 0;
   if (cached > 0) return cached;

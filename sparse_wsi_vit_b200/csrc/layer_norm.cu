@@ -416,9 +416,16 @@ __global__ void __launch_bounds__(1024) layer_norm_sum_kernel(const float* part,
 // elements otherwise.  Runs of 8: few threads with several runs each, as many as the registers hold, so that few warps meet at a
 // barrier and few lanes idle behind the row's end.  Forward, 16-bit rows: a warp up to 1280 values (32768 x 1280: 30 us, four
 // warps 38, five 40), then two runs a thread (16384 x 2048: 25.5 us, one run 33); fp32 rows, twice the registers: one run a
-// thread (4099 x 1280: 11.5 us, two runs 15.7).  Backward: two runs (x, dy, dw and db of 16 values) in 128 registers, or
+// thread (4099 x 1280: 11.5 us, two runs 15.7; it loses where there are many rows: 19531 x 1280 52 us, three warps with two runs 35;
+// 65104 x 384 46, a warp with two runs 35).  Backward: two runs (x, dy, dw and db of 16 values) in 128 registers, or
 // three in 168 where they fit the row better (65536 x 768: 56 us, two warps with two runs 65; 32768 x 1280: 52 us, four warps 65);
-// four runs spill (32768 x 1024: 55 us, two warps with two runs 38.5).  Beyond 8192 values the form that reads the row again.
+// four runs take one CTA an SM instead of two (48828 x 1024: 61 us, two warps with two runs 57).  Beyond 8192 values the form that reads the row again.
+// Both sides of the edges, 50 million bf16 values, us (the rule's form first).  Forward: 1280, a warp 35.3, 128 threads 43.6; 1288,
+// 128 threads 44.7, two warps with three runs 37.6; 1536, 39.0 and 35.8; 2048, 128 threads with two runs 35.4, 256 with one 54.0; 2056,
+// 256 with two 56.7, 128 with three 42.5.  Backward: 768, a warp 56.3, two with two runs 65.0; 776, two warps 66.0, one with four
+// runs 66.8; 1536, two warps with three runs 57.6, 128 threads 65.3; 1544, 128 threads 67.2, two warps with four runs 67.1; 2048, 58.4 and
+// 61.2; 2056, 256 threads 86.9, 128 with three runs 81.3.  So from 1288 to 1536 and behind 2048 another form would be 1.05 to 1.3
+// times as fast.
 struct LnForm {
   int vec, tpr, iter;       // iter = 0: the form for wide rows
 };

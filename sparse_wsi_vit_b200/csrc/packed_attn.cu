@@ -22,8 +22,9 @@
 //       D = 64:  S_A, S_B [0,256), P_A, P_B [256,384), O_A [384,448), O_B [448,512)
 //
 // Bound: the exponential unit (16 per clock and SM) at D = 64, it and the tensor pipe alike at D = 128; both are 63 % busy, by the
-// chain scores -> maximum -> exponentials -> P V of two tiles.  16387 tokens in 5 sequences, 12 heads of 64: 433 us, 0.73 PFLOP/s;
-// 15292 causal tokens in 4 sequences, 16 heads of 128 sharing two key heads: 314 us, 1.2 PFLOP/s.
+// chain scores -> maximum -> exponentials -> P V of two tiles.  16387 tokens in 5 sequences, 12 heads of 64: 437 us, 0.72 PFLOP/s;
+// 15292 causal tokens in 4 sequences, 16 heads of 128 sharing two key heads: 316 us, 1.2 PFLOP/s (in runs of many calls the card's
+// power limit makes it 360, 1.05 PFLOP/s).
 #include <algorithm>
 #include <cmath>
 #include <cstring>

@@ -21,9 +21,9 @@
 // (16-bit operands: each entry is off by at most 2^-8); S's columns are free as soon as it is in registers, so the next tile's
 // products are formed meanwhile.
 //
-// Bound: the tensor pipe, 44 to 66 % busy, and the threads that issue to it (one is blocked 75 to 95 cycles an instruction, which
-// is why there are two).  8188 tokens in 3 sequences, 12 heads of 64: keys' side 245 us, queries' side 204 us; 8192 causal tokens,
-// 16 heads of 128 sharing two key heads: 440 and 362 us.
+// Bound: the tensor pipe, 48 (D = 64) and 66 % (D = 128) busy, and the threads that issue to it (one is blocked 75 to 95 cycles an
+// instruction, which is why there are two).  Both sides: 8188 tokens in 3 sequences, 12 heads of 64: 471 us; 8192 causal tokens,
+// 16 heads of 128 sharing two key heads: 780 us.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

@@ -9,7 +9,9 @@
 // bits a coordinate of 10^5 would leave an error of 4e-3 in the angle.  One such angle serves a pair of all heads.
 //
 // A thread owns 8 channels of a token (4 or 8 pairs) and walks over heads; where the tokens are few, the heads are divided
-// over the grid.  Bound: HBM, every element read and written once (24576 tokens, 24 heads of 64 bf16: 24.6 us, 6.1 TB/s).
+// over the grid.  Bound: HBM, every element read and written once (24576 tokens, 24 heads of 64 bf16: 30 us in a run of launches on
+// different buffers, 5.0 TB/s; 27 where one pair of buffers stays in part in L2; 24.6 for a launch by itself, whose last writes
+// are still in L2 at its end).
 #include <algorithm>
 #include <type_traits>
 
